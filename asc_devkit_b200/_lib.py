@@ -13,7 +13,7 @@ LIB_PATH = os.path.join(_PKG, "libascq.so")
 OK, ERR_INVALID_ARG, ERR_UNSUPPORTED, ERR_ALIGNMENT, ERR_CUDA, ERR_NCCL, ERR_TIMEOUT = range(7)
 # ascq_dtype
 (DT_F16, DT_BF16, DT_F32, DT_I8, DT_I32, DT_U64, DT_FP4X2_E2M1, DT_E8M0, DT_FP8_E4M3, DT_FP8_E5M2, DT_HIF8,
- DT_FP4X2_E1M2, DT_I4X2) = range(13)
+ DT_FP4X2_E1M2, DT_I4X2, DT_I64) = range(14)
 # ascq_policy
 PER_TENSOR, PER_CHANNEL, PER_TOKEN, PER_GROUP, PER_CHANNEL_PER_GROUP, PER_TOKEN_PER_GROUP = range(6)
 # ascq_round
@@ -41,6 +41,11 @@ class QuantizeParam(C.Structure):
                 ("kDim", C.c_int32), ("roundMode", C.c_int)]
 
 
+class RmsNormParam(C.Structure):
+    _fields_ = [("m", C.c_uint32), ("n", C.c_uint32), ("epsilon", C.c_float), ("ldSrc", C.c_int64), ("ldResidual", C.c_int64),
+                ("ldResidualOut", C.c_int64), ("ldNormOut", C.c_int64)]
+
+
 class AscqError(RuntimeError):
     def __init__(self, status: int, message: str):
         super().__init__(f"{status_string(status)}: {message}")
@@ -59,6 +64,7 @@ SIGNATURES = {
     "ascq_quant": (_i, [_vp, _i, _vp, _i, _vp, _vp, _i, _f, _f, _i, C.POINTER(QuantParam), _vp]),
     "ascq_dynamic_quant_per_token": (_i, [_vp, _vp, _vp, _vp, _i, _u32, _u32, _vp]),
     "ascq_dynamic_quant_mxfp4": (_i, [_vp, _vp, _vp, _i, _u32, _u32, _vp]),
+    "ascq_residual_rms_norm_quant": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, C.POINTER(RmsNormParam), _vp]),
     "ascq_dequant": (_i, [_vp, _i, _vp, _i, _vp, _vp, _i, _f, _i, C.POINTER(DequantParam), _vp]),
     "ascq_antiquant": (_i, [_vp, _i, _vp, _i, _vp, _vp, _i, _f, _f, _i, C.POINTER(AntiQuantParam), _vp]),
    "ascq_quantize": (_i, [_vp, _i, _vp, _i, _vp, _vp, _i, _f, _f, _i, C.POINTER(QuantizeParam), _vp]),
@@ -92,6 +98,10 @@ SIGNATURES = {
     "ascq_set_wait_limit_cycles": (_i, [C.c_longlong]),
     "ascq_test_withhold_after": (_i, [_i]),
     "ascq_measure_tensor_rate": (_i, [_i, _i, C.POINTER(C.c_double), _vp]),
+    "ascq_expert_sort": (_i, [_vp, _vp, _vp, _vp, _i, C.c_int64, _i, _vp]),
+    "ascq_expert_dispatch": (_i, [_vp, _vp, C.c_size_t, C.c_size_t, _vp, _vp, C.c_size_t, _vp, C.c_int64, _i, C.c_int64, _vp]),
+    "ascq_expert_combine": (_i, [_vp, _vp, _i, _vp, _vp, C.c_int64, _i, C.c_int64, C.c_int64, _vp]),
+    "ascq_expert_combine_grad": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _vp, C.c_int64, _i, C.c_int64, C.c_int64, _vp]),
     "ascq_group_matmul_mxfp4": (_i, [_vp, _vp, _vp, _vp, _vp, _P64, _i, _i, _i, _vp, C.c_size_t, _vp]),
     "ascq_group_matmul_mxfp4_scatter": (_i, [C.POINTER(_vp), _i, _i, _P64, _vp, _vp, _vp, _vp, _P64, _i, _i, _i, _vp, C.c_size_t, _vp]),
     "ascq_group_matmul_mxfp8": (_i, [_vp, _i, _vp, _i, _vp, _vp, _i, _vp, _P64, _i, _i, _i, _vp, C.c_size_t, _vp]),

@@ -24,12 +24,19 @@ inline int dtype_size(ascq_dtype t)
         case ASCQ_DT_F32: case ASCQ_DT_I32: return 4;
         case ASCQ_DT_I8: case ASCQ_DT_E8M0: case ASCQ_DT_FP4X2_E2M1: case ASCQ_DT_FP4X2_E1M2:
         case ASCQ_DT_FP8_E4M3: case ASCQ_DT_FP8_E5M2: case ASCQ_DT_HIF8: case ASCQ_DT_I4X2: return 1;
-        case ASCQ_DT_U64: return 8;
+        case ASCQ_DT_U64: case ASCQ_DT_I64: return 8;
     }
     return 0;
 }
 // Defined in gemm_mxfp4.cu: reads and clears that kernel's device status word (synchronises the stream).
 ascq_status mxfp4_read_status(::CUstream_st* stream);
+
+// Whether [a, a + an) and [b, b + bn) share a byte (an empty or absent range shares none).
+inline bool spans_overlap(const void* a, size_t an, const void* b, size_t bn)
+{
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a && b && an && bn && x < y + bn && y < x + an;
+}
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

@@ -1,0 +1,530 @@
+// Tokens into expert order and back, around the grouped matmuls:
+//   sort      slots (token t, choice j: slot t * k + j) ordered by expert, equal experts in slot order; rows per expert
+//   dispatch  rows[rowOfSlot[s]] = src[s / k]                      (any element type; per-token scales alongside)
+//   combine   out[t] = sum_j w[t, j] * rows[rowOfSlot[t, j]]       (fp32, j ascending; without weights: the gradient of dispatch)
+//   gradient  dRows[rowOfSlot[s]] = w[s] * dOut[t],  dW[s] = <rows[rowOfSlot[s]], dOut[t]>
+// Slots without a row (-1, or a number outside the rows) take no part.  Nothing here uses an atomic on a result: every
+// sum has a fixed order.
+#include "elementwise.cuh"
+#include "experts.cuh"
+#include "sm100_ptx.cuh"
+
+using namespace ascq;
+using namespace ascq::ptx;
+
+namespace ascq {
+namespace {
+
+template <typename K, typename... Args>
+cudaError_t launch_rows(K kernel, dim3 grid, unsigned block, size_t smem, unsigned cluster, cudaStream_t st, Args... args)
+{
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(block, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+__device__ __forceinline__ void pdl_begin()
+{
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// ---- sort ------------------------------------------------------------------------------------------------------------
+// One cluster.  Every warp owns a contiguous run of slots and a private histogram in shared memory; the histograms are
+// summed over the warps and, through distributed shared memory, over the cluster's CTAs, which gives each warp its first position in
+// every expert's run; a second walk over the same slots hands the positions out (equal keys inside a warp's step are
+// ranked with a match).  One launch, no scratch memory, and the order of equal keys is the slots' own.
+template <typename Id> __device__ __forceinline__ int sort_key(const Id* ids, int64_t s, int64_t end, int keys)
+{
+    if (s >= end) return -1;
+    const Id v = ids[s];
+    return v >= 0 && v < static_cast<Id>(keys) ? static_cast<int>(v) : -1;
+}
+
+template <typename Id>
+__global__ void __launch_bounds__(1024) key_sort_kernel(int64_t* counts, int32_t* rowOfSlot, int32_t* slotOfRow, const Id* ids, int64_t slots, int keys,
+                                                        int ctas)
+{
+    extern __shared__ uint32_t smem[];
+    const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t* hist = smem;                    // [warps][keys]: counts, then first positions
+    uint32_t* total = hist + warps * keys;    // [keys]: this CTA's slots per key (read by the other CTAs)
+    uint32_t* first = total + keys;           // [keys]: the key's slots in all CTAs, then where its run starts
+    uint32_t* scan = first + keys;            // [33]
+    for (int i = threadIdx.x; i < warps * keys; i += blockDim.x) hist[i] = 0u;
+    pdl_begin();
+    __syncthreads();
+
+    const int rank = blockIdx.x;
+    const int64_t perWarp = ((slots + static_cast<int64_t>(ctas) * warps - 1) / (static_cast<int64_t>(ctas) * warps) + 31) / 32 * 32;
+    const int64_t begin = (static_cast<int64_t>(rank) * warps + warp) * perWarp;
+    const int64_t end = begin + perWarp < slots ? begin + perWarp : slots;
+    uint32_t* mine = hist + warp * keys;
+    for (int64_t s = begin; s < end; s += 32) {
+        const int key = sort_key<Id>(ids, s + lane, end, keys);
+        if (key >= 0) atomicAdd(&mine[key], 1u);  // a count: the order of the additions does not show
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < keys; e += blockDim.x) {
+        uint32_t run = 0;
+        for (int w = 0; w < warps; ++w) {
+            const uint32_t c = hist[w * keys + e];
+            hist[w * keys + e] = run;
+            run += c;
+        }
+        total[e] = run;
+    }
+    __syncwarp();
+    if (ctas > 1) {
+        cluster_arrive();
+        cluster_wait();
+    } else {
+        __syncthreads();
+    }
+    for (int e = threadIdx.x; e < keys; e += blockDim.x) {
+        uint32_t before = 0, all = 0;
+        if (ctas > 1) {
+            const uint32_t at = smem_u32(total + e);
+            for (int c = 0; c < ctas; ++c) {
+                uint32_t v;
+                asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(mapa_u32(at, c)) : "memory");
+                if (c < rank) before += v;
+                all += v;
+            }
+        } else {
+            all = total[e];
+        }
+        first[e] = all;
+        for (int w = 0; w < warps; ++w) hist[w * keys + e] += before;
+        if (rank == 0) counts[e] = static_cast<int64_t>(all);
+    }
+    __syncwarp();
+    if (ctas > 1) cluster_arrive();  // no CTA may end while another still reads its totals; the wait is at the end
+    __syncthreads();
+    // exclusive scan of `first` over the keys: each thread takes keys / threads consecutive ones (rounded up)
+    const int per = (keys + blockDim.x - 1) / blockDim.x;
+    uint32_t sum = 0;
+    for (int i = 0; i < per; ++i) {
+        const int e = threadIdx.x * per + i;
+        if (e < keys) sum += first[e];
+    }
+    uint32_t incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+        if (lane >= o) incl += v;
+    }
+    if (lane == 31) scan[warp] = incl;
+    __syncthreads();
+    uint32_t base = 0, kept = 0;
+    for (int w = 0; w < warps; ++w) {
+        if (w < warp) base += scan[w];
+        kept += scan[w];
+    }
+    uint32_t run = base + incl - sum;
+    for (int i = 0; i < per; ++i) {
+        const int e = threadIdx.x * per + i;
+        if (e < keys) {
+            const uint32_t c = first[e];
+            first[e] = run;
+            run += c;
+        }
+    }
+    __syncthreads();
+    for (int64_t s = begin; s < end; s += 32) {
+        const int key = sort_key<Id>(ids, s + lane, end, keys);
+        const uint32_t peers = __match_any_sync(0xFFFFFFFFu, key);
+        uint32_t pos = 0;
+        if (key >= 0) pos = first[key] + mine[key] + __popc(peers & ((1u << lane) - 1u));
+        __syncwarp();
+        if (key >= 0 && lane == __ffs(peers) - 1) mine[key] += __popc(peers);
+        __syncwarp();
+        if (s + lane < end) {
+            if (rowOfSlot) rowOfSlot[s + lane] = key >= 0 ? static_cast<int32_t>(pos) : -1;
+            if (slotOfRow && key >= 0) slotOfRow[pos] = static_cast<int32_t>(s + lane);
+        }
+    }
+    if (slotOfRow)
+        for (int64_t r = kept + static_cast<int64_t>(rank) * blockDim.x + threadIdx.x; r < slots; r += static_cast<int64_t>(ctas) * blockDim.x) slotOfRow[r] = -1;
+    __syncwarp();
+    if (ctas > 1) cluster_wait();
+}
+
+template <typename Id> ascq_status launch_key_sort_typed(int64_t* counts, int32_t* rowOfSlot, int32_t* slotOfRow, const void* ids, int64_t slots, int keys,
+                                                         cudaStream_t st)
+{
+    // enough warps that each walks a few steps of 32 slots; a second CTA only once 32 warps walk more than 8 steps each
+    unsigned threads = 128;
+    while (threads < 1024 && slots > static_cast<int64_t>(threads) * 2) threads *= 2;
+    int ctas = 1;
+    while (ctas < 8 && slots > static_cast<int64_t>(ctas) * 8192) ctas *= 2;
+    const size_t smem = (static_cast<size_t>(threads / 32 + 2) * keys + 64) * 4;
+    static PerDeviceOnce once;
+    const int dev = current_device();
+    if (!once.done(dev)) {
+        ASCQ_CUDA_CHECK(cudaFuncSetAttribute(key_sort_kernel<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, (34 * kMaxSortKeys + 64) * 4));
+        once.mark(dev);
+    }
+    ASCQ_CUDA_CHECK(launch_rows(key_sort_kernel<Id>, dim3(ctas), threads, smem, ctas, st, counts, rowOfSlot, slotOfRow, static_cast<const Id*>(ids), slots, keys, ctas));
+    return ASCQ_OK;
+}
+
+// ---- dispatch ---------------------------------------------------------------------------------------------------------
+struct DispatchArgs {
+    uint8_t* dst;
+    const uint8_t* src;
+    uint8_t* dstScale;        // may be null
+    const uint8_t* srcScale;
+    size_t rowBytes, ldSrc, scaleBytes;
+    const int32_t* rowOfSlot;
+    int64_t tokens, rows;
+    int k;
+    uint32_t segments;        // of 32 * kDispatchVecs vectors in a row
+};
+constexpr int kDispatchVecs = 4;
+
+// A warp takes a segment of a token's row: it reads the segment once and writes it to each of the token's rows.
+template <typename V> __global__ void __launch_bounds__(256) dispatch_kernel(const DispatchArgs a)
+{
+    pdl_begin();
+    const int lane = threadIdx.x & 31;
+    const int64_t item = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    const int64_t t = item / a.segments;
+    const uint32_t seg = static_cast<uint32_t>(item % a.segments);
+    if (t >= a.tokens) return;
+    const size_t nvec = a.rowBytes / sizeof(V), v0 = static_cast<size_t>(seg) * 32 * kDispatchVecs + lane;
+    const V* from = reinterpret_cast<const V*>(a.src + static_cast<size_t>(t) * a.ldSrc);
+    V x[kDispatchVecs];
+#pragma unroll
+    for (int u = 0; u < kDispatchVecs; ++u)
+        if (v0 + u * 32 < nvec) x[u] = __ldcs(from + v0 + u * 32);
+    for (int j0 = 0; j0 < a.k; j0 += 32) {
+        const int32_t mine = j0 + lane < a.k ? a.rowOfSlot[t * a.k + j0 + lane] : -1;
+        for (int j = 0; j < 32 && j0 + j < a.k; ++j) {
+            const int32_t r = __shfl_sync(0xFFFFFFFFu, mine, j);
+            if (r < 0 || r >= a.rows) continue;
+            V* to = reinterpret_cast<V*>(a.dst + static_cast<size_t>(r) * a.rowBytes);
+#pragma unroll
+            for (int u = 0; u < kDispatchVecs; ++u)
+                if (v0 + u * 32 < nvec) __stcs(to + v0 + u * 32, x[u]);
+            if (seg == 0 && a.dstScale)
+                for (size_t i = lane; i < a.scaleBytes; i += 32) a.dstScale[static_cast<size_t>(r) * a.scaleBytes + i] = a.srcScale[static_cast<size_t>(t) * a.scaleBytes + i];
+        }
+    }
+}
+
+// ---- combine ----------------------------------------------------------------------------------------------------------
+struct CombineArgs {
+    void* out;             // combine: [tokens, h]
+    void* gradRows;        // gradient: [rows, h], may be null
+    float* gradWeights;    // gradient: [tokens, k], may be null
+    const void* gradOut;   // gradient: [tokens, h]
+    const void* in;        // [rows, h]
+    const int32_t* rowOfSlot;
+    const float* weights;  // may be null (all 1)
+    int64_t tokens, rows, h;
+    int k;
+    uint32_t segments;
+};
+
+// VEC consecutive elements of T as floats: VEC * sizeof(T) bytes in one access of up to 16 bytes
+template <typename T, int VEC> __device__ __forceinline__ void load_f(const T* p, float (&f)[VEC])
+{
+    const Pack<T, VEC> v = [&] {
+        if constexpr (sizeof(T) * VEC >= 4) return load_pack<T, VEC, true>(p);
+        else return Pack<T, VEC>{{*p}};
+    }();
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) f[i] = to_f32<T>(v.v[i]);
+}
+template <typename T> __device__ __forceinline__ T narrow_sat(float f)
+{
+    if constexpr (std::is_same<T, float>::value) return f;
+    else if constexpr (std::is_same<T, __half>::value) return f32_to_f16_sat(f);
+    else return f32_to_bf16_sat(f);
+}
+template <typename T, int VEC> __device__ __forceinline__ void store_f(T* p, const float (&f)[VEC])
+{
+    if constexpr (sizeof(T) * VEC >= 4) {
+        Pack<T, VEC> v;
+        if constexpr (sizeof(T) == 2) {
+            uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+            for (int i = 0; i < VEC / 2; ++i) w[i] = std::is_same<T, __half>::value ? pack_f16x2_sat(f[2 * i], f[2 * i + 1]) : pack_bf16x2_sat(f[2 * i], f[2 * i + 1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) v.v[i] = narrow_sat<T>(f[i]);
+        }
+        store_pack<T, VEC>(p, v);
+    } else {
+        *p = narrow_sat<T>(f[0]);
+    }
+}
+
+constexpr int kCombineVecs = 2;
+
+template <typename T, int VEC> __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a)
+{
+    pdl_begin();
+    const int lane = threadIdx.x & 31;
+    const int64_t item = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    const int64_t t = item / a.segments;
+    const uint32_t seg = static_cast<uint32_t>(item % a.segments);
+    if (t >= a.tokens) return;
+    const int64_t c0 = (static_cast<int64_t>(seg) * 32 * kCombineVecs + lane) * VEC;
+    float acc[kCombineVecs][VEC] = {};
+    for (int j0 = 0; j0 < a.k; j0 += 32) {
+        int32_t mine = -1;
+        float wMine = 1.0f;
+        if (j0 + lane < a.k) {
+            mine = a.rowOfSlot[t * a.k + j0 + lane];
+            if (a.weights) wMine = a.weights[t * a.k + j0 + lane];
+        }
+        const int jn = a.k - j0 < 32 ? a.k - j0 : 32;
+#pragma unroll 4
+        for (int j = 0; j < jn; ++j) {
+            const int32_t r = __shfl_sync(0xFFFFFFFFu, mine, j);
+            const float w = __shfl_sync(0xFFFFFFFFu, wMine, j);
+            if (r < 0 || r >= a.rows) continue;
+            const T* from = static_cast<const T*>(a.in) + static_cast<int64_t>(r) * a.h;
+#pragma unroll
+            for (int u = 0; u < kCombineVecs; ++u) {
+                const int64_t c = c0 + u * 32 * VEC;
+                if (c < a.h) {
+                    float f[VEC];
+                    load_f<T, VEC>(from + c, f);
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) acc[u][i] = fmaf(w, f[i], acc[u][i]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kCombineVecs; ++u) {
+        const int64_t c = c0 + u * 32 * VEC;
+        if (c < a.h) store_f<T, VEC>(static_cast<T*>(a.out) + t * a.h + c, acc[u]);
+    }
+}
+
+// ---- gradient of combine --------------------------------------------------------------------------------------------------
+// One CTA per token: gradOut's row is read once for up to kGradRows of the token's rows at a time.
+constexpr int kGradRows = 8;
+
+template <typename T, int VEC> __global__ void __launch_bounds__(256) combine_grad_kernel(const CombineArgs a)
+{
+    __shared__ float part[8][kGradRows];
+    pdl_begin();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const int64_t t = blockIdx.x;
+    const T* dOut = static_cast<const T*>(a.gradOut) + t * a.h;
+    for (int j0 = 0; j0 < a.k; j0 += kGradRows) {
+        int32_t r[kGradRows];
+        float w[kGradRows], dot[kGradRows] = {};
+#pragma unroll
+        for (int j = 0; j < kGradRows; ++j) {
+            r[j] = j0 + j < a.k ? a.rowOfSlot[t * a.k + j0 + j] : -1;
+            if (r[j] >= a.rows) r[j] = -1;
+            w[j] = a.weights && j0 + j < a.k ? a.weights[t * a.k + j0 + j] : 1.0f;
+        }
+        for (int64_t c = static_cast<int64_t>(threadIdx.x) * VEC; c < a.h; c += static_cast<int64_t>(blockDim.x) * VEC) {
+            float d[VEC];
+            load_f<T, VEC>(dOut + c, d);
+#pragma unroll
+            for (int j = 0; j < kGradRows; ++j) {
+                if (r[j] < 0) continue;
+                const int64_t at = static_cast<int64_t>(r[j]) * a.h + c;
+                if (a.gradWeights) {
+                    float f[VEC];
+                    load_f<T, VEC>(static_cast<const T*>(a.in) + at, f);
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) dot[j] = fmaf(f[i], d[i], dot[j]);
+                }
+                if (a.gradRows) {
+                    float g[VEC];
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) g[i] = __fmul_rn(w[j], d[i]);
+                    store_f<T, VEC>(static_cast<T*>(a.gradRows) + at, g);
+                }
+            }
+        }
+        if (a.gradWeights) {
+#pragma unroll
+            for (int j = 0; j < kGradRows; ++j)
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) dot[j] += __shfl_xor_sync(0xFFFFFFFFu, dot[j], o);
+            if (lane == 0)
+#pragma unroll
+                for (int j = 0; j < kGradRows; ++j) part[warp][j] = dot[j];
+            __syncthreads();
+            if (threadIdx.x < kGradRows && j0 + static_cast<int>(threadIdx.x) < a.k) {
+                float s = 0.f;
+                for (int i = 0; i < warps; ++i) s += part[i][threadIdx.x];
+                a.gradWeights[t * a.k + j0 + threadIdx.x] = s;
+            }
+            __syncthreads();
+        }
+    }
+}
+
+bool float_type(ascq_dtype t) { return t == ASCQ_DT_F16 || t == ASCQ_DT_BF16 || t == ASCQ_DT_F32; }
+
+// The checks that dispatch, combine and the gradient share.
+ascq_status check_slots(const int32_t* rowOfSlot, int64_t tokens, int k, int64_t rows)
+{
+    if (tokens < 0 || rows < 0 || k <= 0) return fail(ASCQ_ERR_INVALID_ARG, "tokens and rows must not be negative and k must be positive");
+    if (tokens > 0x7FFFFFFFll / k || rows > 0x7FFFFFFFll) return fail(ASCQ_ERR_INVALID_ARG, "tokens * k and rows must be below 2^31");
+    if (tokens && (reinterpret_cast<uintptr_t>(rowOfSlot) & 3u)) return fail(ASCQ_ERR_ALIGNMENT, "rowOfSlot is not aligned to its element type");
+    return ASCQ_OK;
+}
+
+}  // namespace
+
+ascq_status launch_key_sort(int64_t* counts, int32_t* rowOfSlot, int32_t* slotOfRow, const void* ids, bool ids64, int64_t slots, int keys, ::CUstream_st* st)
+{
+    return ids64 ? launch_key_sort_typed<int64_t>(counts, rowOfSlot, slotOfRow, ids, slots, keys, st)
+                 : launch_key_sort_typed<int32_t>(counts, rowOfSlot, slotOfRow, ids, slots, keys, st);
+}
+}  // namespace ascq
+
+extern "C" ascq_status ascq_expert_sort(int64_t* counts, int32_t* rowOfSlot, int32_t* slotOfRow, const void* expertIds, ascq_dtype idT, int64_t slots,
+                                        int numExperts, void* stream)
+{
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (idT != ASCQ_DT_I32 && idT != ASCQ_DT_I64) return fail(ASCQ_ERR_UNSUPPORTED, "expertIds must be int32 or int64");
+    if (numExperts < 1 || numExperts > kMaxSortKeys) return fail(ASCQ_ERR_INVALID_ARG, "numExperts is %d, which must be in [1, %d]", numExperts, kMaxSortKeys);
+    if (slots < 0 || slots > 0x7FFFFFFFll) return fail(ASCQ_ERR_INVALID_ARG, "slots must be in [0, 2^31)");
+    if (!counts || (slots && (!rowOfSlot || !expertIds))) return fail(ASCQ_ERR_INVALID_ARG, "counts, rowOfSlot and expertIds must not be NULL");
+    const size_t idBytes = idT == ASCQ_DT_I64 ? 8 : 4, n = static_cast<size_t>(slots);
+    if ((reinterpret_cast<uintptr_t>(counts) & 7u) || (reinterpret_cast<uintptr_t>(expertIds) & (idBytes - 1)) || (reinterpret_cast<uintptr_t>(rowOfSlot) & 3u) ||
+        (reinterpret_cast<uintptr_t>(slotOfRow) & 3u))
+        return fail(ASCQ_ERR_ALIGNMENT, "a tensor is not aligned to its element type");
+    const void* p[4] = {counts, rowOfSlot, slotOfRow, expertIds};
+    const size_t b[4] = {static_cast<size_t>(numExperts) * 8, n * 4, n * 4, n * idBytes};
+    for (int i = 0; i < 4; ++i)
+        for (int j = 0; j < i; ++j)
+            if (spans_overlap(p[i], b[i], p[j], b[j])) return fail(ASCQ_ERR_INVALID_ARG, "counts, rowOfSlot, slotOfRow and expertIds must not overlap");
+    if (slots == 0) {
+        ASCQ_CUDA_CHECK(cudaMemsetAsync(counts, 0, static_cast<size_t>(numExperts) * 8, st));
+        return ASCQ_OK;
+    }
+    return launch_key_sort(counts, rowOfSlot, slotOfRow, expertIds, idT == ASCQ_DT_I64, slots, numExperts, st);
+}
+
+extern "C" ascq_status ascq_expert_dispatch(void* dst, const void* src, size_t rowBytes, size_t ldSrcBytes, void* dstScale, const void* srcScale,
+                                            size_t scaleRowBytes, const int32_t* rowOfSlot, int64_t tokens, int k, int64_t rows, void* stream)
+{
+    ascq_status rc = check_slots(rowOfSlot, tokens, k, rows);
+    if (rc != ASCQ_OK) return rc;
+    if (ldSrcBytes == 0) ldSrcBytes = rowBytes;
+    if (ldSrcBytes < rowBytes) return fail(ASCQ_ERR_INVALID_ARG, "the row pitch of src is smaller than its rows");
+    if ((dstScale == nullptr) != (srcScale == nullptr)) return fail(ASCQ_ERR_INVALID_ARG, "dstScale and srcScale must both be given or both be NULL");
+    if (rowBytes > (size_t{1} << 40) || ldSrcBytes > (size_t{1} << 40) || scaleRowBytes > (size_t{1} << 40)) return fail(ASCQ_ERR_INVALID_ARG, "a row is longer than 2^40 bytes");
+    if (tokens == 0 || rows == 0 || rowBytes == 0) return ASCQ_OK;
+    if (!dst || !src || !rowOfSlot) return fail(ASCQ_ERR_INVALID_ARG, "dst, src and rowOfSlot must not be NULL");
+    if (dstScale && scaleRowBytes == 0) return fail(ASCQ_ERR_INVALID_ARG, "scaleRowBytes must be positive when scales are given");
+    const size_t T = static_cast<size_t>(tokens), R = static_cast<size_t>(rows);
+    const void* p[5] = {dst, dstScale, src, srcScale, rowOfSlot};
+    const size_t b[5] = {R * rowBytes, dstScale ? R * scaleRowBytes : 0, (T - 1) * ldSrcBytes + rowBytes, srcScale ? T * scaleRowBytes : 0, T * k * 4};
+    for (int i = 0; i < 2; ++i)
+        for (int j = i + 1; j < 5; ++j)
+            if (spans_overlap(p[i], b[i], p[j], b[j])) return fail(ASCQ_ERR_INVALID_ARG, "an output overlaps another tensor of the call");
+
+    DispatchArgs a{static_cast<uint8_t*>(dst), static_cast<const uint8_t*>(src), static_cast<uint8_t*>(dstScale), static_cast<const uint8_t*>(srcScale),
+                   rowBytes, ldSrcBytes, scaleRowBytes, rowOfSlot, tokens, rows, k, 0};
+    // the widest access that every row of both tensors is aligned to
+    const uintptr_t all = reinterpret_cast<uintptr_t>(dst) | reinterpret_cast<uintptr_t>(src) | rowBytes | ldSrcBytes;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    auto run = [&](auto tag) -> ascq_status {
+        using V = decltype(tag);
+        const size_t nvec = rowBytes / sizeof(V), per = 32 * kDispatchVecs;
+        a.segments = static_cast<uint32_t>((nvec + per - 1) / per);
+        const int64_t ctas = (tokens * static_cast<int64_t>(a.segments) + 7) / 8;
+        if (ctas > 0x7FFFFFFFll) return fail(ASCQ_ERR_INVALID_ARG, "the rows are too long for one launch");
+        ASCQ_CUDA_CHECK(launch_rows(dispatch_kernel<V>, dim3(static_cast<unsigned>(ctas)), 256, 0, 1, st, a));
+        return ASCQ_OK;
+    };
+    if (all % 16 == 0) return run(uint4{});
+    if (all % 4 == 0) return run(uint32_t{});
+    if (all % 2 == 0) return run(static_cast<unsigned short>(0));
+    return run(static_cast<unsigned char>(0));
+}
+
+extern "C" ascq_status ascq_expert_combine(void* dst, const void* in, ascq_dtype T, const int32_t* rowOfSlot, const float* weights, int64_t tokens, int k,
+                                           int64_t rows, int64_t h, void* stream)
+{
+    ascq_status rc = check_slots(rowOfSlot, tokens, k, rows);
+    if (rc != ASCQ_OK) return rc;
+    if (!float_type(T)) return fail(ASCQ_ERR_UNSUPPORTED, "rows must be half, bfloat16_t or float");
+    if (h < 0 || h > 0x7FFFFFFFll) return fail(ASCQ_ERR_INVALID_ARG, "h must be in [0, 2^31)");
+    if (tokens == 0 || h == 0) return ASCQ_OK;
+    if (!dst || (rows && !in) || !rowOfSlot) return fail(ASCQ_ERR_INVALID_ARG, "dst, rows and rowOfSlot must not be NULL");
+    const size_t es = dtype_size(T), N = static_cast<size_t>(tokens);
+    const uintptr_t all = reinterpret_cast<uintptr_t>(dst) | reinterpret_cast<uintptr_t>(in) | static_cast<uintptr_t>(h) * es;
+    if (all % es || (reinterpret_cast<uintptr_t>(weights) & 3u)) return fail(ASCQ_ERR_ALIGNMENT, "a tensor is not aligned to its element type");
+    const void* p[4] = {dst, in, weights, rowOfSlot};
+    const size_t b[4] = {N * h * es, static_cast<size_t>(rows) * h * es, weights ? N * k * 4 : 0, N * k * 4};
+    for (int j = 1; j < 4; ++j)
+        if (spans_overlap(p[0], b[0], p[j], b[j])) return fail(ASCQ_ERR_INVALID_ARG, "dst overlaps another tensor of the call");
+    CombineArgs a{};
+    a.out = dst; a.in = in; a.rowOfSlot = rowOfSlot; a.weights = weights; a.tokens = tokens; a.rows = rows; a.h = h; a.k = k;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    auto run = [&](auto kernel, int vec) -> ascq_status {
+        const int64_t per = 32ll * kCombineVecs * vec;
+        a.segments = static_cast<uint32_t>((h + per - 1) / per);
+        const int64_t ctas = (tokens * static_cast<int64_t>(a.segments) + 7) / 8;
+        if (ctas > 0x7FFFFFFFll) return fail(ASCQ_ERR_INVALID_ARG, "the rows are too long for one launch");
+        ASCQ_CUDA_CHECK(launch_rows(kernel, dim3(static_cast<unsigned>(ctas)), 256, 0, 1, st, a));
+        return ASCQ_OK;
+    };
+    const bool vec = all % 16 == 0;
+    if (T == ASCQ_DT_F16) return vec ? run(combine_kernel<__half, 8>, 8) : run(combine_kernel<__half, 1>, 1);
+    if (T == ASCQ_DT_BF16) return vec ? run(combine_kernel<__nv_bfloat16, 8>, 8) : run(combine_kernel<__nv_bfloat16, 1>, 1);
+    return vec ? run(combine_kernel<float, 4>, 4) : run(combine_kernel<float, 1>, 1);
+}
+
+extern "C" ascq_status ascq_expert_combine_grad(void* gradRows, float* gradWeights, const void* gradOut, const void* in, ascq_dtype T, const int32_t* rowOfSlot,
+                                                const float* weights, int64_t tokens, int k, int64_t rows, int64_t h, void* stream)
+{
+    ascq_status rc = check_slots(rowOfSlot, tokens, k, rows);
+    if (rc != ASCQ_OK) return rc;
+    if (!float_type(T)) return fail(ASCQ_ERR_UNSUPPORTED, "rows must be half, bfloat16_t or float");
+    if (h < 0 || h > 0x7FFFFFFFll) return fail(ASCQ_ERR_INVALID_ARG, "h must be in [0, 2^31)");
+    if (tokens == 0 || (rows == 0 && !gradWeights)) return ASCQ_OK;
+    if (!gradRows && !gradWeights) return fail(ASCQ_ERR_INVALID_ARG, "gradRows and gradWeights are both NULL");
+    if ((h && !gradOut) || !rowOfSlot || (gradWeights && rows && h && !in)) return fail(ASCQ_ERR_INVALID_ARG, "gradOut, rows and rowOfSlot must not be NULL");
+    const size_t es = dtype_size(T), N = static_cast<size_t>(tokens);
+    const uintptr_t all = reinterpret_cast<uintptr_t>(gradRows) | reinterpret_cast<uintptr_t>(gradOut) | (gradWeights ? reinterpret_cast<uintptr_t>(in) : 0) |
+                          static_cast<uintptr_t>(h) * es;
+    if (all % es || (reinterpret_cast<uintptr_t>(weights) & 3u) || (reinterpret_cast<uintptr_t>(gradWeights) & 3u))
+        return fail(ASCQ_ERR_ALIGNMENT, "a tensor is not aligned to its element type");
+    const size_t rowsBytes = static_cast<size_t>(rows) * h * es;
+    const void* p[6] = {gradRows, gradWeights, gradOut, gradWeights ? in : nullptr, weights, rowOfSlot};
+    const size_t b[6] = {rowsBytes, N * k * 4, N * h * es, rowsBytes, N * k * 4, N * k * 4};
+    for (int i = 0; i < 2; ++i)
+        for (int j = i + 1; j < 6; ++j)
+            if (spans_overlap(p[i], b[i], p[j], b[j])) return fail(ASCQ_ERR_INVALID_ARG, "an output overlaps another tensor of the call");
+    CombineArgs a{};
+    a.gradRows = gradRows; a.gradWeights = gradWeights; a.gradOut = gradOut; a.in = in; a.rowOfSlot = rowOfSlot; a.weights = weights;
+    a.tokens = tokens; a.rows = rows; a.h = h; a.k = k;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    auto run = [&](auto kernel, int vec) -> ascq_status {
+        const int64_t nvec = (h + vec - 1) / vec;
+        const unsigned block = nvec >= 256 ? 256u : nvec <= 32 ? 32u : static_cast<unsigned>((nvec + 31) / 32 * 32);
+        ASCQ_CUDA_CHECK(launch_rows(kernel, dim3(static_cast<unsigned>(tokens)), block, 0, 1, st, a));
+        return ASCQ_OK;
+    };
+    const bool vec = all % 16 == 0;
+    if (T == ASCQ_DT_F16) return vec ? run(combine_grad_kernel<__half, 8>, 8) : run(combine_grad_kernel<__half, 1>, 1);
+    if (T == ASCQ_DT_BF16) return vec ? run(combine_grad_kernel<__nv_bfloat16, 8>, 8) : run(combine_grad_kernel<__nv_bfloat16, 1>, 1);
+    return vec ? run(combine_grad_kernel<float, 4>, 4) : run(combine_grad_kernel<float, 1>, 1);
+}

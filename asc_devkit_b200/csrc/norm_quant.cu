@@ -1,0 +1,472 @@
+// Residual addition, root-mean-square norm and quantisation of the result in one pass: the producer of the A operand of the
+// W8A8 matmuls (int8, one fp32 scale per row) and of the MX matmuls (fp8 / fp4, one E8M0 scale per 32 elements).
+//
+//   h = src + residual (fp32, not rounded)            residualOut = cast(h)
+//   y = h * rstd * gamma,  rstd = 1 / sqrt(mean(h^2) + epsilon)                        normOut = cast(y)
+//   int8:  scale = max|y| / 127,  q = RINT(y * 127 / max|y|)
+//   MX:    e = floor(log2 max|y|) - emax per block of 32,  scale byte = e + 127,  q = cast(y * 2^-e)
+//
+// What bounds it: HBM.  With bf16 tensors and residualOut an element costs 2 + 2 bytes read, 2 + 1 written.  A CTA owns whole rows and
+// keeps a row in registers between the reduction and the quantisation, so each byte moves once.  For int8 the row's
+// maximum needs no second reduction: max|y| = rstd * max|h * gamma|, so sum(h^2) and max|h * gamma| go through the same
+// shuffles and the same barrier, and RINT(y * 127 / max|y|) = RINT((h * gamma) * (127 / max|h * gamma|)) does not need rstd.
+#include "elementwise.cuh"
+
+using namespace ascq;
+
+namespace ascq {
+namespace {
+
+enum : int { kOutI8 = 0, kOutE4M3 = 1, kOutE5M2 = 2, kOutE2M1 = 3 };
+// exponent of the largest binade of each element type (OCP MX: the shared exponent is floor(log2 amax) minus it)
+__host__ __device__ constexpr int out_emax(int out) { return out == kOutE4M3 ? 8 : out == kOutE5M2 ? 15 : 2; }
+
+struct NormArgs {
+    void* dst;
+    void* scaleOut;
+    void* residualOut;     // may be null
+    void* normOut;         // may be null
+    const void* src;
+    const void* residual;  // may be null
+    const void* gamma;
+    uint32_t m, n;
+    int64_t ldSrc, ldResidual, ldResidualOut, ldNormOut;
+    float epsilon;
+    int out;               // kernel for odd shapes only: the vector kernel has it as a template parameter
+};
+
+__device__ __forceinline__ float max_nan(float a, float b)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ bool finite_f32(float v) { return fabsf(v) <= 3.4028234663852886e38f; }
+
+// 8 consecutive elements: 16 bytes of a 16-bit type, 32 of fp32 (two 16-byte loads)
+template <typename T> struct Vec8 {
+    uint4 w[sizeof(T) / 2];
+};
+template <typename T> __device__ __forceinline__ Vec8<T> load8(const T* p)
+{
+    Vec8<T> v;
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) v.w[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+    return v;
+}
+template <typename T> __device__ __forceinline__ void widen8(const Vec8<T>& v, float (&f)[8])
+{
+    if constexpr (sizeof(T) == 4) {
+        const uint32_t a[8] = {v.w[0].x, v.w[0].y, v.w[0].z, v.w[0].w, v.w[1].x, v.w[1].y, v.w[1].z, v.w[1].w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(a[i]);
+    } else {
+        const uint32_t a[4] = {v.w[0].x, v.w[0].y, v.w[0].z, v.w[0].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                f[2 * i] = __uint_as_float(a[i] << 16);
+                f[2 * i + 1] = __uint_as_float(a[i] & 0xFFFF0000u);
+            } else {
+                const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&a[i]));
+                f[2 * i] = t.x;
+                f[2 * i + 1] = t.y;
+            }
+        }
+    }
+}
+template <typename T> __device__ __forceinline__ T narrow(float f)
+{
+    if constexpr (std::is_same<T, float>::value) return f;
+    else if constexpr (std::is_same<T, __half>::value) return f32_to_f16_sat(f);
+    else return f32_to_bf16_sat(f);
+}
+// the framework's narrowing rule: round to nearest even, a finite value that overflows saturates
+template <typename T> __device__ __forceinline__ void store8(T* p, const float (&f)[8])
+{
+    if constexpr (sizeof(T) == 4) {
+        __stcs(reinterpret_cast<float4*>(p), make_float4(f[0], f[1], f[2], f[3]));
+        __stcs(reinterpret_cast<float4*>(p) + 1, make_float4(f[4], f[5], f[6], f[7]));
+    } else {
+        uint32_t r[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (std::is_same<T, __half>::value) r[i] = pack_f16x2_sat(f[2 * i], f[2 * i + 1]);
+            else r[i] = pack_bf16x2_sat(f[2 * i], f[2 * i + 1]);
+        }
+        __stcs(reinterpret_cast<uint4*>(p), make_uint4(r[0], r[1], r[2], r[3]));
+    }
+}
+
+// Two scaled values -> two codes, the first in the low byte (or nibble); round to nearest even, saturating.  fp4 goes through
+// bfloat16 first, the conversion chain of AscendQuant's fp4 destination.
+template <int OUT> __device__ __forceinline__ uint32_t mx_pair(float first, float second)
+{
+    unsigned short r;
+    if constexpr (OUT == kOutE4M3) asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(r) : "f"(first), "f"(second));
+    else if constexpr (OUT == kOutE5M2) asm("cvt.rn.satfinite.e5m2x2.f32 %0, %2, %1;" : "=h"(r) : "f"(first), "f"(second));
+    else {
+        uint32_t b2;
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b2) : "f"(second), "f"(first));
+        asm("{ .reg .b8 t;\n cvt.rn.satfinite.e2m1x2.f32 t, %2, %1;\n mov.b16 %0, {t, 0}; }"
+            : "=h"(r)
+            : "f"(__uint_as_float(b2 << 16)), "f"(__uint_as_float(b2 & 0xFFFF0000u)));
+    }
+    return r;
+}
+// Shared exponent of a block from its largest magnitude (finite): floor(log2(amax)) - emax inside the E8M0 range, 0 for an
+// all-zero block.  A subnormal amax counts as 2^-126; with emax >= 2 it ends at the range's lower end either way.
+__device__ __forceinline__ int mx_exponent(float amax, int emax)
+{
+    if (!(amax > 0.f)) return 0;
+    const int ex = static_cast<int>(__float_as_uint(amax) >> 23);
+    return min(max((ex == 0 ? -126 : ex - 127) - emax, -127), 127);
+}
+// 2^-e for e in [-127, 127]; 2^-127 is a subnormal
+__device__ __forceinline__ float exp2_neg(int e) { return e == 127 ? __uint_as_float(0x00400000u) : __uint_as_float(static_cast<uint32_t>(127 - e) << 23); }
+
+// The int8 chain's multiplier 127 / amax, in two factors so that it does not overflow where amax is close to the smallest
+// normal number: q = RINT((p * pre) * mul).  pre is 1 for every amax that a norm leaves in practice.
+struct I8Factor {
+    float pre, mul;
+};
+__device__ __forceinline__ I8Factor i8_factor(float amax)
+{
+    I8Factor f;
+    f.pre = amax < 1e-30f ? 1.2089258196146292e24f : 1.0f;  // 2^80
+    f.mul = amax > 0.f ? __fdiv_rn(127.0f, amax * f.pre) : 1.0f;
+    return f;
+}
+
+// Sum and maximum over the CTA, the same result in every thread.  `slot` alternates between the rows of a CTA: a warp
+// that is already at the next row then writes the other half of the array, so one barrier per row is enough.
+__device__ __forceinline__ void cta_sum_max(float& sum, float& mx, float2 (*part)[16], int slot)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        mx = max_nan(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
+    }
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    if (warps == 1) return;
+    if (lane == 0) part[slot][warp] = make_float2(sum, mx);
+    __syncthreads();
+    const float2 p = lane < warps ? part[slot][lane] : make_float2(0.f, 0.f);
+    sum = p.x;
+    mx = p.y;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+        sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        mx = max_nan(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
+    }
+    sum = __shfl_sync(0xFFFFFFFFu, sum, 0);
+    mx = __shfl_sync(0xFFFFFFFFu, mx, 0);
+}
+
+// The vector kernel: a thread owns NV vectors of 8 elements of a row, spaced by the CTA's width.
+template <typename T, typename G, int OUT, int NV> __global__ void __launch_bounds__(512) norm_rows_kernel(const NormArgs a)
+{
+    __shared__ float2 part[2][16];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const uint32_t nvec = a.n / 8;
+    const T* src = static_cast<const T*>(a.src);
+    const T* res = static_cast<const T*>(a.residual);
+    Vec8<G> g[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const uint32_t v = i * blockDim.x + threadIdx.x;
+        if (v < nvec) {
+            const uint4* p = reinterpret_cast<const uint4*>(static_cast<const G*>(a.gamma) + v * 8);
+#pragma unroll
+            for (int j = 0; j < static_cast<int>(sizeof(G)) / 2; ++j) g[i].w[j] = __ldg(p + j);
+        }
+    }
+    int slot = 0;
+    for (uint32_t row = blockIdx.x; row < a.m; row += gridDim.x, slot ^= 1) {
+        float h[NV][8];
+        float sum = 0.f, mx = 0.f;
+        {
+            Vec8<T> xs[NV], rs[NV];
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const uint32_t v = i * blockDim.x + threadIdx.x;
+                if (v < nvec) {
+                    xs[i] = load8<T>(src + row * a.ldSrc + v * 8);
+                    if (res) rs[i] = load8<T>(res + row * a.ldResidual + v * 8);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const uint32_t v = i * blockDim.x + threadIdx.x;
+                if (v < nvec) {
+                    widen8<T>(xs[i], h[i]);
+                    if (res) {
+                        float r[8];
+                        widen8<T>(rs[i], r);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) h[i][j] = __fadd_rn(h[i][j], r[j]);
+                    }
+                    if (a.residualOut) store8<T>(static_cast<T*>(a.residualOut) + row * a.ldResidualOut + v * 8, h[i]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) h[i][j] = 0.f;
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const uint32_t v = i * blockDim.x + threadIdx.x;
+            if (v < nvec) {
+                float gf[8];
+                widen8<G>(g[i], gf);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    sum = fmaf(h[i][j], h[i][j], sum);
+                    h[i][j] = __fmul_rn(h[i][j], gf[j]);  // from here on h * gamma
+                    if constexpr (OUT == kOutI8) mx = max_nan(mx, fabsf(h[i][j]));
+                }
+            }
+        }
+        cta_sum_max(sum, mx, part, slot);
+        const float rstd = finite_f32(sum) ? __frsqrt_rn(__fadd_rn(__fdiv_rn(sum, static_cast<float>(a.n)), a.epsilon)) : __int_as_float(0x7FFFFFFF);
+        if (a.normOut) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const uint32_t v = i * blockDim.x + threadIdx.x;
+                if (v < nvec) {
+                    float y[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) y[j] = __fmul_rn(h[i][j], rstd);
+                    store8<T>(static_cast<T*>(a.normOut) + row * a.ldNormOut + v * 8, y);
+                }
+            }
+        }
+        if constexpr (OUT == kOutI8) {
+            const float top = __fmul_rn(mx, rstd);  // the row's largest |y|; NaN with rstd
+            const bool ok = finite_f32(mx) && finite_f32(top);
+            if (threadIdx.x == 0)
+                static_cast<float*>(a.scaleOut)[row] = !ok ? __int_as_float(0x7FFFFFFF) : mx > 0.f ? __fdiv_rn(top, 127.0f) : 1.0f;
+            const I8Factor f = i8_factor(mx);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const uint32_t v = i * blockDim.x + threadIdx.x;
+                if (v < nvec) {
+                    if (f.pre != 1.0f) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) h[i][j] *= f.pre;
+                    }
+                    uint2 q;
+                    q.x = pack_i8x4_rni(__fmul_rn(h[i][0], f.mul), __fmul_rn(h[i][1], f.mul), __fmul_rn(h[i][2], f.mul), __fmul_rn(h[i][3], f.mul));
+                    q.y = pack_i8x4_rni(__fmul_rn(h[i][4], f.mul), __fmul_rn(h[i][5], f.mul), __fmul_rn(h[i][6], f.mul), __fmul_rn(h[i][7], f.mul));
+                    if (!ok) q = make_uint2(0u, 0u);
+                    __stcs(reinterpret_cast<uint2*>(static_cast<int8_t*>(a.dst) + static_cast<size_t>(row) * a.n + v * 8), q);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const uint32_t v = i * blockDim.x + threadIdx.x;
+                float amax = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    h[i][j] = __fmul_rn(h[i][j], rstd);
+                    amax = max_nan(amax, fabsf(h[i][j]));
+                }
+                // four neighbouring lanes hold a block; n is a multiple of 32, so they are inside the row together or not at all
+                amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
+                amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 2));
+                if (v < nvec) {
+                    const bool ok = finite_f32(amax);
+                    const int e = mx_exponent(amax, out_emax(OUT));
+                    const float up = exp2_neg(e);
+                    uint32_t c[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) c[j] = ok ? mx_pair<OUT>(__fmul_rn(h[i][2 * j], up), __fmul_rn(h[i][2 * j + 1], up)) : 0u;
+                    const size_t at = (static_cast<size_t>(row) * nvec + v);
+                    if constexpr (OUT == kOutE2M1) static_cast<uint32_t*>(a.dst)[at] = c[0] | (c[1] << 8) | (c[2] << 16) | (c[3] << 24);
+                    else __stcs(static_cast<uint2*>(a.dst) + at, make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16)));
+                    if ((threadIdx.x & 3) == 0) static_cast<uint8_t*>(a.scaleOut)[at / 4] = static_cast<uint8_t>(ok ? e + 127 : 0xFF);
+                }
+            }
+        }
+    }
+}
+
+// Odd widths, unaligned tensors, rows too long for registers: one CTA per row, one element per thread and step; the second
+// pass computes h again from the sources (a row is in L2).  The same arithmetic.
+template <typename T, typename G> __global__ void __launch_bounds__(256) norm_any_kernel(const NormArgs a)
+{
+    __shared__ float2 part[2][16];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const uint32_t row = blockIdx.x;
+    const T* src = static_cast<const T*>(a.src) + row * a.ldSrc;
+    const T* res = a.residual ? static_cast<const T*>(a.residual) + row * a.ldResidual : nullptr;
+    const G* gamma = static_cast<const G*>(a.gamma);
+    T* resOut = a.residualOut ? static_cast<T*>(a.residualOut) + row * a.ldResidualOut : nullptr;
+    T* normOut = a.normOut ? static_cast<T*>(a.normOut) + row * a.ldNormOut : nullptr;
+    float sum = 0.f, mx = 0.f;
+    for (uint32_t c = threadIdx.x; c < a.n; c += blockDim.x) {
+        const float h = res ? __fadd_rn(to_f32<T>(src[c]), to_f32<T>(res[c])) : to_f32<T>(src[c]);
+        sum = fmaf(h, h, sum);
+        mx = max_nan(mx, fabsf(__fmul_rn(h, to_f32<G>(gamma[c]))));
+    }
+    cta_sum_max(sum, mx, part, 0);
+    const float rstd = finite_f32(sum) ? __frsqrt_rn(__fadd_rn(__fdiv_rn(sum, static_cast<float>(a.n)), a.epsilon)) : __int_as_float(0x7FFFFFFF);
+    const float top = __fmul_rn(mx, rstd);
+    const bool rowOk = finite_f32(mx) && finite_f32(top);
+    const I8Factor f = i8_factor(mx);
+    const size_t out0 = static_cast<size_t>(row) * a.n;
+    if (a.out == kOutI8 && threadIdx.x == 0)
+        static_cast<float*>(a.scaleOut)[row] = !rowOk ? __int_as_float(0x7FFFFFFF) : mx > 0.f ? __fdiv_rn(top, 127.0f) : 1.0f;
+    // each element is read again by the thread that then overwrites it where residualOut is one of the sources
+    for (uint32_t c0 = 0; c0 < a.n; c0 += blockDim.x) {
+        const uint32_t c = c0 + threadIdx.x;
+        float p = 0.f;
+        if (c < a.n) {
+            const float h = res ? __fadd_rn(to_f32<T>(src[c]), to_f32<T>(res[c])) : to_f32<T>(src[c]);
+            p = __fmul_rn(h, to_f32<G>(gamma[c]));
+            if (resOut) resOut[c] = narrow<T>(h);
+            if (normOut) normOut[c] = narrow<T>(__fmul_rn(p, rstd));
+        }
+        if (a.out == kOutI8) {
+            if (c < a.n)
+                static_cast<int8_t*>(a.dst)[out0 + c] =
+                    static_cast<int8_t>(rowOk ? f32_to_i8_sat(__fmul_rn(f.pre != 1.0f ? p * f.pre : p, f.mul), kRoundRint) : 0);
+        } else {  // n is a multiple of 32: a warp holds one block, whole or not at all
+            const float y = __fmul_rn(p, rstd);
+            float amax = fabsf(y);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
+            const bool ok = finite_f32(amax);
+            const int e = mx_exponent(amax, out_emax(a.out));
+            const float v = __fmul_rn(y, exp2_neg(e));
+            const float next = __shfl_down_sync(0xFFFFFFFFu, v, 1);
+            if (c < a.n) {
+                if (a.out == kOutE2M1) {
+                    if ((c & 1) == 0) static_cast<uint8_t*>(a.dst)[(out0 + c) / 2] = static_cast<uint8_t>(ok ? mx_pair<kOutE2M1>(v, next) : 0u);
+                } else {
+                    const uint32_t code = a.out == kOutE4M3 ? mx_pair<kOutE4M3>(v, 0.f) : mx_pair<kOutE5M2>(v, 0.f);
+                    static_cast<uint8_t*>(a.dst)[out0 + c] = static_cast<uint8_t>(ok ? code & 0xFFu : 0u);
+                }
+                if ((c & 31) == 0) static_cast<uint8_t*>(a.scaleOut)[(out0 + c) / 32] = static_cast<uint8_t>(ok ? e + 127 : 0xFF);
+            }
+        }
+    }
+}
+
+template <typename K> cudaError_t launch_norm(K kernel, unsigned grid, unsigned block, cudaStream_t st, const NormArgs& a)
+{
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid, 1, 1);
+    cfg.blockDim = dim3(block, 1, 1);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
+constexpr uint32_t kNormThreads = 512, kNormMaxVectors = 4;  // the longest row the vector kernel holds: 512 * 4 * 8 elements
+
+template <typename T, typename G, int OUT> cudaError_t launch_norm_rows(const NormArgs& a, cudaStream_t st)
+{
+    const uint32_t nvec = a.n / 8;
+    uint32_t nv = 1;
+    while (nv < kNormMaxVectors && (nvec + nv - 1) / nv > kNormThreads) nv *= 2;
+    const unsigned block = ((nvec + nv - 1) / nv + 31) / 32 * 32;
+    const unsigned perSm = nv >= 4 ? 1u : std::max(1u, 1024u / block);
+    const unsigned grid = std::min<uint64_t>(a.m, static_cast<uint64_t>(sm_count()) * perSm);
+    if (nv == 1) return launch_norm(norm_rows_kernel<T, G, OUT, 1>, grid, block, st, a);
+    if (nv == 2) return launch_norm(norm_rows_kernel<T, G, OUT, 2>, grid, block, st, a);
+    return launch_norm(norm_rows_kernel<T, G, OUT, 4>, grid, block, st, a);
+}
+
+template <typename T, typename G> cudaError_t launch_norm_typed(const NormArgs& a, bool vec, cudaStream_t st)
+{
+    if (!vec) return launch_norm(norm_any_kernel<T, G>, a.m, 256, st, a);
+    switch (a.out) {
+        case kOutI8: return launch_norm_rows<T, G, kOutI8>(a, st);
+        case kOutE4M3: return launch_norm_rows<T, G, kOutE4M3>(a, st);
+        case kOutE5M2: return launch_norm_rows<T, G, kOutE5M2>(a, st);
+        default: return launch_norm_rows<T, G, kOutE2M1>(a, st);
+    }
+}
+
+// Bytes from the first element of a pitched matrix to the end of its last row
+size_t extent(uint32_t rows, uint32_t cols, int64_t ld, int size) { return (static_cast<size_t>(rows - 1) * static_cast<size_t>(ld) + cols) * size; }
+
+}  // namespace
+}  // namespace ascq
+
+extern "C" ascq_status ascq_residual_rms_norm_quant(void* dst, ascq_dtype dstT, void* scaleOut, void* residualOut, void* normOut, const void* src,
+                                                    const void* residual, const void* gamma, ascq_dtype srcT, ascq_dtype gammaT,
+                                                    const ascq_rms_norm_param* p, void* stream)
+{
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (!p) return fail(ASCQ_ERR_INVALID_ARG, "param must not be NULL");
+    auto is_float = [](ascq_dtype t) { return t == ASCQ_DT_F16 || t == ASCQ_DT_BF16 || t == ASCQ_DT_F32; };
+    if (!is_float(srcT)) return fail(ASCQ_ERR_UNSUPPORTED, "src dtype must be half, bfloat16_t or float");
+    if (gammaT != srcT && gammaT != ASCQ_DT_F32) return fail(ASCQ_ERR_UNSUPPORTED, "gamma must have src's dtype or float");
+    NormArgs a{};
+    switch (dstT) {
+        case ASCQ_DT_I8: a.out = kOutI8; break;
+        case ASCQ_DT_FP8_E4M3: a.out = kOutE4M3; break;
+        case ASCQ_DT_FP8_E5M2: a.out = kOutE5M2; break;
+        case ASCQ_DT_FP4X2_E2M1: a.out = kOutE2M1; break;
+        default: return fail(ASCQ_ERR_UNSUPPORTED, "dst dtype %d is not built (int8, fp8_e4m3, fp8_e5m2 and fp4x2_e2m1 are)", static_cast<int>(dstT));
+    }
+    if (!(p->epsilon > 0.f) || p->epsilon > 3.4028234663852886e38f) return fail(ASCQ_ERR_INVALID_ARG, "epsilon must be positive and finite");
+    if (a.out != kOutI8 && p->n % 32 != 0) return fail(ASCQ_ERR_INVALID_ARG, "n is %u, which must be a multiple of the MX block size 32", p->n);
+    if (p->m > 0x7FFFFFFFu || p->n > 0x7FFFFFFFu) return fail(ASCQ_ERR_INVALID_ARG, "m and n must be below 2^31");
+    auto pitch = [&](int64_t ld) { return ld == 0 ? static_cast<int64_t>(p->n) : ld; };
+    a.ldSrc = pitch(p->ldSrc);
+    a.ldResidual = pitch(p->ldResidual);
+    a.ldResidualOut = pitch(p->ldResidualOut);
+    a.ldNormOut = pitch(p->ldNormOut);
+    for (int64_t ld : {a.ldSrc, a.ldResidual, a.ldResidualOut, a.ldNormOut})
+        if (ld < static_cast<int64_t>(p->n)) return fail(ASCQ_ERR_INVALID_ARG, "a row pitch is %lld, which must be 0 or at least n = %u", static_cast<long long>(ld), p->n);
+    if (p->m == 0 || p->n == 0) return ASCQ_OK;
+    if (!dst || !scaleOut || !src || !gamma) return fail(ASCQ_ERR_INVALID_ARG, "dst, scaleOut, src and gamma must not be NULL");
+
+    const int es = dtype_size(srcT);
+    auto bad = [&](const void* q, uintptr_t by) { return (reinterpret_cast<uintptr_t>(q) & (by - 1)) != 0; };
+    if (bad(src, es) || bad(residual, es) || bad(residualOut, es) || bad(normOut, es) || bad(gamma, dtype_size(gammaT)) || (a.out == kOutI8 && bad(scaleOut, 4)))
+        return fail(ASCQ_ERR_ALIGNMENT, "a tensor is not aligned to its element type");
+    // outputs overlap nothing, except that residualOut may be src or residual itself (the same matrix with the same pitch)
+    const size_t elems = static_cast<size_t>(p->m) * p->n;
+    struct Span { const void* p; size_t bytes; int64_t ld; };
+    const Span in[3] = {{src, extent(p->m, p->n, a.ldSrc, es), a.ldSrc},
+                        {residual, residual ? extent(p->m, p->n, a.ldResidual, es) : 0, a.ldResidual},
+                        {gamma, static_cast<size_t>(p->n) * dtype_size(gammaT), 0}};
+    const Span out[4] = {{residualOut, residualOut ? extent(p->m, p->n, a.ldResidualOut, es) : 0, a.ldResidualOut},
+                         {normOut, normOut ? extent(p->m, p->n, a.ldNormOut, es) : 0, a.ldNormOut},
+                         {dst, a.out == kOutE2M1 ? elems / 2 : elems, 0},
+                         {scaleOut, a.out == kOutI8 ? p->m * size_t{4} : elems / 32, 0}};
+    for (int i = 0; i < 4; ++i) {
+        for (int j = 0; j < 3; ++j) {
+            const bool same = i == 0 && j < 2 && out[i].p == in[j].p && out[i].ld == in[j].ld;
+            if (!same && spans_overlap(out[i].p, out[i].bytes, in[j].p, in[j].bytes))
+                return fail(ASCQ_ERR_INVALID_ARG, "an output overlaps an input (only residualOut may be src or residual, with the same pitch)");
+        }
+        for (int j = 0; j < i; ++j)
+            if (spans_overlap(out[i].p, out[i].bytes, out[j].p, out[j].bytes)) return fail(ASCQ_ERR_INVALID_ARG, "two outputs overlap");
+    }
+
+    a.dst = dst; a.scaleOut = scaleOut; a.residualOut = residualOut; a.normOut = normOut;
+    a.src = src; a.residual = residual; a.gamma = gamma;
+    a.m = p->m; a.n = p->n; a.epsilon = p->epsilon;
+    // The vector kernel wants 16-byte vectors of 8 elements everywhere (codes: 8 or 4 bytes) and a row that fits its registers.
+    const bool vec = p->n % 8 == 0 && p->n / 8 <= kNormThreads * kNormMaxVectors && !bad(src, 16) && !bad(residual, 16) && !bad(residualOut, 16) &&
+                     !bad(normOut, 16) && !bad(gamma, 16) && !bad(dst, a.out == kOutE2M1 ? 4 : 8) && a.ldSrc * es % 16 == 0 &&
+                     (!residual || a.ldResidual * es % 16 == 0) && (!residualOut || a.ldResidualOut * es % 16 == 0) && (!normOut || a.ldNormOut * es % 16 == 0);
+    cudaError_t rc;
+    if (srcT == ASCQ_DT_F16) rc = gammaT == srcT ? launch_norm_typed<__half, __half>(a, vec, st) : launch_norm_typed<__half, float>(a, vec, st);
+    else if (srcT == ASCQ_DT_BF16) rc = gammaT == srcT ? launch_norm_typed<__nv_bfloat16, __nv_bfloat16>(a, vec, st) : launch_norm_typed<__nv_bfloat16, float>(a, vec, st);
+    else rc = launch_norm_typed<float, float>(a, vec, st);
+    ASCQ_CUDA_CHECK(rc);
+    return ASCQ_OK;
+}

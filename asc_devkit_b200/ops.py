@@ -128,6 +128,73 @@ def DynamicQuantMxfp4(dstTensor: torch.Tensor, scaleOut: torch.Tensor, srcTensor
     return dstTensor, scaleOut
 
 
+def _ptr_rows(t: Optional[torch.Tensor]):
+    """(pointer, row pitch in elements) of an optional 2-D tensor whose rows are contiguous but may be spaced by a pitch."""
+    if t is None:
+        return None, 0
+    if not t.is_cuda:
+        raise ValueError("ascq operators take CUDA tensors (there is no CPU path)")
+    m, n = t.shape if t.dim() == 2 else (-1, -1)
+    if m < 0 or (n > 1 and t.stride(1) != 1) or (m > 1 and t.stride(0) < n):
+        raise ValueError("expected a 2-D tensor with contiguous rows that do not overlap")
+    return C.c_void_p(t.data_ptr()), (t.stride(0) if m > 1 else n)
+
+
+def _on_device(fn, stream, *tensors):
+    """Calls ``fn(raw stream)`` with the tensors' device current.  All of them have to be on one device; a given stream
+    has to belong to it, otherwise its current stream is taken."""
+    dev = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise ValueError(f"the tensors of one call are on {dev} and {t.device}")
+    if stream is not None and stream.device != dev:
+        raise ValueError(f"the stream is on {stream.device}, the tensors are on {dev}")
+    if dev.type != "cuda":
+        raise ValueError("ascq operators take CUDA tensors (there is no CPU path)")
+    if dev.index == torch._C._cuda_getDevice():
+        return fn(_stream(stream))
+    with torch.cuda.device(dev):
+        return fn(_stream(stream))
+
+
+def _need(cond: bool, what: str):
+    if not cond:
+        raise ValueError(what)
+
+
+_MX_TARGETS = {L.DT_FP8_E4M3: 1, L.DT_FP8_E5M2: 1, L.DT_FP4X2_E2M1: 2}
+
+
+def ResidualRmsNormQuant(dstTensor: torch.Tensor, scaleOut: torch.Tensor, srcTensor: torch.Tensor, gamma: torch.Tensor, epsilon: float, *,
+                         residual: Optional[torch.Tensor] = None, residualOut: Optional[torch.Tensor] = None,
+                         normOut: Optional[torch.Tensor] = None, dst_dtype: int = L.DT_I8, stream=None):
+    """Residual addition, root-mean-square norm and quantisation in one launch (``ascq_residual_rms_norm_quant``):
+    ``h = src + residual``, ``y = h * gamma / sqrt(mean(h^2) + epsilon)``.
+
+    ``DT_I8``: dst int8 [m, n], scaleOut fp32 [m] (``max|y| / 127``: ``scaleA`` of MatmulW8A8 / GroupMatmulW8A8).
+    ``DT_FP8_E4M3`` / ``DT_FP8_E5M2``: dst uint8 [m, n], scaleOut uint8 [m, n/32] (e8m0); ``DT_FP4X2_E2M1``: dst uint8
+    [m, n/2].  ``residualOut`` takes ``h`` and ``normOut`` takes ``y`` in src's dtype; ``residualOut`` may be ``residual``
+    or ``srcTensor`` itself.  src, residual, residualOut and normOut are 2-D and may have a row pitch."""
+    m, n = srcTensor.shape
+    for t in (residual, residualOut, normOut):
+        _need(t is None or (t.shape == srcTensor.shape and t.dtype == srcTensor.dtype),
+              "residual, residualOut and normOut must have srcTensor's shape and dtype")
+    _need(gamma.shape == (n,), "gamma must have one element per column")
+    if dst_dtype == L.DT_I8:
+        _need(dstTensor.dtype == torch.int8 and dstTensor.shape == (m, n), "dstTensor must be int8 of srcTensor's shape")
+        _need(scaleOut.dtype == torch.float32 and scaleOut.numel() == m, "scaleOut must hold one float per row")
+    elif dst_dtype in _MX_TARGETS:
+        _need(dstTensor.element_size() == 1 and dstTensor.shape == (m, n // _MX_TARGETS[dst_dtype]),
+              "dstTensor must hold one byte per code (fp4: per two codes)")
+        _need(scaleOut.element_size() == 1 and scaleOut.numel() == m * (n // 32), "scaleOut must hold one byte per 32 elements")
+    (sp, ls), (rp, lr), (ro, lro), (no, lno) = _ptr_rows(srcTensor), _ptr_rows(residual), _ptr_rows(residualOut), _ptr_rows(normOut)
+    p = L.RmsNormParam(m, n, float(epsilon), ls, lr, lro, lno)
+    _on_device(lambda st: L.check(L.lib().ascq_residual_rms_norm_quant(
+        _ptr(dstTensor), dst_dtype, _ptr(scaleOut), ro, no, sp, rp, _ptr(gamma), dtype_code(srcTensor), dtype_code(gamma), C.byref(p), st)),
+        stream, srcTensor, dstTensor, scaleOut, gamma, residual, residualOut, normOut)
+    return dstTensor, scaleOut
+
+
 @dataclass
 class DequantParams:
     """include/adv_api/quantization/ascend_dequant_utils.h:26-30"""
@@ -343,6 +410,88 @@ def MatmulW4A16(C: torch.Tensor, A: torch.Tensor, B_nk_int4: torch.Tensor, offse
                                       0.0 if st else float(offset), 0.0 if st else float(scale), M, N, K, C.stride(0),
                                       _ptr(workspace), workspace.numel(), _stream(stream)))
     return C
+
+
+# ---- tokens into expert order and back, around the grouped matmuls ------------------------------------------------
+_ID_CODE = {torch.int32: L.DT_I32, torch.int64: L.DT_I64}
+
+
+def _id_code(t: torch.Tensor) -> int:
+    if t.dtype not in _ID_CODE:
+        raise TypeError(f"expert and adapter numbers are int32 or int64 tensors, not {t.dtype}")
+    return _ID_CODE[t.dtype]
+
+
+def ExpertSort(counts: torch.Tensor, rowOfSlot: torch.Tensor, expertIds: torch.Tensor, *, slotOfRow: Optional[torch.Tensor] = None,
+               stream=None):
+    """Orders the slots (a token's choices of an expert) by expert, equal ones by slot (``ascq_expert_sort``).  expertIds
+    int32 / int64, usually [tokens, k]; numbers outside ``[0, counts.numel())`` get no row.  counts int64 [experts] = rows per
+    expert (``counts.tolist()`` is the groupList of the grouped matmuls); rowOfSlot int32 of expertIds' shape (-1: no row); slotOfRow
+    int32 with as many elements (-1 behind the last row)."""
+    n = expertIds.numel()
+    _need(counts.dtype == torch.int64 and counts.dim() == 1, "counts must be an int64 vector with one element per expert")
+    _need(rowOfSlot.dtype == torch.int32 and rowOfSlot.numel() == n, "rowOfSlot must be int32 with one element per slot")
+    _need(slotOfRow is None or (slotOfRow.dtype == torch.int32 and slotOfRow.numel() == n), "slotOfRow must be int32 with one element per slot")
+    code = _id_code(expertIds)
+    _on_device(lambda st: L.check(L.lib().ascq_expert_sort(_ptr(counts), _ptr(rowOfSlot), _ptr(slotOfRow), _ptr(expertIds), code, n,
+                                                           counts.numel(), st)), stream, expertIds, counts, rowOfSlot, slotOfRow)
+    return counts, rowOfSlot
+
+
+def _slots(rowOfSlot: torch.Tensor, tokens: int) -> int:
+    _need(rowOfSlot.dtype == torch.int32 and rowOfSlot.dim() == 2 and rowOfSlot.shape[0] == tokens and rowOfSlot.shape[1] > 0,
+          "rowOfSlot must be int32 [tokens, k]")
+    return rowOfSlot.shape[1]
+
+
+def ExpertDispatch(dstTensor: torch.Tensor, srcTensor: torch.Tensor, rowOfSlot: torch.Tensor, *, dstScale: Optional[torch.Tensor] = None,
+                   srcScale: Optional[torch.Tensor] = None, stream=None):
+    """Copies every token's row to its experts' rows (``ascq_expert_dispatch``): ``dst[rowOfSlot[t, j]] = src[t]``.  src
+    [tokens, width] of any dtype (it may have a row pitch), dst [rows, width] of the same; srcScale / dstScale, a float per
+    token or a row of e8m0 scales per token, go along.  Rows that no slot names are left as they were."""
+    tokens, width = srcTensor.shape
+    _need(dstTensor.dim() == 2 and dstTensor.shape[1] == width and dstTensor.dtype == srcTensor.dtype, "dstTensor must be [rows, width] of srcTensor's dtype")
+    k, rows = _slots(rowOfSlot, tokens), dstTensor.shape[0]
+    scaleBytes = 0
+    _need((dstScale is None) == (srcScale is None), "dstScale and srcScale go together")
+    if srcScale is not None:
+        _need(srcScale.dtype == dstScale.dtype and srcScale.shape[:1] == (tokens,) and dstScale.shape == (rows,) + tuple(srcScale.shape[1:]),
+              "srcScale must be [tokens, ...] and dstScale [rows, ...] of the same dtype")
+        scaleBytes = srcScale[:1].numel() * srcScale.element_size() if tokens else 0
+    sp, ld = _ptr_rows(srcTensor)
+    es = srcTensor.element_size()
+    _on_device(lambda st: L.check(L.lib().ascq_expert_dispatch(_ptr(dstTensor), sp, width * es, ld * es, _ptr(dstScale), _ptr(srcScale), scaleBytes,
+                                                               _ptr(rowOfSlot), tokens, k, rows, st)),
+               stream, srcTensor, dstTensor, rowOfSlot, dstScale, srcScale)
+    return dstTensor
+
+
+def ExpertCombine(dstTensor: torch.Tensor, rows: torch.Tensor, rowOfSlot: torch.Tensor, weights: Optional[torch.Tensor] = None, *, stream=None):
+    """Brings the experts' rows back to their tokens (``ascq_expert_combine``): ``dst[t] = sum_j weights[t, j] *
+    rows[rowOfSlot[t, j]]`` in fp32.  ``weights`` fp32 [tokens, k]; without them it is the gradient of ExpertDispatch."""
+    tokens, h = dstTensor.shape
+    _need(rows.dim() == 2 and rows.shape[1] == h and rows.dtype == dstTensor.dtype, "rows must be [rows, h] of dstTensor's dtype")
+    k = _slots(rowOfSlot, tokens)
+    _need(weights is None or (weights.dtype == torch.float32 and weights.shape == rowOfSlot.shape), "weights must be float32 of rowOfSlot's shape")
+    _on_device(lambda st: L.check(L.lib().ascq_expert_combine(_ptr(dstTensor), _ptr(rows), dtype_code(rows), _ptr(rowOfSlot), _ptr(weights), tokens, k,
+                                                              rows.shape[0], h, st)), stream, dstTensor, rows, rowOfSlot, weights)
+    return dstTensor
+
+
+def ExpertCombineGrad(gradRows: Optional[torch.Tensor], gradWeights: Optional[torch.Tensor], gradOut: torch.Tensor, rows: torch.Tensor,
+                      rowOfSlot: torch.Tensor, weights: Optional[torch.Tensor] = None, *, stream=None):
+    """Gradient of ExpertCombine (``ascq_expert_combine_grad``): ``gradRows[rowOfSlot[t, j]] = weights[t, j] * gradOut[t]`` and
+    ``gradWeights[t, j] = <rows[rowOfSlot[t, j]], gradOut[t]>`` (fp32, 0 for slots without a row).  Either output may be None."""
+    tokens, h = gradOut.shape
+    _need(rows.dim() == 2 and rows.shape[1] == h and rows.dtype == gradOut.dtype, "rows must be [rows, h] of gradOut's dtype")
+    k = _slots(rowOfSlot, tokens)
+    _need(weights is None or (weights.dtype == torch.float32 and weights.shape == rowOfSlot.shape), "weights must be float32 of rowOfSlot's shape")
+    _need(gradRows is None or (gradRows.shape == rows.shape and gradRows.dtype == rows.dtype), "gradRows must have rows' shape and dtype")
+    _need(gradWeights is None or (gradWeights.dtype == torch.float32 and gradWeights.shape == rowOfSlot.shape), "gradWeights must be float32 of rowOfSlot's shape")
+    _on_device(lambda st: L.check(L.lib().ascq_expert_combine_grad(_ptr(gradRows), _ptr(gradWeights), _ptr(gradOut), _ptr(rows), dtype_code(rows),
+                                                                   _ptr(rowOfSlot), _ptr(weights), tokens, k, rows.shape[0], h, st)),
+               stream, gradOut, rows, rowOfSlot, gradRows, gradWeights, weights)
+    return gradRows, gradWeights
 
 
 def GroupMatmulMxfp4Workspace(sumM: int, G: int, K: int, N: int) -> int:

@@ -55,7 +55,8 @@ typedef enum {
     ASCQ_DT_FP8_E5M2 = 9,   /* targets or antiquant sources they are declared by the reference and not built here  */
     ASCQ_DT_HIF8 = 10,      /* declared by the reference, not built here: ASCQ_ERR_UNSUPPORTED */
     ASCQ_DT_FP4X2_E1M2 = 11,
-    ASCQ_DT_I4X2 = 12       /* int4b_t, two per byte (even element in the low nibble): AscendAntiQuant source only */
+    ASCQ_DT_I4X2 = 12,      /* int4b_t, two per byte (even element in the low nibble): AscendAntiQuant source only */
+    ASCQ_DT_I64 = 13        /* expert and adapter numbers (ascq_expert_sort, ascq_low_rank_add) */
 } ascq_dtype;
 
 /* include/adv_api/quantization/ascend_quant_utils.h:73-80 (same order in the
@@ -166,6 +167,32 @@ ascq_status ascq_dynamic_quant_mxfp4(uint8_t* dst_fp4, uint8_t* scale_e8m0, cons
                                      uint32_t n, void* stream);
 
 /*
+ * Residual addition, root-mean-square norm and quantisation of the result in one pass (no counterpart in the reference's
+ * quantization operators): the producer of the A operand of the W8A8 and MX matmuls from a transformer's residual stream.
+ *   h = src + residual  (fp32, not rounded; residual NULL: h = src)            residualOut = cast(h)  (NULL: not written)
+ *   y = h * gamma / sqrt(mean(h^2) + epsilon)   over the n elements of a row   normOut = cast(y)      (NULL: not written)
+ *   dstT I8:  scaleOut fp32 [m] = max|y| / 127 (1.0 for an all-zero row), dst [m, n] = RINT(y * 127 / max|y|): dst and
+ *             scaleOut are A and sA of ascq_matmul_w8a8 / ascq_group_matmul_w8a8.
+ *   dstT FP8_E4M3, FP8_E5M2, FP4X2_E2M1:  per block of 32 elements e = floor(log2 max|y|) - emax (8, 15, 2; 0 for an
+ *             all-zero block) clamped to [-127, 127], scaleOut E8M0 [m, n/32] = e + 127, dst = cast(y * 2^-e), to nearest
+ *             even and saturating (fp4 through bfloat16, as ascq_dynamic_quant_mxfp4): operands of ascq_group_matmul_mxfp8
+ *             / ascq_group_matmul_mxfp4.
+ * All arithmetic and both sums in fp32.  src, residual, residualOut, normOut have type srcT (half, bfloat16_t or float) and
+ * their own row pitches; gamma [n] has srcT or float; dst and scaleOut are contiguous.  A row whose sum of squares or
+ * largest |y| is not finite in fp32 (NaN, infinity, |h| beyond 1e19) gets scale NaN and codes 0 (MX: a block with such a y gets
+ * scale byte 0xFF and codes 0); residualOut is written as ever.  residualOut may be src or residual itself (same pitch); no other overlap is allowed.  Any n for int8,
+ * n % 32 == 0 for the MX types; unaligned tensors and rows beyond 16384 elements take a slower kernel.
+ */
+typedef struct ascq_rms_norm_param {
+    uint32_t m, n;        /* rows (tokens), elements of a row */
+    float epsilon;        /* > 0 */
+    int64_t ldSrc, ldResidual, ldResidualOut, ldNormOut;  /* row pitches in elements, 0 = n */
+} ascq_rms_norm_param;
+ascq_status ascq_residual_rms_norm_quant(void* dst, ascq_dtype dstT, void* scaleOut, void* residualOut, void* normOut,
+                                         const void* src, const void* residual, const void* gamma, ascq_dtype srcT,
+                                         ascq_dtype gammaT, const ascq_rms_norm_param* param, void* stream);
+
+/*
  * AscendDequant.  dst = cast(float(src) * scale), fp32 arithmetic, final cast RINT + saturate.
  *   PER_TENSOR  scalar deqScale overloads, include/adv_api/quantization/ascend_dequant.h:186-281
  *               (scaleScalar; `scale` NULL).
@@ -274,6 +301,37 @@ ascq_status ascq_matmul_w8a8(void* C_bf16, const int8_t* A, const int8_t* B_nk, 
 ascq_status ascq_group_matmul_w8a8(void* C, ascq_dtype cT, const int8_t* A, const int8_t* B_gnk, const float* sA_m,
                                    const float* sB_gn, const void* bias_bf16_gn, const int64_t* groupList_host,
                                    int G, int N, int K, int activation, void* stream);
+
+/*
+ * Tokens into expert order and back around the grouped matmuls (no counterpart in the reference, whose grouped sample gets its
+ * rows sorted).  A slot is a token's j-th choice of an expert, number t * k + j.
+ *
+ * ascq_expert_sort: expertIds [slots] (idT int32 or int64) -> counts int64 [numExperts] = rows of each expert (copied to the
+ *   host it is the groupList of the grouped matmuls), rowOfSlot int32 [slots] = the slot's row, slotOfRow int32 [slots]
+ *   (optional, may be NULL) = the row's slot.  Rows are ordered by expert, those of one expert by slot.  A slot whose number is
+ *   outside [0, numExperts) -- an expert of another rank, a padded token -- gets no row: rowOfSlot -1; slotOfRow is -1
+ *   behind the last row.  1 <= numExperts <= 1024, slots < 2^31.  One launch.
+ * ascq_expert_dispatch: dst[rowOfSlot[t * k + j]] = src[t], rows of rowBytes bytes (any element type, packed fp4 too), src with
+ *   a pitch of ldSrcBytes (0 = rowBytes), dst [rows] contiguous; dstScale / srcScale (optional) are rows of scaleRowBytes
+ *   bytes that go with them (4: a float per token; h / 32: E8M0 scales).  Each source row is read once.
+ * ascq_expert_combine: dst[t] = cast(sum_j weights[t, j] * in[rowOfSlot[t, j]]) in fp32, j ascending; T in half, bfloat16_t,
+ *   float; weights fp32 [tokens, k], NULL = 1 each.  With NULL it is the gradient of ascq_expert_dispatch.
+ * ascq_expert_combine_grad: gradRows[rowOfSlot[s]] = cast(weights[s] * gradOut[t]), gradWeights[s] = sum over h of
+ *   in[rowOfSlot[s]] * gradOut[t] (fp32); either output may be NULL (without gradWeights `in` is not read).
+ * In all three, slots with a row outside [0, rows) take no part (their gradWeights are 0, a token without rows combines to 0)
+ * and rows that no slot names are left as they were; two slots with the same row are the caller's error (which one's copy stays
+ * is not defined).  No output may overlap another tensor of the call.
+ */
+ascq_status ascq_expert_sort(int64_t* counts, int32_t* rowOfSlot, int32_t* slotOfRow, const void* expertIds, ascq_dtype idT,
+                             int64_t slots, int numExperts, void* stream);
+ascq_status ascq_expert_dispatch(void* dst, const void* src, size_t rowBytes, size_t ldSrcBytes, void* dstScale,
+                                 const void* srcScale, size_t scaleRowBytes, const int32_t* rowOfSlot, int64_t tokens, int k,
+                                 int64_t rows, void* stream);
+ascq_status ascq_expert_combine(void* dst, const void* in, ascq_dtype T, const int32_t* rowOfSlot, const float* weights,
+                                int64_t tokens, int k, int64_t rows, int64_t h, void* stream);
+ascq_status ascq_expert_combine_grad(void* gradRows, float* gradWeights, const void* gradOut, const void* in, ascq_dtype T,
+                                     const int32_t* rowOfSlot, const float* weights, int64_t tokens, int k, int64_t rows,
+                                     int64_t h, void* stream);
 
 /*
  * MX-FP4 grouped matmul (MatmulWithScalePolicy, impl/adv_api/detail/matmul/mx_matmul_impl.h:29-181;
