@@ -44,16 +44,16 @@ __device__ __forceinline__ void pdl_begin()
 // summed over the warps and, through distributed shared memory, over the cluster's CTAs, which gives each warp its first position in
 // every expert's run; a second walk over the same slots hands the positions out (equal keys inside a warp's step are
 // ranked with a match).  One launch, no scratch memory, and the order of equal keys is the slots' own.
-template <typename Id> __device__ __forceinline__ int sort_key(const Id* ids, int64_t s, int64_t end, int keys)
+template <typename Id> __device__ __forceinline__ int sort_key(const Id* ids, int64_t s, int64_t end, int keys, int outside)
 {
     if (s >= end) return -1;
     const Id v = ids[s];
-    return v >= 0 && v < static_cast<Id>(keys) ? static_cast<int>(v) : -1;
+    return v >= 0 && v < static_cast<Id>(keys) ? static_cast<int>(v) : outside;
 }
 
 template <typename Id>
 __global__ void __launch_bounds__(1024) key_sort_kernel(int64_t* counts, int32_t* rowOfSlot, int32_t* slotOfRow, const Id* ids, int64_t slots, int keys,
-                                                        int ctas)
+                                                        int outside, int ctas)
 {
     extern __shared__ uint32_t smem[];
     const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(1024) key_sort_kernel(int64_t* counts, int32_t
     const int64_t end = begin + perWarp < slots ? begin + perWarp : slots;
     uint32_t* mine = hist + warp * keys;
     for (int64_t s = begin; s < end; s += 32) {
-        const int key = sort_key<Id>(ids, s + lane, end, keys);
+        const int key = sort_key<Id>(ids, s + lane, end, keys, outside);
         if (key >= 0) atomicAdd(&mine[key], 1u);  // a count: the order of the additions does not show
     }
     __syncthreads();
@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(1024) key_sort_kernel(int64_t* counts, int32_t
     }
     __syncthreads();
     for (int64_t s = begin; s < end; s += 32) {
-        const int key = sort_key<Id>(ids, s + lane, end, keys);
+        const int key = sort_key<Id>(ids, s + lane, end, keys, outside);
         const uint32_t peers = __match_any_sync(0xFFFFFFFFu, key);
         uint32_t pos = 0;
         if (key >= 0) pos = first[key] + mine[key] + __popc(peers & ((1u << lane) - 1u));
@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(1024) key_sort_kernel(int64_t* counts, int32_t
 }
 
 template <typename Id> ascq_status launch_key_sort_typed(int64_t* counts, int32_t* rowOfSlot, int32_t* slotOfRow, const void* ids, int64_t slots, int keys,
-                                                         cudaStream_t st)
+                                                         int outside, cudaStream_t st)
 {
     // enough warps that each walks a few steps of 32 slots; a second CTA only once 32 warps walk more than 8 steps each
     unsigned threads = 128;
@@ -175,7 +175,8 @@ template <typename Id> ascq_status launch_key_sort_typed(int64_t* counts, int32_
         ASCQ_CUDA_CHECK(cudaFuncSetAttribute(key_sort_kernel<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, (34 * kMaxSortKeys + 64) * 4));
         once.mark(dev);
     }
-    ASCQ_CUDA_CHECK(launch_rows(key_sort_kernel<Id>, dim3(ctas), threads, smem, ctas, st, counts, rowOfSlot, slotOfRow, static_cast<const Id*>(ids), slots, keys, ctas));
+    ASCQ_CUDA_CHECK(launch_rows(key_sort_kernel<Id>, dim3(ctas), threads, smem, ctas, st, counts, rowOfSlot, slotOfRow, static_cast<const Id*>(ids), slots, keys,
+                                outside, ctas));
     return ASCQ_OK;
 }
 
@@ -389,10 +390,11 @@ ascq_status check_slots(const int32_t* rowOfSlot, int64_t tokens, int k, int64_t
 
 }  // namespace
 
-ascq_status launch_key_sort(int64_t* counts, int32_t* rowOfSlot, int32_t* slotOfRow, const void* ids, bool ids64, int64_t slots, int keys, ::CUstream_st* st)
+ascq_status launch_key_sort(int64_t* counts, int32_t* rowOfSlot, int32_t* slotOfRow, const void* ids, bool ids64, int64_t slots, int keys, int outside,
+                            ::CUstream_st* st)
 {
-    return ids64 ? launch_key_sort_typed<int64_t>(counts, rowOfSlot, slotOfRow, ids, slots, keys, st)
-                 : launch_key_sort_typed<int32_t>(counts, rowOfSlot, slotOfRow, ids, slots, keys, st);
+    return ids64 ? launch_key_sort_typed<int64_t>(counts, rowOfSlot, slotOfRow, ids, slots, keys, outside, st)
+                 : launch_key_sort_typed<int32_t>(counts, rowOfSlot, slotOfRow, ids, slots, keys, outside, st);
 }
 }  // namespace ascq
 
@@ -417,7 +419,7 @@ extern "C" ascq_status ascq_expert_sort(int64_t* counts, int32_t* rowOfSlot, int
         ASCQ_CUDA_CHECK(cudaMemsetAsync(counts, 0, static_cast<size_t>(numExperts) * 8, st));
         return ASCQ_OK;
     }
-    return launch_key_sort(counts, rowOfSlot, slotOfRow, expertIds, idT == ASCQ_DT_I64, slots, numExperts, st);
+    return launch_key_sort(counts, rowOfSlot, slotOfRow, expertIds, idT == ASCQ_DT_I64, slots, numExperts, -1, st);
 }
 
 extern "C" ascq_status ascq_expert_dispatch(void* dst, const void* src, size_t rowBytes, size_t ldSrcBytes, void* dstScale, const void* srcScale,

@@ -494,6 +494,31 @@ def ExpertCombineGrad(gradRows: Optional[torch.Tensor], gradWeights: Optional[to
     return gradRows, gradWeights
 
 
+def LowRankAdd(dstTensor: torch.Tensor, base: Optional[torch.Tensor], X: torch.Tensor, A: torch.Tensor, B: torch.Tensor, adapterIds: torch.Tensor, *,
+               scale: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None, stream=None):
+    """Low-rank adapters of many requests beside a shared projection (``ascq_low_rank_add``): ``dst[t] = base[t] + scale[a] *
+    (X[t] @ A[a].T) @ B[a].T`` with ``a = adapterIds[t]``; a token whose number is outside ``[0, L)`` keeps ``base[t]``.
+
+    X [M, K], A [L, r, K], B [L, N, r], base and dst [M, N], half or bfloat16 (X, base and dst may have a row pitch); base is the
+    projection's result, None for 0, or dst itself; adapterIds int32 or int64 [M]; scale fp32 [L]."""
+    M, K = X.shape
+    _need(A.dim() == 3 and A.shape[2] == K and B.dim() == 3 and B.shape[0] == A.shape[0] and B.shape[2] == A.shape[1], "A must be [L, r, K] and B [L, N, r]")
+    Lo, r, N = A.shape[0], A.shape[1], B.shape[1]
+    _need(dstTensor.shape == (M, N) and (base is None or base.shape == (M, N)), "base and dstTensor must be [M, N]")
+    _need(all(t is None or t.dtype == X.dtype for t in (dstTensor, base, A, B)), "X, A, B, base and dstTensor must have one dtype")
+    _need(adapterIds.shape == (M,), "adapterIds must be [M]")
+    _need(scale is None or (scale.dtype == torch.float32 and scale.shape == (Lo,)), "scale must be float32 [L]")
+    code, idc = dtype_code(X), _id_code(adapterIds)
+    need = int(L.lib().ascq_low_rank_add_workspace_size(M, Lo))
+    if need and workspace is None:
+        workspace = _workspace(need, X.device, stream)
+    (dp, ldd), (bp, ldb), (xp, ldx) = _ptr_rows(dstTensor), _ptr_rows(base), _ptr_rows(X)
+    _on_device(lambda st: L.check(L.lib().ascq_low_rank_add(dp, ldd, bp, ldb, xp, ldx, _ptr(A), _ptr(B), code, _ptr(adapterIds), idc, _ptr(scale), M, N, K, r,
+                                                            Lo, _ptr(workspace), workspace.numel() if workspace is not None else 0, st)),
+               stream, X, dstTensor, base, A, B, adapterIds, scale, workspace)
+    return dstTensor
+
+
 def GroupMatmulMxfp4Workspace(sumM: int, G: int, K: int, N: int) -> int:
     return int(L.lib().ascq_group_matmul_mxfp4_workspace_size(sumM, G, K, N))
 

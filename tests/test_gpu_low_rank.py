@@ -1,0 +1,228 @@
+"""LowRankAdd against its formula in 64 bits.
+
+Tolerance, with u = 2^-24 and s the half step of the output's type.  The inner product of K terms and the second one of r terms run in the
+tensor cores' fp32 accumulators, which may truncate where fp32 arithmetic rounds: at most 2 u of the terms' absolute sum
+per addition.  The inner product enters the second as two 16-bit values: what they leave out is s^2 of it, and no more than
+2^-35 of the row's largest where fp16's subnormals end.  The scale and the addition of base add a few u, the result's rounding s of it."""
+import ctypes as C
+
+import pytest
+import torch
+
+from asc_devkit_b200 import _lib as L
+from asc_devkit_b200 import ops
+
+gpu = pytest.mark.gpu
+DEV = "cuda:0"
+U = 2.0 ** -24
+HALF_STEP = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+
+
+def case(m, n, k, r, lo, dt, span=1, seed=0, ids=None):
+    g = torch.Generator().manual_seed(seed + 7 * m + n + 3 * k + r + lo)
+    x = torch.randn(m, k, generator=g).to(dt)
+    base = torch.randn(m, n, generator=g).to(dt)
+    a = (torch.randn(lo, r, k, generator=g) * k ** -0.5).to(dt)
+    b = (torch.randn(lo, n, r, generator=g) * r ** -0.5).to(dt)
+    scale = 0.5 + torch.rand(lo, generator=g)
+    if ids is None:
+        ids = torch.randint(-1, lo, (-(-m // span),), generator=g).repeat_interleave(span)[:m]
+    return [t.to(DEV) for t in (x, base, a, b, scale, ids.to(torch.int32))]
+
+
+def check(got, x, base, a, b, scale, ids):
+    dt, k, r = x.dtype, x.shape[1], a.shape[1]
+    want = base.double() if base is not None else torch.zeros(got.shape, dtype=torch.float64, device=DEV)
+    tol = torch.zeros_like(want)
+    for e in range(a.shape[0]):
+        at = (ids == e).nonzero()[:, 0]
+        if not len(at):
+            continue
+        s = float(scale[e]) if scale is not None else 1.0
+        xa, aa, ba = x[at].double(), a[e].double(), b[e].double()
+        inner, mag = xa @ aa.T, xa.abs() @ aa.abs().T
+        want[at] += s * (inner @ ba.T)
+        off = mag * (2 * (k + 2 * r + 8) * U) + inner.abs() * HALF_STEP[dt] ** 2 + inner.abs().amax(-1, keepdim=True) * 2.0 ** -35
+        tol[at] += abs(s) * (off @ ba.abs().T)
+    tol += (want.abs() + tol) * (HALF_STEP[dt] + 4 * U) + (2.0 ** -25 if dt == torch.float16 else 0.0)  # half a step among fp16's subnormals
+    none = (ids < 0) | (ids >= a.shape[0])
+    if base is not None:
+        assert torch.equal(got[none], base[none])
+    else:
+        assert (got[none] == 0).all()
+    worst = ((got.double() - want).abs() - tol).max() if got.numel() else 0
+    assert worst <= 0, f"{float(worst)} beyond the bound"
+
+
+SHAPES = [  # m, n, k, r, adapters, tokens of a request
+    (1, 8, 8, 8, 1, 1), (1, 4096, 4096, 16, 16, 1), (32, 4096, 4096, 16, 16, 1), (5, 264, 520, 8, 3, 1), (17, 1000, 72, 24, 2, 1), (16, 96, 2048, 40, 40, 1),
+    (64, 512, 1024, 64, 64, 1), (200, 2048, 512, 128, 5, 33), (1024, 256, 512, 16, 1000, 1), (1025, 256, 512, 32, 1023, 1), (1337, 640, 1376, 32, 8, 97),
+    (2500, 264, 136, 64, 3, 700), (3000, 520, 1032, 104, 7, 1), (1100, 4096, 256, 128, 4, 300), (4096, 1024, 1024, 64, 16, 256)]
+
+
+@gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,n,k,r,lo,span", SHAPES)
+def test_against_the_formula(m, n, k, r, lo, span, dt):
+    x, base, a, b, scale, ids = case(m, n, k, r, lo, dt, span)
+    for bs, sc, i in ((base, scale, ids), (None, None, ids.long())):
+        got = torch.full((m, n), 3.0, dtype=dt, device=DEV)
+        ops.LowRankAdd(got, bs, x, a, b, i, scale=sc)
+        check(got, x, bs, a, b, sc, ids)
+
+
+@gpu
+@pytest.mark.parametrize("m", [1, 16, 40, 1500])
+def test_one_adapter_or_none_for_all(m):
+    for value in (0, 2, -1, 3, 2 ** 31 - 1):
+        x, base, a, b, scale, ids = case(m, 136, 264, 16, 3, torch.bfloat16, ids=torch.full((m,), value))
+        got = torch.empty_like(base)
+        ops.LowRankAdd(got, base, x, a, b, ids, scale=scale)
+        check(got, x, base, a, b, scale, ids)
+
+
+@gpu
+@pytest.mark.parametrize("m", [48, 1200])
+def test_in_place_pitched_rows_and_repeated_calls(m):
+    x, base, a, b, scale, ids = case(m, 256, 512, 32, 6, torch.float16)
+    want = torch.empty_like(base)
+    ops.LowRankAdd(want, base, x, a, b, ids, scale=scale)
+    wide = torch.full((m, 256 + 24), 5.0, dtype=torch.float16, device=DEV)
+    wide[:, 8:264] = base
+    xw = torch.full((m, 512 + 16), 9.0, dtype=torch.float16, device=DEV)
+    xw[:, 16:] = x
+    ops.LowRankAdd(wide[:, 8:264], wide[:, 8:264], xw[:, 16:], a, b, ids, scale=scale)
+    assert torch.equal(wide[:, 8:264], want) and (wide[:, :8] == 5).all() and (wide[:, 264:] == 5).all()
+    for _ in range(3):
+        again = torch.empty_like(base)
+        ops.LowRankAdd(again, base, x, a, b, ids, scale=scale)
+        assert torch.equal(again, want)
+
+
+@gpu
+def test_large_and_small_inner_products():
+    """Inner products beyond fp16's range and among its subnormals: the second product brings them back."""
+    x, base, a, b, scale, ids = case(40, 128, 256, 16, 2, torch.float16, ids=torch.zeros(40))
+    for fx, fb in ((2000.0, 2.0 ** -14), (2.0 ** -14, 1000.0)):
+        xs, bs = (x.float() * fx).to(torch.float16), (b.float() * fb).to(torch.float16)
+        got = torch.empty_like(base)
+        ops.LowRankAdd(got, None, xs, a, bs, ids, scale=scale)
+        check(got, xs, None, a, bs, scale, ids)
+
+
+@gpu
+def test_values_that_are_not_finite_stay_in_their_token():
+    x, base, a, b, scale, ids = case(60, 64, 128, 16, 3, torch.bfloat16)
+    want = torch.empty_like(base)
+    ops.LowRankAdd(want, base, x, a, b, ids, scale=scale)
+    t = int((ids >= 0).nonzero()[3])
+    x2 = x.clone()
+    x2[t, 5] = float("nan")
+    got = torch.empty_like(base)
+    ops.LowRankAdd(got, base, x2, a, b, ids, scale=scale)
+    rest = torch.arange(60, device=DEV) != t
+    assert torch.equal(got[rest], want[rest]) and torch.isnan(got[t]).all()
+    # NaN in the input of a token without an adapter, and in an adapter that no token uses
+    none = int((ids < 0).nonzero()[0])
+    x2 = x.clone()
+    x2[none] = float("nan")
+    ops.LowRankAdd(got, base, x2, a, b, ids, scale=scale)
+    assert torch.equal(got, want)
+    a2, b2 = torch.cat([a, torch.full_like(a[:1], float("nan"))]), torch.cat([b, torch.full_like(b[:1], float("nan"))])
+    ops.LowRankAdd(got, base, x, a2, b2, ids, scale=torch.cat([scale, scale[:1]]))
+    assert torch.equal(got, want)
+
+
+@gpu
+def test_result_that_overflows_saturates():
+    x = torch.full((2, 8), 100.0, dtype=torch.float16, device=DEV)
+    a, b = torch.full((1, 8, 8), 10.0, dtype=torch.float16, device=DEV), torch.full((1, 8, 8), 10.0, dtype=torch.float16, device=DEV)
+    got = torch.empty(2, 8, dtype=torch.float16, device=DEV)
+    ops.LowRankAdd(got, None, x, a, b, torch.tensor([0, -1], dtype=torch.int32, device=DEV))
+    assert (got[0] == 65504).all() and (got[1] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("m", [64, 1100])
+def test_other_stream_and_capture(m):
+    x, base, a, b, scale, ids = case(m, 256, 512, 16, 8, torch.bfloat16)
+    want = torch.empty_like(base)
+    ops.LowRankAdd(want, base, x, a, b, ids, scale=scale)
+    s = torch.cuda.Stream()
+    got = torch.zeros_like(base)
+    s.wait_stream(torch.cuda.current_stream())
+    ops.LowRankAdd(got, base, x, a, b, ids, scale=scale, stream=s)
+    s.synchronize()
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.LowRankAdd(got, base, x, a, b, ids, scale=scale)
+        ops.LowRankAdd(got, got, x, a, b, ids, scale=scale)
+    twice = torch.empty_like(base)
+    ops.LowRankAdd(twice, want, x, a, b, ids, scale=scale)
+    for _ in range(2):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, twice)
+
+
+@gpu
+def test_beside_the_w8a8_projection():
+    """One decode step of a projection with adapters: int8 matmul, then the adapters on its result in place."""
+    m, n, k, r, lo = 24, 512, 1024, 16, 5
+    x, _, a, b, scale, ids = case(m, n, k, r, lo, torch.bfloat16)
+    g = torch.ones(k, dtype=torch.bfloat16, device=DEV)
+    q, qs, y = torch.empty(m, k, dtype=torch.int8, device=DEV), torch.empty(m, device=DEV), torch.empty_like(x)
+    ops.ResidualRmsNormQuant(q, qs, x, g, 1e-6, normOut=y)
+    w = torch.randint(-127, 128, (n, k), dtype=torch.int8, device=DEV)
+    ws = 0.001 * torch.rand(n, device=DEV)
+    c = torch.empty(m, n, dtype=torch.bfloat16, device=DEV)
+    ops.MatmulW8A8(c, q, w, qs, ws)
+    base = c.clone()
+    ops.LowRankAdd(c, c, y, a, b, ids, scale=scale)
+    check(c, y, base, a, b, scale, ids)
+
+
+@gpu
+def test_empty():
+    e = lambda *s: torch.empty(*s, dtype=torch.float16, device=DEV)  # noqa: E731
+    ops.LowRankAdd(e(0, 16), e(0, 16), e(0, 8), e(2, 8, 8), e(2, 16, 8), torch.empty(0, dtype=torch.int32, device=DEV))
+
+
+# ---- refusals ---------------------------------------------------------------------------------------------------------
+def test_refusals():
+    P = lambda v: None if v is None else C.c_void_p(v)  # noqa: E731
+
+    def call(dst=0x1000000, ldd=0, base=0x2000000, ldb=0, x=0x3000000, ldx=0, a=0x4000000, b=0x5000000, dt=L.DT_BF16, ids=0x6000000, idt=L.DT_I32, sc=None, m=4,
+             n=64, k=64, r=16, lo=3, ws=None, wsb=0):
+        return L.lib().ascq_low_rank_add(P(dst), ldd, P(base), ldb, P(x), ldx, P(a), P(b), dt, P(ids), idt, P(sc), m, n, k, r, lo, P(ws), wsb, None)
+    assert call(dt=L.DT_F32) == L.ERR_UNSUPPORTED
+    assert call(idt=L.DT_I8) == L.ERR_UNSUPPORTED
+    for bad in (dict(m=-1), dict(n=-8), dict(k=0), dict(n=60), dict(k=60), dict(r=0), dict(r=12), dict(r=136), dict(lo=0), dict(lo=1024), dict(ldd=56), dict(ldx=8), dict(ldb=8),
+                dict(dst=None), dict(x=None), dict(a=None), dict(b=None), dict(ids=None), dict(dst=0x3000000), dict(dst=0x5000010), dict(dst=0x2000010),
+                dict(dst=0x2000000, ldd=72), dict(m=2000), dict(m=2000, ws=0x7000000, wsb=8031), dict(m=2000, ws=0x3000000, wsb=1 << 20)):
+        assert call(**bad) == L.ERR_INVALID_ARG, bad
+    for bad in (dict(dst=0x1000008), dict(x=0x3000002), dict(ldd=68), dict(ldx=68), dict(ids=0x6000002), dict(ids=0x6000004, idt=L.DT_I64), dict(sc=0x8000001),
+                dict(m=2000, ws=0x7000004, wsb=1 << 20)):
+        assert call(**bad) == L.ERR_ALIGNMENT, bad
+    assert L.lib().ascq_low_rank_add_workspace_size(1024, 8) == 0
+    assert L.lib().ascq_low_rank_add_workspace_size(2000, 3) == 4 * 8 + 2000 * 4
+
+
+def test_python_refusals():
+    z = lambda *s: torch.zeros(*s, dtype=torch.float16)  # noqa: E731
+    ids = torch.zeros(4, dtype=torch.int32)
+    good = [z(4, 16), z(4, 16), z(4, 8), z(2, 8, 8), z(2, 16, 8), ids]
+    for i, bad, text in ((0, z(4, 8), "base and dst"), (1, z(3, 16), "base and dst"), (3, z(2, 8, 16), "A must be"), (4, z(1, 16, 8), "A must be"),
+                         (4, z(2, 16, 8).float(), "one dtype"), (5, ids[:3], "adapterIds")):
+        args = list(good)
+        args[i] = bad
+        with pytest.raises(ValueError, match=text):
+            ops.LowRankAdd(*args)
+    with pytest.raises(ValueError, match="scale"):
+        ops.LowRankAdd(*good, scale=torch.zeros(3))
+    with pytest.raises(TypeError):
+        ops.LowRankAdd(*good[:5], ids.float())
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        ops.LowRankAdd(*good)
