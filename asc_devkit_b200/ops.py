@@ -128,33 +128,55 @@ def DynamicQuantMxfp4(dstTensor: torch.Tensor, scaleOut: torch.Tensor, srcTensor
     return dstTensor, scaleOut
 
 
-def _ptr_rows(t: Optional[torch.Tensor]):
-    """(pointer, row pitch in elements) of an optional 2-D tensor whose rows are contiguous but may be spaced by a pitch."""
+def _rows(t: Optional[torch.Tensor], dev: int):
+    """(address, row pitch in elements) of an optional 2-D tensor on device ``dev`` whose rows are contiguous but may be
+    spaced by a pitch."""
     if t is None:
         return None, 0
-    if not t.is_cuda:
-        raise ValueError("ascq operators take CUDA tensors (there is no CPU path)")
-    m, n = t.shape if t.dim() == 2 else (-1, -1)
-    if m < 0 or (n > 1 and t.stride(1) != 1) or (m > 1 and t.stride(0) < n):
+    if t.get_device() != dev:
+        raise ValueError(f"the tensors of one call are on cuda:{dev} and {t.device}")
+    if t.is_contiguous():
+        return t.data_ptr(), 0
+    m, n = t.shape
+    if (n > 1 and t.stride(1) != 1) or (m > 1 and t.stride(0) < n):
         raise ValueError("expected a 2-D tensor with contiguous rows that do not overlap")
-    return C.c_void_p(t.data_ptr()), (t.stride(0) if m > 1 else n)
+    return t.data_ptr(), (t.stride(0) if m > 1 else n)
 
 
-def _on_device(fn, stream, *tensors):
-    """Calls ``fn(raw stream)`` with the tensors' device current.  All of them have to be on one device; a given stream
-    has to belong to it, otherwise its current stream is taken."""
-    dev = tensors[0].device
-    for t in tensors:
-        if t is not None and t.device != dev:
-            raise ValueError(f"the tensors of one call are on {dev} and {t.device}")
-    if stream is not None and stream.device != dev:
-        raise ValueError(f"the stream is on {stream.device}, the tensors are on {dev}")
-    if dev.type != "cuda":
+def _whole(t: Optional[torch.Tensor], dev: int):
+    """Address of an optional contiguous tensor on device ``dev``."""
+    if t is None:
+        return None
+    if t.get_device() != dev:
+        raise ValueError(f"the tensors of one call are on cuda:{dev} and {t.device}")
+    if not t.is_contiguous():
+        raise ValueError("ascq operators take contiguous tensors")
+    return t.data_ptr()
+
+
+def _cuda_index(t: torch.Tensor) -> int:
+    dev = t.get_device()
+    if dev < 0:
         raise ValueError("ascq operators take CUDA tensors (there is no CPU path)")
-    if dev.index == torch._C._cuda_getDevice():
-        return fn(_stream(stream))
-    with torch.cuda.device(dev):
-        return fn(_stream(stream))
+    return dev
+
+
+def _launch(fn, dev: int, stream: Optional[torch.cuda.Stream], *args):
+    """``fn(*args, raw stream)`` with device ``dev`` current, on ``stream`` (which has to be on that device) or on the device's
+    current stream."""
+    if stream is None:
+        raw = torch._C._cuda_getCurrentRawStream(dev)
+    else:
+        if stream.device_index != dev:
+            raise ValueError(f"the stream is on cuda:{stream.device_index}, the tensors are on cuda:{dev}")
+        raw = stream.cuda_stream
+    if torch._C._cuda_getDevice() == dev:
+        rc = fn(*args, raw)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, raw)
+    if rc:
+        L.check(rc)
 
 
 def _need(cond: bool, what: str):
@@ -187,11 +209,10 @@ def ResidualRmsNormQuant(dstTensor: torch.Tensor, scaleOut: torch.Tensor, srcTen
         _need(dstTensor.element_size() == 1 and dstTensor.shape == (m, n // _MX_TARGETS[dst_dtype]),
               "dstTensor must hold one byte per code (fp4: per two codes)")
         _need(scaleOut.element_size() == 1 and scaleOut.numel() == m * (n // 32), "scaleOut must hold one byte per 32 elements")
-    (sp, ls), (rp, lr), (ro, lro), (no, lno) = _ptr_rows(srcTensor), _ptr_rows(residual), _ptr_rows(residualOut), _ptr_rows(normOut)
-    p = L.RmsNormParam(m, n, float(epsilon), ls, lr, lro, lno)
-    _on_device(lambda st: L.check(L.lib().ascq_residual_rms_norm_quant(
-        _ptr(dstTensor), dst_dtype, _ptr(scaleOut), ro, no, sp, rp, _ptr(gamma), dtype_code(srcTensor), dtype_code(gamma), C.byref(p), st)),
-        stream, srcTensor, dstTensor, scaleOut, gamma, residual, residualOut, normOut)
+    dev = _cuda_index(srcTensor)
+    (sp, ls), (rp, lr), (ro, lro), (no, lno) = _rows(srcTensor, dev), _rows(residual, dev), _rows(residualOut, dev), _rows(normOut, dev)
+    _launch(L.lib().ascq_residual_rms_norm_quant, dev, stream, _whole(dstTensor, dev), dst_dtype, _whole(scaleOut, dev), ro, no, sp, rp, _whole(gamma, dev),
+            dtype_code(srcTensor), dtype_code(gamma), L.RmsNormParam(m, n, epsilon, ls, lr, lro, lno))
     return dstTensor, scaleOut
 
 
@@ -433,8 +454,9 @@ def ExpertSort(counts: torch.Tensor, rowOfSlot: torch.Tensor, expertIds: torch.T
     _need(rowOfSlot.dtype == torch.int32 and rowOfSlot.numel() == n, "rowOfSlot must be int32 with one element per slot")
     _need(slotOfRow is None or (slotOfRow.dtype == torch.int32 and slotOfRow.numel() == n), "slotOfRow must be int32 with one element per slot")
     code = _id_code(expertIds)
-    _on_device(lambda st: L.check(L.lib().ascq_expert_sort(_ptr(counts), _ptr(rowOfSlot), _ptr(slotOfRow), _ptr(expertIds), code, n,
-                                                           counts.numel(), st)), stream, expertIds, counts, rowOfSlot, slotOfRow)
+    dev = _cuda_index(expertIds)
+    _launch(L.lib().ascq_expert_sort, dev, stream, _whole(counts, dev), _whole(rowOfSlot, dev), _whole(slotOfRow, dev), _whole(expertIds, dev), code, n,
+            counts.numel())
     return counts, rowOfSlot
 
 
@@ -457,12 +479,12 @@ def ExpertDispatch(dstTensor: torch.Tensor, srcTensor: torch.Tensor, rowOfSlot: 
     if srcScale is not None:
         _need(srcScale.dtype == dstScale.dtype and srcScale.shape[:1] == (tokens,) and dstScale.shape == (rows,) + tuple(srcScale.shape[1:]),
               "srcScale must be [tokens, ...] and dstScale [rows, ...] of the same dtype")
-        scaleBytes = srcScale[:1].numel() * srcScale.element_size() if tokens else 0
-    sp, ld = _ptr_rows(srcTensor)
+        scaleBytes = srcScale.numel() // tokens * srcScale.element_size() if tokens else 0
+    dev = _cuda_index(srcTensor)
+    sp, ld = _rows(srcTensor, dev)
     es = srcTensor.element_size()
-    _on_device(lambda st: L.check(L.lib().ascq_expert_dispatch(_ptr(dstTensor), sp, width * es, ld * es, _ptr(dstScale), _ptr(srcScale), scaleBytes,
-                                                               _ptr(rowOfSlot), tokens, k, rows, st)),
-               stream, srcTensor, dstTensor, rowOfSlot, dstScale, srcScale)
+    _launch(L.lib().ascq_expert_dispatch, dev, stream, _whole(dstTensor, dev), sp, width * es, ld * es, _whole(dstScale, dev), _whole(srcScale, dev), scaleBytes,
+            _whole(rowOfSlot, dev), tokens, k, rows)
     return dstTensor
 
 
@@ -473,8 +495,9 @@ def ExpertCombine(dstTensor: torch.Tensor, rows: torch.Tensor, rowOfSlot: torch.
     _need(rows.dim() == 2 and rows.shape[1] == h and rows.dtype == dstTensor.dtype, "rows must be [rows, h] of dstTensor's dtype")
     k = _slots(rowOfSlot, tokens)
     _need(weights is None or (weights.dtype == torch.float32 and weights.shape == rowOfSlot.shape), "weights must be float32 of rowOfSlot's shape")
-    _on_device(lambda st: L.check(L.lib().ascq_expert_combine(_ptr(dstTensor), _ptr(rows), dtype_code(rows), _ptr(rowOfSlot), _ptr(weights), tokens, k,
-                                                              rows.shape[0], h, st)), stream, dstTensor, rows, rowOfSlot, weights)
+    dev = _cuda_index(dstTensor)
+    _launch(L.lib().ascq_expert_combine, dev, stream, _whole(dstTensor, dev), _whole(rows, dev), dtype_code(rows), _whole(rowOfSlot, dev), _whole(weights, dev),
+            tokens, k, rows.shape[0], h)
     return dstTensor
 
 
@@ -488,9 +511,9 @@ def ExpertCombineGrad(gradRows: Optional[torch.Tensor], gradWeights: Optional[to
     _need(weights is None or (weights.dtype == torch.float32 and weights.shape == rowOfSlot.shape), "weights must be float32 of rowOfSlot's shape")
     _need(gradRows is None or (gradRows.shape == rows.shape and gradRows.dtype == rows.dtype), "gradRows must have rows' shape and dtype")
     _need(gradWeights is None or (gradWeights.dtype == torch.float32 and gradWeights.shape == rowOfSlot.shape), "gradWeights must be float32 of rowOfSlot's shape")
-    _on_device(lambda st: L.check(L.lib().ascq_expert_combine_grad(_ptr(gradRows), _ptr(gradWeights), _ptr(gradOut), _ptr(rows), dtype_code(rows),
-                                                                   _ptr(rowOfSlot), _ptr(weights), tokens, k, rows.shape[0], h, st)),
-               stream, gradOut, rows, rowOfSlot, gradRows, gradWeights, weights)
+    dev = _cuda_index(gradOut)
+    _launch(L.lib().ascq_expert_combine_grad, dev, stream, _whole(gradRows, dev), _whole(gradWeights, dev), _whole(gradOut, dev), _whole(rows, dev),
+            dtype_code(rows), _whole(rowOfSlot, dev), _whole(weights, dev), tokens, k, rows.shape[0], h)
     return gradRows, gradWeights
 
 
@@ -509,13 +532,14 @@ def LowRankAdd(dstTensor: torch.Tensor, base: Optional[torch.Tensor], X: torch.T
     _need(adapterIds.shape == (M,), "adapterIds must be [M]")
     _need(scale is None or (scale.dtype == torch.float32 and scale.shape == (Lo,)), "scale must be float32 [L]")
     code, idc = dtype_code(X), _id_code(adapterIds)
-    need = int(L.lib().ascq_low_rank_add_workspace_size(M, Lo))
-    if need and workspace is None:
-        workspace = _workspace(need, X.device, stream)
-    (dp, ldd), (bp, ldb), (xp, ldx) = _ptr_rows(dstTensor), _ptr_rows(base), _ptr_rows(X)
-    _on_device(lambda st: L.check(L.lib().ascq_low_rank_add(dp, ldd, bp, ldb, xp, ldx, _ptr(A), _ptr(B), code, _ptr(adapterIds), idc, _ptr(scale), M, N, K, r,
-                                                            Lo, _ptr(workspace), workspace.numel() if workspace is not None else 0, st)),
-               stream, X, dstTensor, base, A, B, adapterIds, scale, workspace)
+    dev = _cuda_index(X)
+    if workspace is None:
+        need = L.lib().ascq_low_rank_add_workspace_size(M, r, Lo)
+        if need:
+            workspace = _workspace(need, X.device, stream)
+    (dp, ldd), (bp, ldb), (xp, ldx) = _rows(dstTensor, dev), _rows(base, dev), _rows(X, dev)
+    _launch(L.lib().ascq_low_rank_add, dev, stream, dp, ldd, bp, ldb, xp, ldx, _whole(A, dev), _whole(B, dev), code, _whole(adapterIds, dev), idc,
+            _whole(scale, dev), M, N, K, r, Lo, _whole(workspace, dev), workspace.numel() if workspace is not None else 0)
     return dstTensor
 
 

@@ -201,13 +201,15 @@ def test_refusals():
     assert call(idt=L.DT_I8) == L.ERR_UNSUPPORTED
     for bad in (dict(m=-1), dict(n=-8), dict(k=0), dict(n=60), dict(k=60), dict(r=0), dict(r=12), dict(r=136), dict(lo=0), dict(lo=1024), dict(ldd=56), dict(ldx=8), dict(ldb=8),
                 dict(dst=None), dict(x=None), dict(a=None), dict(b=None), dict(ids=None), dict(dst=0x3000000), dict(dst=0x5000010), dict(dst=0x2000010),
-                dict(dst=0x2000000, ldd=72), dict(m=2000), dict(m=2000, ws=0x7000000, wsb=8031), dict(m=2000, ws=0x3000000, wsb=1 << 20)):
+                dict(dst=0x2000000, ldd=72), dict(m=2000), dict(m=2000, ws=0x7000000, wsb=1000), dict(m=2000, ws=0x3000000, wsb=1 << 20)):
         assert call(**bad) == L.ERR_INVALID_ARG, bad
     for bad in (dict(dst=0x1000008), dict(x=0x3000002), dict(ldd=68), dict(ldx=68), dict(ids=0x6000002), dict(ids=0x6000004, idt=L.DT_I64), dict(sc=0x8000001),
-                dict(m=2000, ws=0x7000004, wsb=1 << 20)):
+                dict(m=2000, ws=0x7000008, wsb=1 << 20)):
         assert call(**bad) == L.ERR_ALIGNMENT, bad
-    assert L.lib().ascq_low_rank_add_workspace_size(1024, 8) == 0
-    assert L.lib().ascq_low_rank_add_workspace_size(2000, 3) == 4 * 8 + 2000 * 4
+    size = L.lib().ascq_low_rank_add_workspace_size
+    assert size(1024, 16, 8) == 0
+    assert size(2000, 16, 1000) == 8016 + 2000 * 4                       # counts and order
+    assert size(2000, 64, 3) == 32 + 8000 + (2000 // 64 + 4) * 16 + 8000 + 2000 * 2 * 64 * 2  # and tiles, units and the inner products
 
 
 def test_python_refusals():
