@@ -231,10 +231,9 @@ template <typename T, int NB> __global__ void __launch_bounds__(32 * kWarps) low
                 w[n] = kIn && n * 8 + g < p.r ? __ldg(reinterpret_cast<const uint4*>(a + static_cast<size_t>(n * 8 + g) * p.K + k)) : zero;
             const uint32_t f0[4] = {u0.x, u1.x, u0.y, u1.y}, f1[4] = {u0.z, u1.z, u0.w, u1.w};
 #pragma unroll
-            for (int n = 0; n < NB; ++n) {
-                mma16816<T>(acc[n], f0, w[n].x, w[n].y);
-                mma16816<T>(acc[n], f1, w[n].z, w[n].w);
-            }
+            for (int n = 0; n < NB; ++n) mma16816<T>(acc[n], f0, w[n].x, w[n].y);
+#pragma unroll
+            for (int n = 0; n < NB; ++n) mma16816<T>(acc[n], f1, w[n].z, w[n].w);
         }
         __syncthreads();  // the tile finder's scratch is read no more
 #pragma unroll
@@ -451,16 +450,18 @@ template <typename T, int NB> __global__ void __launch_bounds__(32 * kLongWarps)
                 const uint4(&f)[4] = xs[d][s];
                 const uint32_t f0[2][4] = {{f[0].x, f[1].x, f[0].y, f[1].y}, {f[2].x, f[3].x, f[2].y, f[3].y}};
                 const uint32_t f1[2][4] = {{f[0].z, f[1].z, f[0].w, f[1].w}, {f[2].z, f[3].z, f[2].w, f[3].w}};
+                uint4 w[NBW];
 #pragma unroll
-                for (int n = 0; n < NBW; ++n) {
-                    const int row = (wr * NBW + n) * 8 + g;
-                    const uint4 w = *reinterpret_cast<const uint4*>(slot + row * 128 + (((half * 4 + c) ^ ((g & 1) << 2)) << 4));
+                for (int n = 0; n < NBW; ++n) w[n] = *reinterpret_cast<const uint4*>(slot + ((wr * NBW + n) * 8 + g) * 128 + (((half * 4 + c) ^ ((g & 1) << 2)) << 4));
+                // MMAs on the same accumulator are kept apart: each waits for the one before
 #pragma unroll
-                    for (int m = 0; m < 2; ++m) {
-                        mma16816<T>(acc[m][n], f0[m], w.x, w.y);
-                        mma16816<T>(acc[m][n], f1[m], w.z, w.w);
-                    }
-                }
+                for (int n = 0; n < NBW; ++n)
+#pragma unroll
+                    for (int m = 0; m < 2; ++m) mma16816<T>(acc[m][n], f0[m], w[n].x, w[n].y);
+#pragma unroll
+                for (int n = 0; n < NBW; ++n)
+#pragma unroll
+                    for (int m = 0; m < 2; ++m) mma16816<T>(acc[m][n], f1[m], w[n].z, w[n].w);
             }
             load_x(xs[d], ck + DEPTH);
         }
@@ -563,33 +564,43 @@ template <typename T, int NB> __global__ void __launch_bounds__(32 * kLongWarps)
 #pragma unroll
         for (int i = 0; i < 2 * MT; ++i) y[i] = base[i] && in[i] && col < nEnd ? *reinterpret_cast<const uint4*>(base[i] + col) : make_uint4(0u, 0u, 0u, 0u);
     };
+    uint4 w[4][KS];
+    auto load_b = [&](int n0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            // column g of MMA j is column 8 (g / 2) + 2 j + (g & 1) of the group: accumulators 2c, 2c + 1 of the four MMAs are 8 neighbours
+            const int n = n0 + 8 * (g >> 1) + 2 * j + (g & 1);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const int k = s * 32 + c * 8;
+                w[j][s] = has && n < nEnd && k < p.r ? __ldg(reinterpret_cast<const uint4*>(b + static_cast<size_t>(n) * p.r + k)) : make_uint4(0u, 0u, 0u, 0u);
+            }
+        }
+    };
     int n0 = blockIdx.x * kColumns + wn * 32;
     load_base(n0);
+    load_b(n0);
     for (; n0 < nEnd; n0 += WN * 32) {
         float acc[MT][4][4] = {};
         if (has) {
-            uint4 w[4][KS];
+            uint4 wNow[4][KS];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                // column g of MMA j is column 8 (g / 2) + 2 j + (g & 1) of the group: accumulators 2c, 2c + 1 of the four MMAs are 8 neighbours
-                const int n = n0 + 8 * (g >> 1) + 2 * j + (g & 1);
+            for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                    const int k = s * 32 + c * 8;
-                    w[j][s] = n < nEnd && k < p.r ? __ldg(reinterpret_cast<const uint4*>(b + static_cast<size_t>(n) * p.r + k)) : make_uint4(0u, 0u, 0u, 0u);
-                }
-            }
+                for (int s = 0; s < KS; ++s) wNow[j][s] = w[j][s];
+            load_b(n0 + WN * 32);
+            // MMAs on the same accumulator are kept apart: each waits for the one before
 #pragma unroll
             for (int s = 0; s < KS; ++s)
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                for (int q = 0; q < 2; ++q)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
+                    for (int h = 0; h < 2; ++h)
 #pragma unroll
-                        for (int m = 0; m < MT; ++m) {
-                            mma16816<T>(acc[m][j], f[h][m][s][0], w[j][s].x, w[j][s].y);
-                            mma16816<T>(acc[m][j], f[h][m][s][1], w[j][s].z, w[j][s].w);
-                        }
+                        for (int j = 0; j < 4; ++j)
+#pragma unroll
+                            for (int m = 0; m < MT; ++m)
+                                mma16816<T>(acc[m][j], f[h][m][s][q], q ? wNow[j][s].z : wNow[j][s].x, q ? wNow[j][s].w : wNow[j][s].y);
         }
         uint4 now[2 * MT];
 #pragma unroll
