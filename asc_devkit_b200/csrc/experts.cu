@@ -40,43 +40,78 @@ __device__ __forceinline__ void pdl_begin()
 }
 
 // ---- sort ------------------------------------------------------------------------------------------------------------
-// One cluster.  Every warp owns a contiguous run of slots and a private histogram in shared memory; the histograms are
-// summed over the warps and, through distributed shared memory, over the cluster's CTAs, which gives each warp its first position in
-// every expert's run; a second walk over the same slots hands the positions out (equal keys inside a warp's step are
-// ranked with a match).  One launch, no scratch memory, and the order of equal keys is the slots' own.
+// One cluster.  Every warp owns a contiguous run of slots and a private histogram in shared memory, filled 32 slots at a time: a
+// ballot per bit of the key finds a step's equal keys (a match instruction takes several times as long when most differ), which
+// ranks each slot among the warp's slots of its key.  The histograms are summed over
+// the warps and, through distributed shared memory, over the cluster's CTAs: each warp then knows its first position in every key's
+// run.  One launch, no scratch memory, and the order of equal keys is the slots' own.
+// What bounds it is latency (the slots themselves are a few hundred KB): a warp's numbers are all requested at the start and keys and
+// ranks stay in registers (HELD steps of 32 slots).  Longer runs (HELD = 0) count first and walk over the slots a second time.
 template <typename Id> __device__ __forceinline__ int sort_key(const Id* ids, int64_t s, int64_t end, int keys, int outside)
 {
     if (s >= end) return -1;
     const Id v = ids[s];
     return v >= 0 && v < static_cast<Id>(keys) ? static_cast<int>(v) : outside;
 }
+// Rank of each lane's slot among the warp's slots of its key so far; counts the step's slots into `mine`.
+__device__ __forceinline__ uint32_t rank_step(uint32_t* mine, int key, int bits)
+{
+    const int lane = threadIdx.x & 31;
+    uint32_t peers = __ballot_sync(0xFFFFFFFFu, key >= 0);
+    if (key < 0) peers = ~peers;
+    for (int b = 0; b < bits; ++b) {
+        const bool mineSet = (key >> b) & 1;
+        const uint32_t set = __ballot_sync(0xFFFFFFFFu, mineSet);
+        peers &= mineSet ? set : ~set;
+    }
+    const uint32_t before = key >= 0 ? mine[key] : 0u;
+    __syncwarp();
+    if (key >= 0 && lane == __ffs(peers) - 1) mine[key] = before + __popc(peers);
+    __syncwarp();
+    return before + __popc(peers & ((1u << lane) - 1u));
+}
 
-template <typename Id>
+template <typename Id, int HELD>
 __global__ void __launch_bounds__(1024) key_sort_kernel(int64_t* counts, int32_t* rowOfSlot, int32_t* slotOfRow, const Id* ids, int64_t slots, int keys,
                                                         int outside, int ctas)
 {
     extern __shared__ uint32_t smem[];
     const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    uint32_t* hist = smem;                    // [warps][keys]: counts, then first positions
+    uint32_t* hist = smem;                    // [warps][keys]: counts, then the slots of the CTA's earlier warps
     uint32_t* total = hist + warps * keys;    // [keys]: this CTA's slots per key (read by the other CTAs)
-    uint32_t* first = total + keys;           // [keys]: the key's slots in all CTAs, then where its run starts
-    uint32_t* scan = first + keys;            // [33]
+    uint32_t* before = total + keys;          // [keys]: slots of the key in earlier CTAs
+    uint32_t* first = before + keys;          // [keys]: the key's slots in all CTAs, then this CTA's first position in its run
+    uint32_t* scan = first + keys;            // [32]
     for (int i = threadIdx.x; i < warps * keys; i += blockDim.x) hist[i] = 0u;
     pdl_begin();
-    __syncthreads();
 
     const int rank = blockIdx.x;
     const int64_t perWarp = ((slots + static_cast<int64_t>(ctas) * warps - 1) / (static_cast<int64_t>(ctas) * warps) + 31) / 32 * 32;
     const int64_t begin = (static_cast<int64_t>(rank) * warps + warp) * perWarp;
     const int64_t end = begin + perWarp < slots ? begin + perWarp : slots;
     uint32_t* mine = hist + warp * keys;
-    for (int64_t s = begin; s < end; s += 32) {
-        const int key = sort_key<Id>(ids, s + lane, end, keys, outside);
-        if (key >= 0) atomicAdd(&mine[key], 1u);  // a count: the order of the additions does not show
+    const int bits = 32 - __clz(keys - 1);  // of the largest key (__clz(0) is 32)
+    int key[HELD ? HELD : 1];
+    uint32_t place[HELD ? HELD : 1];
+    if constexpr (HELD > 0) {
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) key[i] = sort_key<Id>(ids, begin + 32 * i + lane, end, keys, outside);
+    }
+    __syncthreads();
+    if constexpr (HELD > 0) {
+#pragma unroll
+        for (int i = 0; i < HELD; ++i)
+            if (begin + 32 * i < end) place[i] = rank_step(mine, key[i], bits);
+    } else {
+        for (int64_t s = begin; s < end; s += 32) {
+            const int k = sort_key<Id>(ids, s + lane, end, keys, outside);
+            if (k >= 0) atomicAdd(&mine[k], 1u);  // a count: the order of the additions does not show
+        }
     }
     __syncthreads();
     for (int e = threadIdx.x; e < keys; e += blockDim.x) {
         uint32_t run = 0;
+#pragma unroll 8
         for (int w = 0; w < warps; ++w) {
             const uint32_t c = hist[w * keys + e];
             hist[w * keys + e] = run;
@@ -84,28 +119,27 @@ __global__ void __launch_bounds__(1024) key_sort_kernel(int64_t* counts, int32_t
         }
         total[e] = run;
     }
-    __syncwarp();
     if (ctas > 1) {
+        __syncwarp();
         cluster_arrive();
         cluster_wait();
-    } else {
-        __syncthreads();
     }
     for (int e = threadIdx.x; e < keys; e += blockDim.x) {
-        uint32_t before = 0, all = 0;
+        uint32_t earlier = 0, all = 0;
         if (ctas > 1) {
             const uint32_t at = smem_u32(total + e);
+#pragma unroll 8
             for (int c = 0; c < ctas; ++c) {
                 uint32_t v;
                 asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(mapa_u32(at, c)) : "memory");
-                if (c < rank) before += v;
+                if (c < rank) earlier += v;
                 all += v;
             }
         } else {
             all = total[e];
         }
+        before[e] = earlier;
         first[e] = all;
-        for (int w = 0; w < warps; ++w) hist[w * keys + e] += before;
         if (rank == 0) counts[e] = static_cast<int64_t>(all);
     }
     __syncwarp();
@@ -126,32 +160,37 @@ __global__ void __launch_bounds__(1024) key_sort_kernel(int64_t* counts, int32_t
     }
     if (lane == 31) scan[warp] = incl;
     __syncthreads();
-    uint32_t base = 0, kept = 0;
-    for (int w = 0; w < warps; ++w) {
-        if (w < warp) base += scan[w];
-        kept += scan[w];
+    const uint32_t sums = lane < warps ? scan[lane] : 0u;
+    uint32_t base = lane < warp ? sums : 0u, kept = sums;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        base += __shfl_xor_sync(0xFFFFFFFFu, base, o);
+        kept += __shfl_xor_sync(0xFFFFFFFFu, kept, o);
     }
     uint32_t run = base + incl - sum;
     for (int i = 0; i < per; ++i) {
         const int e = threadIdx.x * per + i;
         if (e < keys) {
             const uint32_t c = first[e];
-            first[e] = run;
+            first[e] = run + before[e];
             run += c;
         }
     }
     __syncthreads();
-    for (int64_t s = begin; s < end; s += 32) {
-        const int key = sort_key<Id>(ids, s + lane, end, keys, outside);
-        const uint32_t peers = __match_any_sync(0xFFFFFFFFu, key);
-        uint32_t pos = 0;
-        if (key >= 0) pos = first[key] + mine[key] + __popc(peers & ((1u << lane) - 1u));
-        __syncwarp();
-        if (key >= 0 && lane == __ffs(peers) - 1) mine[key] += __popc(peers);
-        __syncwarp();
-        if (s + lane < end) {
-            if (rowOfSlot) rowOfSlot[s + lane] = key >= 0 ? static_cast<int32_t>(pos) : -1;
-            if (slotOfRow && key >= 0) slotOfRow[pos] = static_cast<int32_t>(s + lane);
+    auto put = [&](int64_t s, int k, uint32_t at) {
+        if (s >= end) return;
+        const uint32_t pos = k >= 0 ? first[k] + at : 0u;
+        if (rowOfSlot) rowOfSlot[s] = k >= 0 ? static_cast<int32_t>(pos) : -1;
+        if (slotOfRow && k >= 0) slotOfRow[pos] = static_cast<int32_t>(s);
+    };
+    if constexpr (HELD > 0) {
+#pragma unroll
+        for (int i = 0; i < HELD; ++i)
+            if (begin + 32 * i < end) put(begin + 32 * i + lane, key[i], (key[i] >= 0 ? mine[key[i]] : 0u) + place[i]);
+    } else {
+        for (int64_t s = begin; s < end; s += 32) {
+            const int k = sort_key<Id>(ids, s + lane, end, keys, outside);
+            put(s + lane, k, rank_step(mine, k, bits));  // `mine` holds the earlier warps' slots, then this warp's too
         }
     }
     if (slotOfRow)
@@ -160,24 +199,65 @@ __global__ void __launch_bounds__(1024) key_sort_kernel(int64_t* counts, int32_t
     if (ctas > 1) cluster_wait();
 }
 
+constexpr unsigned kSortThreads = 1024;
+
+// Per-device set-up; *most receives the largest cluster the device can place (16 CTAs are beyond the portable size of 8).
+template <typename Id, int HELD> ascq_status sort_setup(int* most)
+{
+    static PerDeviceOnce once, wide;
+    const int dev = current_device();
+    if (!once.done(dev)) {
+        const int smem = (static_cast<int>(kSortThreads / 32 + 3) * kMaxSortKeys + 32) * 4;
+        ASCQ_CUDA_CHECK(cudaFuncSetAttribute(key_sort_kernel<Id, HELD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        ASCQ_CUDA_CHECK(cudaFuncSetAttribute(key_sort_kernel<Id, HELD>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(16, 1, 1);
+        cfg.blockDim = dim3(kSortThreads, 1, 1);
+        cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 16;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int clusters = 0;
+        if (cudaOccupancyMaxActiveClusters(&clusters, key_sort_kernel<Id, HELD>, &cfg) == cudaSuccess && clusters > 0) wide.mark(dev);
+        else cudaGetLastError();  // not placeable: the portable size it is
+        once.mark(dev);
+    }
+    *most = wide.done(dev) ? 16 : 8;
+    return ASCQ_OK;
+}
+
+template <typename Id, int HELD> ascq_status launch_key_sort_held(int64_t* counts, int32_t* rowOfSlot, int32_t* slotOfRow, const void* ids, int64_t slots,
+                                                                  int keys, int outside, unsigned threads, int ctas, cudaStream_t st)
+{
+    const size_t smem = (static_cast<size_t>(threads / 32 + 3) * keys + 32) * 4;
+    ASCQ_CUDA_CHECK(launch_rows(key_sort_kernel<Id, HELD>, dim3(ctas), threads, smem, ctas, st, counts, rowOfSlot, slotOfRow, static_cast<const Id*>(ids), slots,
+                                keys, outside, ctas));
+    return ASCQ_OK;
+}
 template <typename Id> ascq_status launch_key_sort_typed(int64_t* counts, int32_t* rowOfSlot, int32_t* slotOfRow, const void* ids, int64_t slots, int keys,
                                                          int outside, cudaStream_t st)
 {
-    // enough warps that each walks a few steps of 32 slots; a second CTA only once 32 warps walk more than 8 steps each
-    unsigned threads = 128;
-    while (threads < 1024 && slots > static_cast<int64_t>(threads) * 2) threads *= 2;
+    // A CTA takes 1024 slots (one step of its warps) while the cluster can grow.  Measured, 64 keys, us: 1024 slots 4.1 with one CTA (4.7
+    // with two), 4096 slots 5.1 / 6.2 / 7.5 with four / two / one, 16384 slots 5.5 / 6.7 / 8.6 with 16 / 8 / 4, 65536 slots 9.9 / 14.1 with 16 / 8.
+    unsigned threads = 256;
+    while (threads < kSortThreads && slots > threads) threads *= 2;
+    int most[4] = {};
+    ascq_status rc = sort_setup<Id, 1>(&most[0]);
+    if (rc == ASCQ_OK) rc = sort_setup<Id, 4>(&most[1]);
+    if (rc == ASCQ_OK) rc = sort_setup<Id, 8>(&most[2]);
+    if (rc == ASCQ_OK) rc = sort_setup<Id, 0>(&most[3]);
+    if (rc != ASCQ_OK) return rc;
+    const int cap = std::min(std::min(most[0], most[1]), std::min(most[2], most[3]));
     int ctas = 1;
-    while (ctas < 8 && slots > static_cast<int64_t>(ctas) * 8192) ctas *= 2;
-    const size_t smem = (static_cast<size_t>(threads / 32 + 2) * keys + 64) * 4;
-    static PerDeviceOnce once;
-    const int dev = current_device();
-    if (!once.done(dev)) {
-        ASCQ_CUDA_CHECK(cudaFuncSetAttribute(key_sort_kernel<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, (34 * kMaxSortKeys + 64) * 4));
-        once.mark(dev);
-    }
-    ASCQ_CUDA_CHECK(launch_rows(key_sort_kernel<Id>, dim3(ctas), threads, smem, ctas, st, counts, rowOfSlot, slotOfRow, static_cast<const Id*>(ids), slots, keys,
-                                outside, ctas));
-    return ASCQ_OK;
+    while (ctas < cap && slots > static_cast<int64_t>(ctas) * kSortThreads) ctas *= 2;
+    const int64_t steps = (slots + static_cast<int64_t>(ctas) * threads - 1) / (static_cast<int64_t>(ctas) * threads);  // of 32 slots, of a warp
+    if (steps <= 1) return launch_key_sort_held<Id, 1>(counts, rowOfSlot, slotOfRow, ids, slots, keys, outside, threads, ctas, st);
+    if (steps <= 4) return launch_key_sort_held<Id, 4>(counts, rowOfSlot, slotOfRow, ids, slots, keys, outside, threads, ctas, st);
+    if (steps <= 8) return launch_key_sort_held<Id, 8>(counts, rowOfSlot, slotOfRow, ids, slots, keys, outside, threads, ctas, st);
+    return launch_key_sort_held<Id, 0>(counts, rowOfSlot, slotOfRow, ids, slots, keys, outside, threads, ctas, st);
 }
 
 // ---- dispatch ---------------------------------------------------------------------------------------------------------
@@ -239,12 +319,14 @@ struct CombineArgs {
 };
 
 // VEC consecutive elements of T as floats: VEC * sizeof(T) bytes in one access of up to 16 bytes
+template <typename T, int VEC> __device__ __forceinline__ Pack<T, VEC> load_v(const T* p)
+{
+    if constexpr (sizeof(T) * VEC >= 4) return load_pack<T, VEC, true>(p);
+    else return Pack<T, VEC>{{*p}};
+}
 template <typename T, int VEC> __device__ __forceinline__ void load_f(const T* p, float (&f)[VEC])
 {
-    const Pack<T, VEC> v = [&] {
-        if constexpr (sizeof(T) * VEC >= 4) return load_pack<T, VEC, true>(p);
-        else return Pack<T, VEC>{{*p}};
-    }();
+    const Pack<T, VEC> v = load_v<T, VEC>(p);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) f[i] = to_f32<T>(v.v[i]);
 }
@@ -318,12 +400,16 @@ template <typename T, int VEC> __global__ void __launch_bounds__(256) combine_ke
 }
 
 // ---- gradient of combine --------------------------------------------------------------------------------------------------
-// One CTA per token: gradOut's row is read once for up to kGradRows of the token's rows at a time.
-constexpr int kGradRows = 8;
+// One CTA per token.  A thread requests its vectors of kGradRows of the token's rows together; gradOut's row is read again (from
+// L1 or L2) for the next kGradRows.  What bounds it is how many requests an SM has in flight, so the rows per step trade against
+// occupancy: at 8192 tokens, k = 8, h = 4096 in bf16 (177 us at the copy rate) 187 us with 4 rows and 64 registers, 213 with 2 rows
+// and 40, 196 with 4 rows and 80, 249 with 8 rows and 120; CTAs of 128 threads rather than 256 (193 us) or 64 (198 us).
+constexpr int kGradRows = 4, kGradThreads = 128;
 
-template <typename T, int VEC> __global__ void __launch_bounds__(256) combine_grad_kernel(const CombineArgs a)
+
+template <typename T, int VEC> __global__ void __launch_bounds__(kGradThreads, 8) combine_grad_kernel(const CombineArgs a)
 {
-    __shared__ float part[8][kGradRows];
+    __shared__ float part[kGradThreads / 32][kGradRows];
     pdl_begin();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const int64_t t = blockIdx.x;
@@ -338,23 +424,32 @@ template <typename T, int VEC> __global__ void __launch_bounds__(256) combine_gr
             w[j] = a.weights && j0 + j < a.k ? a.weights[t * a.k + j0 + j] : 1.0f;
         }
         for (int64_t c = static_cast<int64_t>(threadIdx.x) * VEC; c < a.h; c += static_cast<int64_t>(blockDim.x) * VEC) {
+            const Pack<T, VEC> dv = load_v<T, VEC>(dOut + c);
+            Pack<T, VEC> v[kGradRows];
+            if (a.gradWeights) {
+#pragma unroll
+                for (int j = 0; j < kGradRows; ++j)
+                    if (r[j] >= 0) v[j] = load_v<T, VEC>(static_cast<const T*>(a.in) + static_cast<int64_t>(r[j]) * a.h + c);
+            }
             float d[VEC];
-            load_f<T, VEC>(dOut + c, d);
 #pragma unroll
-            for (int j = 0; j < kGradRows; ++j) {
-                if (r[j] < 0) continue;
-                const int64_t at = static_cast<int64_t>(r[j]) * a.h + c;
-                if (a.gradWeights) {
-                    float f[VEC];
-                    load_f<T, VEC>(static_cast<const T*>(a.in) + at, f);
+            for (int i = 0; i < VEC; ++i) d[i] = to_f32<T>(dv.v[i]);
+            if (a.gradRows) {
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i) dot[j] = fmaf(f[i], d[i], dot[j]);
-                }
-                if (a.gradRows) {
+                for (int j = 0; j < kGradRows; ++j) {
+                    if (r[j] < 0) continue;
                     float g[VEC];
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) g[i] = __fmul_rn(w[j], d[i]);
-                    store_f<T, VEC>(static_cast<T*>(a.gradRows) + at, g);
+                    store_f<T, VEC>(static_cast<T*>(a.gradRows) + static_cast<int64_t>(r[j]) * a.h + c, g);
+                }
+            }
+            if (a.gradWeights) {
+#pragma unroll
+                for (int j = 0; j < kGradRows; ++j) {
+                    if (r[j] < 0) continue;
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) dot[j] = fmaf(to_f32<T>(v[j].v[i]), d[i], dot[j]);
                 }
             }
         }
@@ -521,7 +616,8 @@ extern "C" ascq_status ascq_expert_combine_grad(void* gradRows, float* gradWeigh
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     auto run = [&](auto kernel, int vec) -> ascq_status {
         const int64_t nvec = (h + vec - 1) / vec;
-        const unsigned block = nvec >= 256 ? 256u : nvec <= 32 ? 32u : static_cast<unsigned>((nvec + 31) / 32 * 32);
+        const int64_t steps = std::max<int64_t>((nvec + kGradThreads - 1) / kGradThreads, 1);  // of a thread along the row; the CTA is no wider than they need
+        const unsigned block = std::max(static_cast<unsigned>((nvec + steps - 1) / steps + 31) / 32 * 32, 32u);
         ASCQ_CUDA_CHECK(launch_rows(kernel, dim3(static_cast<unsigned>(tokens)), block, 0, 1, st, a));
         return ASCQ_OK;
     };

@@ -7,7 +7,8 @@
 //   MX:    e = floor(log2 max|y|) - emax per block of 32,  scale byte = e + 127,  q = cast(y * 2^-e)
 //
 // What bounds it: HBM.  With bf16 tensors and residualOut an element costs 2 + 2 bytes read, 2 + 1 written.  A CTA owns whole rows and
-// keeps a row in registers between the reduction and the quantisation, so each byte moves once.  For int8 the row's
+// keeps a row in registers between the reduction and the quantisation, so each byte moves once; the next row is requested before the
+// reduction.  bf16 [16384, 7168] to e4m3: 135 us = 6.1 TB/s, 0.95 of the measured copy rate (164 us without the early request).  For int8 the row's
 // maximum needs no second reduction: max|y| = rstd * max|h * gamma|, so sum(h^2) and max|h * gamma| go through the same
 // shuffles and the same barrier, and RINT(y * 127 / max|y|) = RINT((h * gamma) * (127 / max|h * gamma|)) does not need rstd.
 #include "elementwise.cuh"
@@ -183,37 +184,39 @@ template <typename T, typename G, int OUT, int NV> __global__ void __launch_boun
         }
     }
     int slot = 0;
+    Vec8<T> xs[NV], rs[NV];
+    auto load_row = [&](uint32_t row) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const uint32_t v = i * blockDim.x + threadIdx.x;
+            if (v < nvec) {
+                xs[i] = load8<T>(src + row * a.ldSrc + v * 8);
+                if (res) rs[i] = load8<T>(res + row * a.ldResidual + v * 8);
+            }
+        }
+    };
+    load_row(blockIdx.x);
     for (uint32_t row = blockIdx.x; row < a.m; row += gridDim.x, slot ^= 1) {
         float h[NV][8];
         float sum = 0.f, mx = 0.f;
-        {
-            Vec8<T> xs[NV], rs[NV];
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const uint32_t v = i * blockDim.x + threadIdx.x;
-                if (v < nvec) {
-                    xs[i] = load8<T>(src + row * a.ldSrc + v * 8);
-                    if (res) rs[i] = load8<T>(res + row * a.ldResidual + v * 8);
+        for (int i = 0; i < NV; ++i) {
+            const uint32_t v = i * blockDim.x + threadIdx.x;
+            if (v < nvec) {
+                widen8<T>(xs[i], h[i]);
+                if (res) {
+                    float r[8];
+                    widen8<T>(rs[i], r);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) h[i][j] = __fadd_rn(h[i][j], r[j]);
                 }
-            }
+                if (a.residualOut) store8<T>(static_cast<T*>(a.residualOut) + row * a.ldResidualOut + v * 8, h[i]);
+            } else {
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const uint32_t v = i * blockDim.x + threadIdx.x;
-                if (v < nvec) {
-                    widen8<T>(xs[i], h[i]);
-                    if (res) {
-                        float r[8];
-                        widen8<T>(rs[i], r);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) h[i][j] = __fadd_rn(h[i][j], r[j]);
-                    }
-                    if (a.residualOut) store8<T>(static_cast<T*>(a.residualOut) + row * a.ldResidualOut + v * 8, h[i]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) h[i][j] = 0.f;
-                }
+                for (int j = 0; j < 8; ++j) h[i][j] = 0.f;
             }
         }
+        if (row + gridDim.x < a.m) load_row(row + gridDim.x);  // on its way while this row is reduced and quantised
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const uint32_t v = i * blockDim.x + threadIdx.x;
@@ -378,7 +381,10 @@ template <typename T, typename G, int OUT> cudaError_t launch_norm_rows(const No
     uint32_t nv = 1;
     while (nv < kNormMaxVectors && (nvec + nv - 1) / nv > kNormThreads) nv *= 2;
     const unsigned block = ((nvec + nv - 1) / nv + 31) / 32 * 32;
-    const unsigned perSm = nv >= 4 ? 1u : std::max(1u, 1024u / block);
+    // About 1280 threads per SM, each CTA walking over its rows with the next one on its way.  Measured: bf16 [16384, 7168] to e4m3 (448
+    // threads) 182 / 135 / 147 us with 1 / 2 / 3 CTAs per SM; half [1031, 5120] to int8 (320 threads) 8.2 / 8.1 / 5.6 / 5.5 / 5.6 us with
+    // 1 to 5.  Rows above 8192 elements need 128 registers a thread: one CTA.
+    const unsigned perSm = nv >= 4 ? 1u : std::max(1u, 1280u / block);
     const unsigned grid = std::min<uint64_t>(a.m, static_cast<uint64_t>(sm_count()) * perSm);
     if (nv == 1) return launch_norm(norm_rows_kernel<T, G, OUT, 1>, grid, block, st, a);
     if (nv == 2) return launch_norm(norm_rows_kernel<T, G, OUT, 2>, grid, block, st, a);

@@ -58,7 +58,7 @@ def route(t, k, e, seed=0, outside=0.0, dtype=torch.int64):
 # ---- sort ---------------------------------------------------------------------------------------------------------
 @gpu
 @pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
-@pytest.mark.parametrize("t,k,e", [(1, 1, 1), (1, 8, 256), (3, 2, 5), (33, 3, 7), (100, 8, 60), (1021, 4, 64), (257, 6, 1024), (2500, 8, 128), (9001, 8, 256)])
+@pytest.mark.parametrize("t,k,e", [(1, 1, 1), (1, 8, 256), (3, 2, 5), (33, 3, 7), (100, 8, 60), (1021, 4, 64), (257, 6, 1024), (2500, 8, 128), (9001, 8, 256), (129, 8, 9), (4097, 4, 30), (20000, 8, 64)])
 def test_sort(t, k, e, dtype):
     check_sort(route(t, k, e, dtype=dtype), e)
 
