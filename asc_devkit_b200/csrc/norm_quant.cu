@@ -115,13 +115,19 @@ template <int OUT> __device__ __forceinline__ uint32_t mx_pair(float first, floa
     }
     return r;
 }
-// Shared exponent of a block from its largest magnitude (finite): floor(log2(amax)) - emax inside the E8M0 range, 0 for an
-// all-zero block.  A subnormal amax counts as 2^-126; with emax >= 2 it ends at the range's lower end either way.
-__device__ __forceinline__ int mx_exponent(float amax, int emax)
+// Shared exponent of a block whose largest |h * gamma| is `amax`: floor(log2(amax * rstd)) - emax inside the E8M0 range, 0 for an all-zero
+// block.  The product is taken with the remainder of rstd and of its own rounding: where it rounds up to a power of two the exact
+// one may lie below, and an exponent off by one doubles the block's grid.  A subnormal product counts as 2^-126; with emax >= 2
+// it ends at the range's lower end either way.
+__device__ __forceinline__ int mx_exponent(float amax, float rstd, float rstdLo, int emax)
 {
     if (!(amax > 0.f)) return 0;
-    const int ex = static_cast<int>(__float_as_uint(amax) >> 23);
-    return min(max((ex == 0 ? -126 : ex - 127) - emax, -127), 127);
+    const float y = __fmul_rn(amax, rstd), rest = fmaf(amax, rstdLo, fmaf(amax, rstd, -y));
+    const uint32_t bits = __float_as_uint(y);
+    int ex = static_cast<int>(bits >> 23);
+    ex = ex == 0 ? -126 : ex - 127;
+    if ((bits & 0x7FFFFFu) == 0 && rest < 0.f) --ex;
+    return min(max(ex - emax, -127), 127);
 }
 // 2^-e for e in [-127, 127]; 2^-127 is a subnormal
 __device__ __forceinline__ float exp2_neg(int e) { return e == 127 ? __uint_as_float(0x00400000u) : __uint_as_float(static_cast<uint32_t>(127 - e) << 23); }
@@ -139,33 +145,59 @@ __device__ __forceinline__ I8Factor i8_factor(float amax)
     return f;
 }
 
-// Sum and maximum over the CTA, the same result in every thread.  `slot` alternates between the rows of a CTA: a warp
-// that is already at the next row then writes the other half of the array, so one barrier per row is enough.
-__device__ __forceinline__ void cta_sum_max(float& sum, float& mx, float2 (*part)[16], int slot)
+// A sum as two floats: hi is its nearest float, lo what is missing.
+struct Sum2 {
+    float hi, lo;
+};
+__device__ __forceinline__ Sum2 add_exact(Sum2 a, Sum2 b)
+{
+    const float s = __fadd_rn(a.hi, b.hi), t = __fsub_rn(s, a.hi);
+    const float e = __fadd_rn(__fsub_rn(a.hi, __fsub_rn(s, t)), __fsub_rn(b.hi, t));  // what s lost of a.hi + b.hi
+    return Sum2{s, __fadd_rn(e, __fadd_rn(a.lo, b.lo))};
+}
+
+// 1 / sqrt(sum / n + epsilon) as two floats: a Newton step on the float result, its residual 1 - v r^2 formed from exact products.
+__device__ __forceinline__ Sum2 rstd_of(Sum2 sum, float n, float epsilon)
+{
+    const float q = __fdiv_rn(sum.hi, n);
+    const float ql = __fdiv_rn(__fadd_rn(fmaf(-q, n, sum.hi), sum.lo), n);
+    const Sum2 v = add_exact(Sum2{q, ql}, Sum2{epsilon, 0.f});
+    const float r = __frsqrt_rn(v.hi), t = __fmul_rn(r, r), tl = fmaf(r, r, -t);
+    const float e = fmaf(-v.lo, t, fmaf(-v.hi, tl, fmaf(-v.hi, t, 1.0f)));
+    return Sum2{r, 0.5f * r * e};
+}
+
+// Sum and maximum over the CTA, the same result in every thread; the warps' sums are added exactly, since every code of the row depends on the
+// result.  `slot` alternates between the rows of a CTA: a warp that is already at the next row then writes the other half of the array, so one
+// barrier per row is enough.
+struct SumMax {
+    Sum2 sum;
+    float mx;
+};
+__device__ __forceinline__ SumMax cta_sum_max(float sum, float mx, float2 (*part)[16], int slot)
 {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
         mx = max_nan(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
     }
+    SumMax v{{sum, 0.f}, mx};
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-    if (warps == 1) return;
+    if (warps == 1) return v;
     if (lane == 0) part[slot][warp] = make_float2(sum, mx);
     __syncthreads();
-    const float2 p = lane < warps ? part[slot][lane] : make_float2(0.f, 0.f);
-    sum = p.x;
-    mx = p.y;
+    const float2 p = (lane & 15) < warps ? part[slot][lane & 15] : make_float2(0.f, 0.f);
+    v = SumMax{{p.x, 0.f}, p.y};
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) {
-        sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-        mx = max_nan(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
+        v.sum = add_exact(v.sum, Sum2{__shfl_xor_sync(0xFFFFFFFFu, v.sum.hi, o), __shfl_xor_sync(0xFFFFFFFFu, v.sum.lo, o)});
+        v.mx = max_nan(v.mx, __shfl_xor_sync(0xFFFFFFFFu, v.mx, o));
     }
-    sum = __shfl_sync(0xFFFFFFFFu, sum, 0);
-    mx = __shfl_sync(0xFFFFFFFFu, mx, 0);
+    return v;
 }
 
 // The vector kernel: a thread owns NV vectors of 8 elements of a row, spaced by the CTA's width.
-template <typename T, typename G, int OUT, int NV> __global__ void __launch_bounds__(512) norm_rows_kernel(const NormArgs a)
+template <typename T, typename G, int OUT, int NV> __global__ void __launch_bounds__(512, NV <= 2 && sizeof(T) == 2 ? 2 : 1) norm_rows_kernel(const NormArgs a)
 {
     __shared__ float2 part[2][16];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -231,8 +263,10 @@ template <typename T, typename G, int OUT, int NV> __global__ void __launch_boun
                 }
             }
         }
-        cta_sum_max(sum, mx, part, slot);
-        const float rstd = finite_f32(sum) ? __frsqrt_rn(__fadd_rn(__fdiv_rn(sum, static_cast<float>(a.n)), a.epsilon)) : __int_as_float(0x7FFFFFFF);
+        const SumMax both = cta_sum_max(sum, mx, part, slot);
+        mx = both.mx;
+        const Sum2 exact = rstd_of(both.sum, static_cast<float>(a.n), a.epsilon);
+        const float rstd = finite_f32(both.sum.hi) ? exact.hi : __int_as_float(0x7FFFFFFF);
         if (a.normOut) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
@@ -272,20 +306,18 @@ template <typename T, typename G, int OUT, int NV> __global__ void __launch_boun
                 const uint32_t v = i * blockDim.x + threadIdx.x;
                 float amax = 0.f;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    h[i][j] = __fmul_rn(h[i][j], rstd);
-                    amax = max_nan(amax, fabsf(h[i][j]));
-                }
+                for (int j = 0; j < 8; ++j) amax = max_nan(amax, fabsf(h[i][j]));
                 // four neighbouring lanes hold a block; n is a multiple of 32, so they are inside the row together or not at all
                 amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
                 amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 2));
                 if (v < nvec) {
-                    const bool ok = finite_f32(amax);
-                    const int e = mx_exponent(amax, out_emax(OUT));
+                    const bool ok = finite_f32(__fmul_rn(amax, rstd));
+                    const int e = mx_exponent(amax, rstd, exact.lo, out_emax(OUT));
                     const float up = exp2_neg(e);
                     uint32_t c[4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) c[j] = ok ? mx_pair<OUT>(__fmul_rn(h[i][2 * j], up), __fmul_rn(h[i][2 * j + 1], up)) : 0u;
+                    for (int j = 0; j < 4; ++j)
+                        c[j] = ok ? mx_pair<OUT>(__fmul_rn(__fmul_rn(h[i][2 * j], rstd), up), __fmul_rn(__fmul_rn(h[i][2 * j + 1], rstd), up)) : 0u;
                     const size_t at = (static_cast<size_t>(row) * nvec + v);
                     if constexpr (OUT == kOutE2M1) static_cast<uint32_t*>(a.dst)[at] = c[0] | (c[1] << 8) | (c[2] << 16) | (c[3] << 24);
                     else __stcs(static_cast<uint2*>(a.dst) + at, make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16)));
@@ -315,8 +347,10 @@ template <typename T, typename G> __global__ void __launch_bounds__(256) norm_an
         sum = fmaf(h, h, sum);
         mx = max_nan(mx, fabsf(__fmul_rn(h, to_f32<G>(gamma[c]))));
     }
-    cta_sum_max(sum, mx, part, 0);
-    const float rstd = finite_f32(sum) ? __frsqrt_rn(__fadd_rn(__fdiv_rn(sum, static_cast<float>(a.n)), a.epsilon)) : __int_as_float(0x7FFFFFFF);
+    const SumMax both = cta_sum_max(sum, mx, part, 0);
+    mx = both.mx;
+    const Sum2 exact = rstd_of(both.sum, static_cast<float>(a.n), a.epsilon);
+    const float rstd = finite_f32(both.sum.hi) ? exact.hi : __int_as_float(0x7FFFFFFF);
     const float top = __fmul_rn(mx, rstd);
     const bool rowOk = finite_f32(mx) && finite_f32(top);
     const I8Factor f = i8_factor(mx);
@@ -339,11 +373,11 @@ template <typename T, typename G> __global__ void __launch_bounds__(256) norm_an
                     static_cast<int8_t>(rowOk ? f32_to_i8_sat(__fmul_rn(f.pre != 1.0f ? p * f.pre : p, f.mul), kRoundRint) : 0);
         } else {  // n is a multiple of 32: a warp holds one block, whole or not at all
             const float y = __fmul_rn(p, rstd);
-            float amax = fabsf(y);
+            float amax = fabsf(p);
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
-            const bool ok = finite_f32(amax);
-            const int e = mx_exponent(amax, out_emax(a.out));
+            const bool ok = finite_f32(__fmul_rn(amax, rstd));
+            const int e = mx_exponent(amax, rstd, exact.lo, out_emax(a.out));
             const float v = __fmul_rn(y, exp2_neg(e));
             const float next = __shfl_down_sync(0xFFFFFFFFu, v, 1);
             if (c < a.n) {

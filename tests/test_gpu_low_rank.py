@@ -175,8 +175,9 @@ def test_beside_the_w8a8_projection():
     g = torch.ones(k, dtype=torch.bfloat16, device=DEV)
     q, qs, y = torch.empty(m, k, dtype=torch.int8, device=DEV), torch.empty(m, device=DEV), torch.empty_like(x)
     ops.ResidualRmsNormQuant(q, qs, x, g, 1e-6, normOut=y)
-    w = torch.randint(-127, 128, (n, k), dtype=torch.int8, device=DEV)
-    ws = 0.001 * torch.rand(n, device=DEV)
+    rng = torch.Generator().manual_seed(5)
+    w = torch.randint(-127, 128, (n, k), generator=rng, dtype=torch.int8).to(DEV)
+    ws = (0.001 * torch.rand(n, generator=rng)).to(DEV)
     c = torch.empty(m, n, dtype=torch.bfloat16, device=DEV)
     ops.MatmulW8A8(c, q, w, qs, ws)
     base = c.clone()

@@ -239,11 +239,13 @@ def test_feeds_the_w8a8_matmul():
     m, n, out = 48, 512, 256
     x, r, g = inputs(m, n, torch.bfloat16)
     q, scale, _, _ = run(x, r, g, L.DT_I8)
-    w = torch.randint(-127, 128, (out, n), dtype=torch.int8, device=DEV)
-    ws = torch.rand(out, device=DEV) * 0.01
+    rng = torch.Generator().manual_seed(5)
+    w = torch.randint(-127, 128, (out, n), generator=rng, dtype=torch.int8).to(DEV)
+    ws = (0.01 * torch.rand(out, generator=rng)).to(DEV)
     c = torch.empty(m, out, dtype=torch.bfloat16, device=DEV)
     ops.MatmulW8A8(c, q, w, scale, ws)
-    want = (q.double() * scale.double()[:, None]) @ (w.double() * ws.double()[:, None]).T
+    # whole numbers first: they add up exactly, also to 0
+    want = (q.double() @ w.double().T) * scale.double()[:, None] * ws.double()
     assert torch.all((c.double() - want).abs() <= want.abs() * (2.0 ** -8 + 8 * U))
 
 
