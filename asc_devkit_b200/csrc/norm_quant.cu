@@ -42,6 +42,24 @@ __device__ __forceinline__ float max_nan(float a, float b)
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
+// largest magnitude of three, NaN if one of them is
+__device__ __forceinline__ float max_abs3(float a, float b, float c)
+{
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float max_abs8(const float (&f)[8])
+{
+    return max_abs3(max_abs3(max_abs3(f[0], f[1], f[2]), f[3], f[4]), max_abs3(f[5], f[6], f[7]), 0.f);
+}
+// d += a^2 for two lanes, each rounded on its own
+__device__ __forceinline__ void fma2_square(float& d0, float& d1, float a0, float a1)
+{
+    asm("{\n\t.reg .b64 a, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 d, {%0, %1};\n\tfma.rn.f32x2 d, a, a, d;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "+f"(d0), "+f"(d1)
+        : "f"(a0), "f"(a1));
+}
 __device__ __forceinline__ bool finite_f32(float v) { return fabsf(v) <= 3.4028234663852886e38f; }
 
 // 8 consecutive elements: 16 bytes of a 16-bit type, 32 of fp32 (two 16-byte loads)
@@ -82,18 +100,27 @@ template <typename T> __device__ __forceinline__ T narrow(float f)
     else if constexpr (std::is_same<T, __half>::value) return f32_to_f16_sat(f);
     else return f32_to_bf16_sat(f);
 }
-// the framework's narrowing rule: round to nearest even, a finite value that overflows saturates
-template <typename T> __device__ __forceinline__ void store8(T* p, const float (&f)[8])
+// the framework's narrowing rule: round to nearest even, a finite value that overflows saturates.  `top`: the largest of the magnitudes
+// (NaN if there is one); only a vector that holds something beyond the type's largest value is looked at element by element.
+template <typename T> __device__ __forceinline__ void store8(T* p, const float (&f)[8], float top)
 {
     if constexpr (sizeof(T) == 4) {
         __stcs(reinterpret_cast<float4*>(p), make_float4(f[0], f[1], f[2], f[3]));
         __stcs(reinterpret_cast<float4*>(p) + 1, make_float4(f[4], f[5], f[6], f[7]));
     } else {
+        constexpr float kMost = std::is_same<T, __half>::value ? 65504.0f : 3.3895313892515355e38f;
         uint32_t r[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if constexpr (std::is_same<T, __half>::value) r[i] = pack_f16x2_sat(f[2 * i], f[2 * i + 1]);
-            else r[i] = pack_bf16x2_sat(f[2 * i], f[2 * i + 1]);
+            if constexpr (std::is_same<T, __half>::value) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r[i]) : "f"(f[2 * i + 1]), "f"(f[2 * i]));
+            else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r[i]) : "f"(f[2 * i + 1]), "f"(f[2 * i]));
+        }
+        if (__builtin_expect(!(top <= kMost), 0)) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (std::is_same<T, __half>::value) r[i] = pack_f16x2_sat(f[2 * i], f[2 * i + 1]);
+                else r[i] = pack_bf16x2_sat(f[2 * i], f[2 * i + 1]);
+            }
         }
         __stcs(reinterpret_cast<uint4*>(p), make_uint4(r[0], r[1], r[2], r[3]));
     }
@@ -167,39 +194,44 @@ __device__ __forceinline__ Sum2 rstd_of(Sum2 sum, float n, float epsilon)
     return Sum2{r, 0.5f * r * e};
 }
 
-// Sum and maximum over the CTA, the same result in every thread; the warps' sums are added exactly, since every code of the row depends on the
-// result.  `slot` alternates between the rows of a CTA: a warp that is already at the next row then writes the other half of the array, so one
-// barrier per row is enough.
-struct SumMax {
-    Sum2 sum;
-    float mx;
+// What a row's elements need to know: rstd and its remainder, the largest |h * gamma| (int8), NaN in rstd for a sum that is not finite.
+struct RowStats {
+    float rstd, rstdLo, mx, pad;
 };
-__device__ __forceinline__ SumMax cta_sum_max(float sum, float mx, float2 (*part)[16], int slot)
+// Sum and maximum over the CTA.  The warps' sums are added exactly, since every code of the row depends on the result, and the division, the square
+// root and its correction take some two hundred instructions: one warp does that and the others read the outcome (in every warp it
+// cost as many issue slots as the elements did: 163 us instead of 136 at [16384, 7168]).
+__device__ __forceinline__ RowStats row_stats(float sum, float mx, float2* part, RowStats* stats, float n, float epsilon)
 {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
         mx = max_nan(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
     }
-    SumMax v{{sum, 0.f}, mx};
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-    if (warps == 1) return v;
-    if (lane == 0) part[slot][warp] = make_float2(sum, mx);
+    if (lane == 0) part[warp] = make_float2(sum, mx);
     __syncthreads();
-    const float2 p = (lane & 15) < warps ? part[slot][lane & 15] : make_float2(0.f, 0.f);
-    v = SumMax{{p.x, 0.f}, p.y};
+    if (warp == 0) {
+        const float2 p = (lane & 15) < warps ? part[lane & 15] : make_float2(0.f, 0.f);
+        Sum2 all{p.x, 0.f};
+        mx = p.y;
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) {
-        v.sum = add_exact(v.sum, Sum2{__shfl_xor_sync(0xFFFFFFFFu, v.sum.hi, o), __shfl_xor_sync(0xFFFFFFFFu, v.sum.lo, o)});
-        v.mx = max_nan(v.mx, __shfl_xor_sync(0xFFFFFFFFu, v.mx, o));
+        for (int o = 8; o > 0; o >>= 1) {
+            all = add_exact(all, Sum2{__shfl_xor_sync(0xFFFFFFFFu, all.hi, o), __shfl_xor_sync(0xFFFFFFFFu, all.lo, o)});
+            mx = max_nan(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
+        }
+        const Sum2 r = rstd_of(all, n, epsilon);
+        if (lane == 0) *stats = RowStats{finite_f32(all.hi) ? r.hi : __int_as_float(0x7FFFFFFF), r.lo, mx, 0.f};
     }
-    return v;
+    __syncthreads();  // `part` may be written again; `stats` is, only behind the next row's first barrier
+    return *stats;
 }
 
 // The vector kernel: a thread owns NV vectors of 8 elements of a row, spaced by the CTA's width.
 template <typename T, typename G, int OUT, int NV> __global__ void __launch_bounds__(512, NV <= 2 && sizeof(T) == 2 ? 2 : 1) norm_rows_kernel(const NormArgs a)
 {
-    __shared__ float2 part[2][16];
+    __shared__ float2 part[16];
+    __shared__ __align__(16) RowStats stats;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint32_t nvec = a.n / 8;
@@ -215,7 +247,6 @@ template <typename T, typename G, int OUT, int NV> __global__ void __launch_boun
             for (int j = 0; j < static_cast<int>(sizeof(G)) / 2; ++j) g[i].w[j] = __ldg(p + j);
         }
     }
-    int slot = 0;
     Vec8<T> xs[NV], rs[NV];
     auto load_row = [&](uint32_t row) {
 #pragma unroll
@@ -228,9 +259,9 @@ template <typename T, typename G, int OUT, int NV> __global__ void __launch_boun
         }
     };
     load_row(blockIdx.x);
-    for (uint32_t row = blockIdx.x; row < a.m; row += gridDim.x, slot ^= 1) {
+    for (uint32_t row = blockIdx.x; row < a.m; row += gridDim.x) {
         float h[NV][8];
-        float sum = 0.f, mx = 0.f;
+        float sum = 0.f, sumOdd = 0.f, mx = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const uint32_t v = i * blockDim.x + threadIdx.x;
@@ -240,9 +271,9 @@ template <typename T, typename G, int OUT, int NV> __global__ void __launch_boun
                     float r[8];
                     widen8<T>(rs[i], r);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) h[i][j] = __fadd_rn(h[i][j], r[j]);
+                    for (int j = 0; j < 8; j += 2) add2_rn(h[i][j], h[i][j + 1], r[j], r[j + 1]);
                 }
-                if (a.residualOut) store8<T>(static_cast<T*>(a.residualOut) + row * a.ldResidualOut + v * 8, h[i]);
+                if (a.residualOut) store8<T>(static_cast<T*>(a.residualOut) + row * a.ldResidualOut + v * 8, h[i], sizeof(T) == 4 ? 0.f : max_abs8(h[i]));
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) h[i][j] = 0.f;
@@ -256,17 +287,16 @@ template <typename T, typename G, int OUT, int NV> __global__ void __launch_boun
                 float gf[8];
                 widen8<G>(g[i], gf);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    sum = fmaf(h[i][j], h[i][j], sum);
-                    h[i][j] = __fmul_rn(h[i][j], gf[j]);  // from here on h * gamma
-                    if constexpr (OUT == kOutI8) mx = max_nan(mx, fabsf(h[i][j]));
+                for (int j = 0; j < 8; j += 2) {
+                    fma2_square(sum, sumOdd, h[i][j], h[i][j + 1]);
+                    mul2_rn(h[i][j], h[i][j + 1], gf[j], gf[j + 1]);  // from here on h * gamma
                 }
+                if constexpr (OUT == kOutI8) mx = max_nan(mx, max_abs8(h[i]));
             }
         }
-        const SumMax both = cta_sum_max(sum, mx, part, slot);
-        mx = both.mx;
-        const Sum2 exact = rstd_of(both.sum, static_cast<float>(a.n), a.epsilon);
-        const float rstd = finite_f32(both.sum.hi) ? exact.hi : __int_as_float(0x7FFFFFFF);
+        const RowStats st = row_stats(sum + sumOdd, mx, part, &stats, static_cast<float>(a.n), a.epsilon);
+        const float rstd = st.rstd;
+        mx = st.mx;
         if (a.normOut) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
@@ -275,7 +305,7 @@ template <typename T, typename G, int OUT, int NV> __global__ void __launch_boun
                     float y[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) y[j] = __fmul_rn(h[i][j], rstd);
-                    store8<T>(static_cast<T*>(a.normOut) + row * a.ldNormOut + v * 8, y);
+                    store8<T>(static_cast<T*>(a.normOut) + row * a.ldNormOut + v * 8, y, max_abs8(y));
                 }
             }
         }
@@ -294,8 +324,10 @@ template <typename T, typename G, int OUT, int NV> __global__ void __launch_boun
                         for (int j = 0; j < 8; ++j) h[i][j] *= f.pre;
                     }
                     uint2 q;
-                    q.x = pack_i8x4_rni(__fmul_rn(h[i][0], f.mul), __fmul_rn(h[i][1], f.mul), __fmul_rn(h[i][2], f.mul), __fmul_rn(h[i][3], f.mul));
-                    q.y = pack_i8x4_rni(__fmul_rn(h[i][4], f.mul), __fmul_rn(h[i][5], f.mul), __fmul_rn(h[i][6], f.mul), __fmul_rn(h[i][7], f.mul));
+#pragma unroll
+                    for (int j = 0; j < 8; j += 2) mul2_rn(h[i][j], h[i][j + 1], f.mul, f.mul);
+                    q.x = pack_i8x4_rni(h[i][0], h[i][1], h[i][2], h[i][3]);
+                    q.y = pack_i8x4_rni(h[i][4], h[i][5], h[i][6], h[i][7]);
                     if (!ok) q = make_uint2(0u, 0u);
                     __stcs(reinterpret_cast<uint2*>(static_cast<int8_t*>(a.dst) + static_cast<size_t>(row) * a.n + v * 8), q);
                 }
@@ -304,20 +336,28 @@ template <typename T, typename G, int OUT, int NV> __global__ void __launch_boun
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const uint32_t v = i * blockDim.x + threadIdx.x;
-                float amax = 0.f;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) amax = max_nan(amax, fabsf(h[i][j]));
+                float amax = max_abs8(h[i]);
                 // four neighbouring lanes hold a block; n is a multiple of 32, so they are inside the row together or not at all
                 amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
                 amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 2));
                 if (v < nvec) {
                     const bool ok = finite_f32(__fmul_rn(amax, rstd));
-                    const int e = mx_exponent(amax, rstd, exact.lo, out_emax(OUT));
-                    const float up = exp2_neg(e);
+                    const int e = mx_exponent(amax, rstd, st.rstdLo, out_emax(OUT));
                     uint32_t c[4];
+                    if (__builtin_expect(ok && e > -80 && e < 80, 1)) {
+                        // rstd * 2^-e is exact: one multiplication gives what y and its scaling would
+                        const float f = __fmul_rn(rstd, exp2_neg(e));
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        c[j] = ok ? mx_pair<OUT>(__fmul_rn(__fmul_rn(h[i][2 * j], rstd), up), __fmul_rn(__fmul_rn(h[i][2 * j + 1], rstd), up)) : 0u;
+                        for (int j = 0; j < 4; ++j) {
+                            mul2_rn(h[i][2 * j], h[i][2 * j + 1], f, f);
+                            c[j] = mx_pair<OUT>(h[i][2 * j], h[i][2 * j + 1]);
+                        }
+                    } else {
+                        const float up = exp2_neg(e);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            c[j] = ok ? mx_pair<OUT>(__fmul_rn(__fmul_rn(h[i][2 * j], rstd), up), __fmul_rn(__fmul_rn(h[i][2 * j + 1], rstd), up)) : 0u;
+                    }
                     const size_t at = (static_cast<size_t>(row) * nvec + v);
                     if constexpr (OUT == kOutE2M1) static_cast<uint32_t*>(a.dst)[at] = c[0] | (c[1] << 8) | (c[2] << 16) | (c[3] << 24);
                     else __stcs(static_cast<uint2*>(a.dst) + at, make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16)));
@@ -332,7 +372,8 @@ template <typename T, typename G, int OUT, int NV> __global__ void __launch_boun
 // pass computes h again from the sources (a row is in L2).  The same arithmetic.
 template <typename T, typename G> __global__ void __launch_bounds__(256) norm_any_kernel(const NormArgs a)
 {
-    __shared__ float2 part[2][16];
+    __shared__ float2 part[16];
+    __shared__ __align__(16) RowStats stats;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint32_t row = blockIdx.x;
@@ -347,10 +388,9 @@ template <typename T, typename G> __global__ void __launch_bounds__(256) norm_an
         sum = fmaf(h, h, sum);
         mx = max_nan(mx, fabsf(__fmul_rn(h, to_f32<G>(gamma[c]))));
     }
-    const SumMax both = cta_sum_max(sum, mx, part, 0);
-    mx = both.mx;
-    const Sum2 exact = rstd_of(both.sum, static_cast<float>(a.n), a.epsilon);
-    const float rstd = finite_f32(both.sum.hi) ? exact.hi : __int_as_float(0x7FFFFFFF);
+    const RowStats st = row_stats(sum, mx, part, &stats, static_cast<float>(a.n), a.epsilon);
+    const float rstd = st.rstd;
+    mx = st.mx;
     const float top = __fmul_rn(mx, rstd);
     const bool rowOk = finite_f32(mx) && finite_f32(top);
     const I8Factor f = i8_factor(mx);
@@ -377,7 +417,7 @@ template <typename T, typename G> __global__ void __launch_bounds__(256) norm_an
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
             const bool ok = finite_f32(__fmul_rn(amax, rstd));
-            const int e = mx_exponent(amax, rstd, exact.lo, out_emax(a.out));
+            const int e = mx_exponent(amax, rstd, st.rstdLo, out_emax(a.out));
             const float v = __fmul_rn(y, exp2_neg(e));
             const float next = __shfl_down_sync(0xFFFFFFFFu, v, 1);
             if (c < a.n) {
