@@ -56,6 +56,8 @@ ascq_status w8a8_small(void* C, const int8_t* A, const int8_t* B_nk, const float
 // Sets the wait limit (SM cycles) of the bounded waits in each matmul translation unit on the current device.
 ascq_status w8a8_set_wait_cycles(long long cycles);
 ascq_status mxfp4_set_wait_cycles(long long cycles);
+ascq_status low_rank_set_wait_cycles(long long cycles);
+ascq_status low_rank_read_status(::CUstream_st* stream);  // low_rank_long.cu: its status word
 
 }  // namespace ascq
 

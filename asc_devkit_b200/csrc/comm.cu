@@ -185,5 +185,7 @@ extern "C" ascq_status ascq_set_wait_limit_cycles(long long cycles)
     g_waitCycles = cycles;
     ascq_status rc = w8a8_set_wait_cycles(cycles);
     if (rc != ASCQ_OK) return rc;
-    return mxfp4_set_wait_cycles(cycles);
+    rc = mxfp4_set_wait_cycles(cycles);
+    if (rc != ASCQ_OK) return rc;
+    return low_rank_set_wait_cycles(cycles);
 }

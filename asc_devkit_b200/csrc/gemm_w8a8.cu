@@ -1238,7 +1238,9 @@ extern "C" ascq_status ascq_matmul_status(void* stream)
         ASCQ_CUDA_CHECK(cudaMemcpyToSymbolAsync(g_w8a8_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st));
         return fail(ASCQ_ERR_TIMEOUT, "a bounded wait inside the W8A8 matmul kernel expired (status %d)", v);
     }
-    const ascq_status rc = mxfp4_read_status(st);
+    ascq_status rc = mxfp4_read_status(st);
+    if (rc != ASCQ_OK) return rc;
+    rc = low_rank_read_status(st);
     if (rc != ASCQ_OK) return rc;
     return comm_read_status(st);
 }

@@ -13,8 +13,8 @@
 // The inner product is a sum in fp32; for the second product it is split into two 16-bit terms, hi = cast(v), lo = cast(v - hi), after
 // each token's row was brought to [512, 1024) by a power of two (so that neither fp16's range nor its subnormals matter).  What the split drops is below
 // 2^-16 (bf16) or 2^-22 (fp16) of the row's largest value: the result carries one visible rounding, the one to dst's type.
-#include "elementwise.cuh"
 #include "experts.cuh"
+#include "low_rank.cuh"
 #include "sm100_ptx.cuh"
 
 using namespace ascq;
@@ -26,17 +26,6 @@ namespace {
 constexpr int kTile = 16;         // tokens of one adapter that share a tile
 constexpr int kWarps = 8;
 constexpr int kInlineTokens = 1024;  // up to here every CTA finds its tile in the adapter numbers itself; beyond, they are sorted first
-
-struct LowRankArgs {
-    const void *x, *a, *b, *base;  // base may be null (0)
-    void* dst;
-    const void* ids;
-    const float* scale;            // [L] or null (1)
-    const int64_t* counts;         // sorted: tokens per adapter, L + 1 entries (the last: tokens without one); else null
-    const int32_t* order;          // sorted: tokens in order of adapter
-    int64_t ldX, ldBase, ldDst;
-    int M, N, K, r, L, ids64;
-};
 
 __device__ __forceinline__ int adapter_of(const LowRankArgs& p, int t)
 {
@@ -52,41 +41,6 @@ struct Tile {
     int adapter;  // L: none; -1: there is no such tile
     int tokens;
 };
-
-// Warp 0 walks the token counts of the adapters (`count(e)`), 32 at a time, to the tile with the given number: its adapter,
-// the number of tokens before the tile inside the adapter, and before the adapter.
-template <int SIZE, typename F> __device__ __forceinline__ void find_tile(int tile, int keys, F count, int* out)
-{
-    const int lane = threadIdx.x & 31;
-    int tilesBefore = 0, tokensBefore = 0;
-    if (lane == 0) out[0] = -1;
-    __syncwarp();
-    for (int e0 = 0; e0 < keys; e0 += 32) {
-        const int n = e0 + lane < keys ? count(e0 + lane) : 0;
-        const int tiles = (n + SIZE - 1) / SIZE;
-        int inclTiles = tiles, inclTokens = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(0xFFFFFFFFu, inclTiles, o), v = __shfl_up_sync(0xFFFFFFFFu, inclTokens, o);
-            if (lane >= o) {
-                inclTiles += u;
-                inclTokens += v;
-            }
-        }
-        const int first = tilesBefore + inclTiles - tiles;
-        if (tile >= first && tile < first + tiles) {
-            const int at = (tile - first) * SIZE;
-            out[0] = e0 + lane;
-            out[1] = n - at < SIZE ? n - at : SIZE;
-            out[2] = at;
-            out[3] = tokensBefore + inclTokens - n + at;
-        }
-        tilesBefore += __shfl_sync(0xFFFFFFFFu, inclTiles, 31);
-        tokensBefore += __shfl_sync(0xFFFFFFFFu, inclTokens, 31);
-        if (tilesBefore > tile) break;
-    }
-    __syncwarp();
-}
 
 // Writes the tile's tokens into `list` (kTile entries, unused ones 0).  `work`: L + 1 + kWarps ints of scratch.
 __device__ __forceinline__ Tile take_tile(const LowRankArgs& p, int tile, int* list, int* found, int* work)
@@ -138,48 +92,6 @@ template <typename T> __device__ __forceinline__ void mma16816(float (&d)[4], co
     else
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi)
-{
-    uint32_t r;
-    if constexpr (std::is_same<T, __half>::value) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t v)
-{
-    if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&v));
-    else return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
-}
-
-template <typename T> __device__ __forceinline__ uint32_t pack_sat(float lo, float hi)
-{
-    if constexpr (std::is_same<T, __half>::value) return pack_f16x2_sat(lo, hi);
-    else return pack_bf16x2_sat(lo, hi);
-}
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr)
-{
-    float f;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(addr) : "memory");
-    return f;
-}
-// Exponent of the power of two that brings a row whose largest magnitude is `top` to [512, 1024); rows that are zero, subnormal or
-// not finite stay as they are.
-__device__ __forceinline__ int range_shift(float top)
-{
-    const int ex = static_cast<int>(__float_as_uint(top) >> 23);
-    return ex == 0 || ex == 255 ? 0 : min(max(ex - 136, -126), 126);
-}
-__device__ __forceinline__ float exp2_int(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
-// v as two 16-bit terms: x = cast(v), y = cast(v - x); 0 for the second where the first is not finite
-template <typename T> __device__ __forceinline__ uint2 split16(float v)
-{
-    uint2 r;
-    r.x = pack2<T>(v, 0.f) & 0xFFFFu;
-    const float back = unpack2<T>(r.x).x;
-    r.y = fabsf(back) <= 3.4028234663852886e38f ? pack2<T>(v - back, 0.f) & 0xFFFFu : 0u;
-    return r;
 }
 
 __host__ __device__ constexpr int padded_rank(int nb) { return nb * 8 < 32 ? 32 : nb * 8; }  // whole 32-wide k steps of the second product
@@ -350,279 +262,6 @@ template <typename T, int NB> __global__ void __launch_bounds__(32 * kWarps) low
     }
 }
 
-// ---- longer runs of tokens per adapter: two launches over tiles of 64 tokens -----------------------------------------------------
-// The first forms the inner products of a tile (a cluster splits K and adds up through distributed shared memory) and leaves
-// them, split in two, in the workspace in sorted order; the second adds B's product to base for a tile and a range of columns.  A and B are then
-// read from L2 once per 64 tokens, and each launch moves one side of the HBM traffic: x in the first, base and dst in the second.
-constexpr int kLong = 64;       // tokens of a tile
-constexpr int kLongWarps = 4;
-constexpr int kStages = 4;      // chunks of 64 k of A in shared memory, and of x in registers
-constexpr int kColumns = 512;   // columns of a CTA of the second launch
-
-__host__ __device__ constexpr int inner_pitch(int nb) { return nb * 8 < 32 ? 32 : nb * 8; }  // elements of the hi (or lo) part of a row
-
-struct InnerOut {
-    int4* tiles;      // adapter (-1: no such tile), first sorted token, tokens
-    void* v;          // [M][2][inner_pitch] of T
-    float* unit;      // [M]
-};
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool in)
-{
-    const int bytes = in ? 16 : 0;  // the rest of the 16 bytes is filled with zeros
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-
-// Four warps: two halves of the tile's tokens, times two halves of each chunk's k (NB <= 8) or of the rank (NB = 16).  x goes
-// from global memory to fragments directly (each element is used by one warp, for NB = 16 by two); A goes through shared memory, where a row of a
-// chunk is 128 bytes and its 16-byte pieces are exchanged between the halves on odd rows, so that 8 lanes of a 16-byte
-// read cover all banks.
-template <typename T, int NB> __global__ void __launch_bounds__(32 * kLongWarps) low_rank_inner_kernel(const LowRankArgs p, const InnerOut o, int clusterCtas)
-{
-    constexpr int R = NB * 8, WR = NB > 8 ? 2 : 1, WK = 2 / WR, NBW = NB / WR, STEPS = 2 / WK, DEPTH = kStages / STEPS;
-    constexpr int kStageBytes = R * 128, kPitch = R + 8;  // kPitch: floats of a row of the partial sums
-    extern __shared__ __align__(128) uint8_t ring[];
-    __shared__ int found[4];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const int wm = warp & 1, wk = WK == 2 ? warp >> 1 : 0, wr = WR == 2 ? warp >> 1 : 0;
-    const int tileIdx = blockIdx.x / clusterCtas, rank = blockIdx.x % clusterCtas;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (warp == 0) find_tile<kLong>(tileIdx, p.L + 1, [&](int e) { return static_cast<int>(p.counts[e]); }, found);
-    __syncthreads();
-    const int adapter = found[0], tokens = adapter < 0 ? 0 : found[1], start = adapter < 0 ? 0 : found[3];
-    if (rank == 0 && threadIdx.x == 0) o.tiles[tileIdx] = make_int4(adapter, start, tokens, 0);
-    if (adapter < 0 || adapter >= p.L) return;  // the same for every CTA of the cluster
-
-    const T* a = static_cast<const T*>(p.a) + static_cast<size_t>(adapter) * p.r * p.K;
-    const T* x[4];
-    bool in[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int row = wm * 32 + g + 8 * i;
-        in[i] = row < tokens;
-        x[i] = static_cast<const T*>(p.x) + static_cast<int64_t>(in[i] ? p.order[start + row] : 0) * p.ldX;
-    }
-    const int chunks = (p.K + 63) / 64, per = (chunks + clusterCtas - 1) / clusterCtas;
-    const int first = rank * per, last = min(first + per, chunks);
-    const uint32_t base = smem_u32(ring);
-    auto load_a = [&](int ck) {
-        const uint32_t slot = base + (ck - first) % kStages * kStageBytes;
-#pragma unroll
-        for (int i = 0; i < (NB * 64 + 127) / 128; ++i) {
-            const int idx = i * 128 + threadIdx.x, row = idx >> 3, ch = idx & 7, k = ck * 64 + ch * 8;
-            const bool ok = row < p.r && k < p.K;
-            if (NB * 64 % 128 == 0 || row < R)
-                cp_async16(slot + row * 128 + ((ch ^ ((row & 1) << 2)) << 4), ok ? a + static_cast<size_t>(row) * p.K + k : a, ok);
-        }
-    };
-    uint4 xs[DEPTH][STEPS][4];
-    auto load_x = [&](uint4 (&to)[STEPS][4], int ck) {
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-            const int k = ck * 64 + (WK == 2 ? wk : s) * 32 + c * 8;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) to[s][i] = in[i] && k < p.K && ck < last ? __ldcs(reinterpret_cast<const uint4*>(x[i] + k)) : make_uint4(0u, 0u, 0u, 0u);
-        }
-    };
-#pragma unroll
-    for (int d = 0; d < kStages - 1; ++d) {
-        if (first + d < last) load_a(first + d);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    }
-#pragma unroll
-    for (int d = 0; d < DEPTH; ++d) load_x(xs[d], first + d);
-
-    float acc[2][NBW][4] = {};
-    for (int ck0 = first; ck0 < last; ck0 += DEPTH) {
-#pragma unroll
-        for (int d = 0; d < DEPTH; ++d) {
-            const int ck = ck0 + d;
-            if (ck >= last) break;
-            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-            __syncthreads();  // chunk ck is there for all, and the slot of chunk ck - 1 is read no more
-            if (ck + kStages - 1 < last) load_a(ck + kStages - 1);
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            const uint8_t* slot = ring + (ck - first) % kStages * kStageBytes;
-#pragma unroll
-            for (int s = 0; s < STEPS; ++s) {
-                const int half = WK == 2 ? wk : s;
-                const uint4(&f)[4] = xs[d][s];
-                const uint32_t f0[2][4] = {{f[0].x, f[1].x, f[0].y, f[1].y}, {f[2].x, f[3].x, f[2].y, f[3].y}};
-                const uint32_t f1[2][4] = {{f[0].z, f[1].z, f[0].w, f[1].w}, {f[2].z, f[3].z, f[2].w, f[3].w}};
-                uint4 w[NBW];
-#pragma unroll
-                for (int n = 0; n < NBW; ++n) w[n] = *reinterpret_cast<const uint4*>(slot + ((wr * NBW + n) * 8 + g) * 128 + (((half * 4 + c) ^ ((g & 1) << 2)) << 4));
-                // MMAs on the same accumulator are kept apart: each waits for the one before
-#pragma unroll
-                for (int n = 0; n < NBW; ++n)
-#pragma unroll
-                    for (int m = 0; m < 2; ++m) mma16816<T>(acc[m][n], f0[m], w[n].x, w[n].y);
-#pragma unroll
-                for (int n = 0; n < NBW; ++n)
-#pragma unroll
-                    for (int m = 0; m < 2; ++m) mma16816<T>(acc[m][n], f1[m], w[n].z, w[n].w);
-            }
-            load_x(xs[d], ck + DEPTH);
-        }
-    }
-    __syncthreads();  // the ring is read no more (and no copy is pending: every chunk was waited for)
-    float* part = reinterpret_cast<float*>(ring);
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int n = 0; n < NBW; ++n) {
-            float* to = part + (wk * kLong + wm * 32 + m * 16 + g) * kPitch + (wr * NBW + n) * 8 + 2 * c;
-            *reinterpret_cast<float2*>(to) = make_float2(acc[m][n][0], acc[m][n][1]);
-            *reinterpret_cast<float2*>(to + 8 * kPitch) = make_float2(acc[m][n][2], acc[m][n][3]);
-        }
-    __syncthreads();
-    if constexpr (WK == 2) {
-        for (int i = threadIdx.x; i < kLong * kPitch; i += blockDim.x) part[i] += part[kLong * kPitch + i];
-    }
-    __syncthreads();
-    cluster_arrive();
-    cluster_wait();
-    const float scale = p.scale ? p.scale[adapter] : 1.0f;
-    constexpr int VP = inner_pitch(NB);
-    for (int row = rank * kLongWarps + warp; row < tokens; row += clusterCtas * kLongWarps) {
-        float v[(VP + 31) / 32];
-        float top = 0.f;
-#pragma unroll
-        for (int i = 0; i < VP / 32; ++i) {
-            const int col = lane + 32 * i;
-            v[i] = 0.f;
-            if (col < R) {
-                const uint32_t at = smem_u32(part + row * kPitch + col);
-                for (int q = 0; q < clusterCtas; ++q) v[i] += ld_cluster_f32(mapa_u32(at, q));
-                v[i] *= scale;
-            }
-            top = fmaxf(top, fabsf(v[i]));
-        }
-#pragma unroll
-        for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, s));
-        const int shift = range_shift(top);
-        const float down = exp2_int(-shift);
-        if (lane == 0) o.unit[start + row] = exp2_int(shift);
-        unsigned short* to = static_cast<unsigned short*>(o.v) + static_cast<size_t>(start + row) * 2 * VP;
-#pragma unroll
-        for (int i = 0; i < VP / 32; ++i) {
-            const uint2 h = split16<T>(v[i] * down);
-            to[lane + 32 * i] = static_cast<unsigned short>(h.x);
-            to[VP + lane + 32 * i] = static_cast<unsigned short>(h.y);
-        }
-    }
-    __syncwarp();
-    cluster_arrive();  // no CTA ends while another reads its sums
-    cluster_wait();
-}
-
-// A warp keeps the split inner products of its tokens (32, or 16 for ranks above 64) in registers and walks over groups of
-// 32 columns; B and base come straight to fragments and the next group's are requested before this one's products.
-template <typename T, int NB> __global__ void __launch_bounds__(32 * kLongWarps) low_rank_outer_kernel(const LowRankArgs p, const InnerOut o)
-{
-    constexpr int VP = inner_pitch(NB), KS = VP / 32, MT = NB > 8 ? 1 : 2, WM = kLong / (16 * MT), WN = kLongWarps / WM;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const int wm = warp % WM, wn = warp / WM;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int4 tile = o.tiles[blockIdx.y];
-    const int adapter = tile.x, start = tile.y, tokens = tile.z;
-    if (adapter < 0 || wm * 16 * MT >= tokens) return;
-    const bool has = adapter < p.L;
-    if (!has && p.base == p.dst) return;
-    const T* base[2 * MT];
-    T* dst[2 * MT];
-    bool in[2 * MT];
-    float unit[2 * MT];
-    uint32_t f[2][MT][KS][2][4];  // hi / lo, 16 tokens, 32 of the rank, 16 of them
-#pragma unroll
-    for (int i = 0; i < 2 * MT; ++i) {
-        const int row = wm * 16 * MT + g + 8 * i;
-        in[i] = row < tokens;
-        const int64_t t = in[i] ? p.order[start + row] : 0;
-        base[i] = p.base ? static_cast<const T*>(p.base) + t * p.ldBase : nullptr;
-        dst[i] = static_cast<T*>(p.dst) + t * p.ldDst;
-        unit[i] = has && in[i] ? o.unit[start + row] : 0.f;
-        const T* v = static_cast<const T*>(o.v) + static_cast<size_t>(start + (in[i] ? row : 0)) * 2 * VP;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                const uint4 w = has && in[i] ? *reinterpret_cast<const uint4*>(v + h * VP + s * 32 + c * 8) : make_uint4(0u, 0u, 0u, 0u);
-                f[h][i >> 1][s][0][i & 1] = w.x;
-                f[h][i >> 1][s][0][2 + (i & 1)] = w.y;
-                f[h][i >> 1][s][1][i & 1] = w.z;
-                f[h][i >> 1][s][1][2 + (i & 1)] = w.w;
-            }
-    }
-    const T* b = static_cast<const T*>(p.b) + static_cast<size_t>(has ? adapter : 0) * p.N * p.r;
-    const int nEnd = min(p.N, static_cast<int>(blockIdx.x + 1) * kColumns);
-    uint4 y[2 * MT];
-    auto load_base = [&](int n0) {
-        const int col = n0 + c * 8;
-#pragma unroll
-        for (int i = 0; i < 2 * MT; ++i) y[i] = base[i] && in[i] && col < nEnd ? *reinterpret_cast<const uint4*>(base[i] + col) : make_uint4(0u, 0u, 0u, 0u);
-    };
-    uint4 w[4][KS];
-    auto load_b = [&](int n0) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            // column g of MMA j is column 8 (g / 2) + 2 j + (g & 1) of the group: accumulators 2c, 2c + 1 of the four MMAs are 8 neighbours
-            const int n = n0 + 8 * (g >> 1) + 2 * j + (g & 1);
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                const int k = s * 32 + c * 8;
-                w[j][s] = has && n < nEnd && k < p.r ? __ldg(reinterpret_cast<const uint4*>(b + static_cast<size_t>(n) * p.r + k)) : make_uint4(0u, 0u, 0u, 0u);
-            }
-        }
-    };
-    int n0 = blockIdx.x * kColumns + wn * 32;
-    load_base(n0);
-    load_b(n0);
-    for (; n0 < nEnd; n0 += WN * 32) {
-        float acc[MT][4][4] = {};
-        if (has) {
-            uint4 wNow[4][KS];
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int s = 0; s < KS; ++s) wNow[j][s] = w[j][s];
-            load_b(n0 + WN * 32);
-            // MMAs on the same accumulator are kept apart: each waits for the one before
-#pragma unroll
-            for (int s = 0; s < KS; ++s)
-#pragma unroll
-                for (int q = 0; q < 2; ++q)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-#pragma unroll
-                            for (int m = 0; m < MT; ++m)
-                                mma16816<T>(acc[m][j], f[h][m][s][q], q ? wNow[j][s].z : wNow[j][s].x, q ? wNow[j][s].w : wNow[j][s].y);
-        }
-        uint4 now[2 * MT];
-#pragma unroll
-        for (int i = 0; i < 2 * MT; ++i) now[i] = y[i];
-        load_base(n0 + WN * 32);
-        const int col = n0 + c * 8;
-        if (col >= nEnd) continue;
-#pragma unroll
-        for (int i = 0; i < 2 * MT; ++i) {
-            if (!in[i]) continue;
-            uint32_t out[4];
-            const uint32_t was[4] = {now[i].x, now[i].y, now[i].z, now[i].w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float2 v = unpack2<T>(was[j]);
-                out[j] = has ? pack_sat<T>(fmaf(acc[i >> 1][j][2 * (i & 1)], unit[i], v.x), fmaf(acc[i >> 1][j][2 * (i & 1) + 1], unit[i], v.y)) : was[j];
-            }
-            __stcs(reinterpret_cast<uint4*>(dst[i] + col), make_uint4(out[0], out[1], out[2], out[3]));
-        }
-    }
-}
-
 template <typename T, int NB> ascq_status launch_low_rank(const LowRankArgs& p, int cluster, unsigned tiles, cudaStream_t st)
 {
     const size_t smem = (static_cast<size_t>(red_words(NB, p.L)) + part_words(NB) + split_words(NB)) * 4;
@@ -659,51 +298,7 @@ template <typename T> ascq_status launch_low_rank_typed(const LowRankArgs& p, in
     return launch_low_rank<T, 16>(p, cluster, tiles, st);
 }
 
-template <typename K, typename... Args>
-cudaError_t launch_pdl(K kernel, dim3 grid, unsigned block, size_t smem, int cluster, cudaStream_t st, Args... args)
-{
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(block, 1, 1);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = cluster > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
-template <typename T, int NB> ascq_status launch_low_rank_long(const LowRankArgs& p, const InnerOut& o, unsigned tiles, cudaStream_t st)
-{
-    constexpr int ringBytes = kStages * NB * 8 * 128, sumBytes = (NB > 8 ? 1 : 2) * kLong * (NB * 8 + 8) * 4;
-    constexpr int smem = ringBytes > sumBytes ? ringBytes : sumBytes;
-    static PerDeviceOnce once;
-    const int dev = current_device();
-    if (!once.done(dev)) {
-        ASCQ_CUDA_CHECK(cudaFuncSetAttribute(low_rank_inner_kernel<T, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        once.mark(dev);
-    }
-    // K is split until there are about two CTAs per SM; a CTA keeps at least four chunks of 64
-    int cluster = 8;
-    while (cluster > 1 && (static_cast<uint64_t>(tiles) * cluster > 3ull * sm_count() || p.K < cluster * 256)) cluster /= 2;
-    ASCQ_CUDA_CHECK(launch_pdl(low_rank_inner_kernel<T, NB>, dim3(tiles * cluster), 32 * kLongWarps, smem, cluster, st, p, o, cluster));
-    ASCQ_CUDA_CHECK(launch_pdl(low_rank_outer_kernel<T, NB>, dim3((p.N + kColumns - 1) / kColumns, tiles), 32 * kLongWarps, 0, 1, st, p, o));
-    return ASCQ_OK;
-}
-template <typename T> ascq_status launch_low_rank_long_typed(const LowRankArgs& p, const InnerOut& o, unsigned tiles, cudaStream_t st)
-{
-    if (p.r <= 16) return launch_low_rank_long<T, 2>(p, o, tiles, st);
-    if (p.r <= 32) return launch_low_rank_long<T, 4>(p, o, tiles, st);
-    if (p.r <= 64) return launch_low_rank_long<T, 8>(p, o, tiles, st);
-    return launch_low_rank_long<T, 16>(p, o, tiles, st);
-}
-
-// Tiles of 64 tokens pay when an adapter has enough tokens to fill them.
+// Tiles of 128 tokens pay when an adapter has enough tokens to fill them.
 bool long_tiles(int M, int L) { return M > kInlineTokens && M / (L + 1) >= 16; }
 
 // Every adapter with tokens, and the tokens without one, can leave one tile partly filled.
@@ -721,9 +316,9 @@ Workspace workspace_of(int M, int r, int L)
     w.bytes = w.order + up(static_cast<size_t>(M) * 4);
     if (long_tiles(M, L)) {
         w.tiles = w.bytes;
-        w.unit = w.tiles + static_cast<size_t>(tile_bound(M, L, kLong)) * 16;
+        w.unit = w.tiles + low_rank_long_tiles_bytes(tile_bound(M, L, kLongTile));
         w.v = w.unit + up(static_cast<size_t>(M) * 4);
-        w.bytes = w.v + static_cast<size_t>(M) * 2 * inner_pitch(r <= 32 ? 4 : r <= 64 ? 8 : 16) * 2;
+        w.bytes = w.v + low_rank_long_inner_bytes(M, r);
     }
     return w;
 }
@@ -786,11 +381,10 @@ extern "C" ascq_status ascq_low_rank_add(void* dst, int64_t ldDst, const void* b
         p.counts = counts;
         p.order = order;
         if (ws.tiles) {
-            const InnerOut o{reinterpret_cast<int4*>(w + ws.tiles), w + ws.v, reinterpret_cast<float*>(w + ws.unit)};
-            const int64_t tiles = tile_bound(M, L, kLong);
+            const LowRankScratch o{w + ws.tiles, w + ws.v, reinterpret_cast<float*>(w + ws.unit)};
+            const int64_t tiles = tile_bound(M, L, kLongTile);
             if (tiles > 65535) return fail(ASCQ_ERR_INVALID_ARG, "M is too large for one launch");
-            return T == ASCQ_DT_F16 ? launch_low_rank_long_typed<__half>(p, o, static_cast<unsigned>(tiles), st)
-                                    : launch_low_rank_long_typed<__nv_bfloat16>(p, o, static_cast<unsigned>(tiles), st);
+            return low_rank_long(p, T == ASCQ_DT_F16, o, static_cast<unsigned>(tiles), st);
         }
     }
     const unsigned tiles = static_cast<unsigned>(tile_bound(M, L, kTile));

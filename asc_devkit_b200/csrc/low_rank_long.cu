@@ -1,0 +1,457 @@
+// The form of ascq_low_rank_add for adapters with many tokens (prompts): two launches over tiles of up to 128 tokens of one adapter, tokens
+// in sorted order, both products on tcgen05 with the accumulators in tensor memory.
+//   inner   V = scale * x . A^T: a cluster of CTAs splits K and adds up through distributed shared memory; V leaves split into two 16-bit
+//           terms, [M][2][pitch] in sorted order, with one power of two per token
+//   outer   dst = base + V . B^T for a tile and a range of columns
+// What bounds both is HBM: the inner launch reads x once, the outer one reads base and writes dst; A and B come from L2 once per 128
+// tokens.  The tokens of a tile lie anywhere, so rows are gathered with 16-byte cp.async into the 128-byte-swizzled layout that the
+// tensor cores read; 64 elements of a row are 128 bytes, and the eight lanes that share a row fill a whole line.
+#include "low_rank.cuh"
+#include "sm100_ptx.cuh"
+
+using namespace ascq;
+using namespace ascq::ptx;
+
+namespace ascq {
+namespace {
+
+constexpr int kRows = kLongTile;
+constexpr int kLoaders = 128;              // threads of the four warps that copy and finish; a fifth warp issues the MMAs
+constexpr int kThreads = kLoaders + 32;
+constexpr int kAtomBytes = kRows * 128;    // 128 rows x 64 elements
+constexpr int kBlockCols = 64, kColumns = 512, kBlocks = kColumns / kBlockCols;  // outer: columns of an MMA, of a CTA
+
+__device__ int g_low_rank_status;  // 1: a bounded wait ran out
+
+__host__ __device__ constexpr int rank_pitch(int nb) { return nb * 8 < 32 ? 32 : nb * 8; }  // elements of the hi (or lo) part of a row of V
+constexpr int rank_blocks(int r) { return r <= 16 ? 2 : r <= 32 ? 4 : r <= 64 ? 8 : 16; }
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool in)
+{
+    const int bytes = in ? 16 : 0;  // the rest of the 16 bytes is filled with zeros
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// this thread's finished copies become visible to the tensor cores, and the barrier learns of it
+__device__ __forceinline__ void publish(uint64_t* bar)
+{
+    fence_proxy_async();
+    mbar_arrive(bar);
+}
+
+// Chunks of 64 k in flight.  A copy is announced LAG chunks after it was requested; its slot is asked for again two chunks after
+// that, so the MMAs that read it have had a chunk's time.
+template <int NB> struct Ring {
+    static constexpr int kStages = 4, kLag = 2;
+    static constexpr int kABytes = NB * 8 * 128, kStageBytes = kAtomBytes + kABytes;
+    static constexpr int kSumBytes = kRows * (NB * 8 + 1) * 4;
+    static constexpr int kBytes = (kStages * kStageBytes > kSumBytes ? kStages * kStageBytes : kSumBytes) + 1024;  // + alignment
+    static constexpr uint32_t kTmemCols = NB * 8 < 32 ? 32 : NB * 8;
+};
+
+template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_rank_inner_kernel(const LowRankArgs p, const LowRankScratch o, int clusterCtas)
+{
+    using C = Ring<NB>;
+    constexpr int R = NB * 8, VP = rank_pitch(NB), kPitch = R + 1;
+    extern __shared__ uint8_t raw[];
+    __shared__ int found[4];
+    __shared__ uint64_t fullBar[C::kStages], emptyBar[C::kStages], doneBar;
+    __shared__ uint32_t tmemSlot;
+    __shared__ int abortFlag;
+    uint8_t* ring = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int tileIdx = blockIdx.x / clusterCtas, rank = blockIdx.x % clusterCtas;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::kStages; ++i) {
+            mbar_init(&fullBar[i], kLoaders);
+            mbar_init(&emptyBar[i], 1);
+        }
+        mbar_init(&doneBar, 1);
+        fence_barrier_init();
+        abortFlag = 0;
+    }
+    if (warp == 4) {
+        tmem_alloc(&tmemSlot, C::kTmemCols);
+        tmem_relinquish();
+    }
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (warp == 0) find_tile<kRows>(tileIdx, p.L + 1, [&](int e) { return static_cast<int>(p.counts[e]); }, found);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const int adapter = found[0], tokens = adapter < 0 ? 0 : found[1], start = adapter < 0 ? 0 : found[3];
+    if (rank == 0 && threadIdx.x == 0) static_cast<int4*>(o.tiles)[tileIdx] = make_int4(adapter, start, tokens, 0);
+    const bool has = adapter >= 0 && adapter < p.L;  // the same for every CTA of the cluster
+    if (has) {
+        const int chunks = (p.K + 63) / 64, per = (chunks + clusterCtas - 1) / clusterCtas;
+        const int first = min(rank * per, chunks), n = min(first + per, chunks) - first;
+        bool ok = true;
+        if (warp < 4) {
+            // 16 rows at a time, eight lanes a row: row (t / 8) + 16 i, piece t % 8; the swizzle exchanges pieces by the row's low three bits
+            const int piece = threadIdx.x & 7, row0 = threadIdx.x >> 3;
+            const uint32_t at = smem_u32(ring) + row0 * 128 + ((piece ^ (row0 & 7)) << 4);
+            const T* x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int row = row0 + 16 * i;
+                x[i] = row < tokens ? static_cast<const T*>(p.x) + static_cast<int64_t>(p.order[start + row]) * p.ldX + first * 64 + piece * 8 : nullptr;
+            }
+            const T* a = static_cast<const T*>(p.a) + (static_cast<size_t>(adapter) * p.r + row0) * p.K + first * 64 + piece * 8;
+            for (int i = 0; i < n && ok; ++i) {
+                const int s = i % C::kStages;
+                if (i >= C::kStages && !(ok = mbar_wait_bounded(&emptyBar[s], (i / C::kStages - 1) & 1, &abortFlag))) break;
+                const bool kIn = (first + i) * 64 + piece * 8 < p.K;
+                const uint32_t slot = at + s * C::kStageBytes;
+                // a row without a token keeps whatever the slot holds: a row of A times it is a row of D that nobody reads
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (x[j]) cp_async16(slot + j * 2048, kIn ? x[j] + i * 64 : p.x, kIn);
+#pragma unroll
+                for (int j = 0; j < NB / 2; ++j) {
+                    const bool in = kIn && row0 + 16 * j < p.r;
+                    cp_async16(slot + kAtomBytes + j * 2048, in ? a + static_cast<size_t>(16 * j) * p.K + i * 64 : p.a, in);
+                }
+                cp_commit();
+                if (i >= C::kLag) {
+                    cp_wait<C::kLag>();
+                    publish(&fullBar[(i - C::kLag) % C::kStages]);
+                }
+            }
+            cp_wait<0>();
+            if (ok)
+                for (int i = max(n - C::kLag, 0); i < n; ++i) publish(&fullBar[i % C::kStages]);
+        } else if (elect_one()) {
+            constexpr uint32_t idesc = idesc_f16(kRows, R, std::is_same<T, __half>::value ? 0 : 1);
+            for (int i = 0; i < n && ok; ++i) {
+                const int s = i % C::kStages;
+                if (!(ok = mbar_wait_bounded(&fullBar[s], (i / C::kStages) & 1, &abortFlag))) break;
+                tc_fence_after();
+                const uint32_t at = smem_u32(ring) + s * C::kStageBytes;
+                const uint64_t descX = smem_desc_sw128(at), descA = smem_desc_sw128(at + kAtomBytes);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) mma_f16(tmemSlot, descX + 2 * k, descA + 2 * k, idesc, (i | k) != 0);
+                tc_commit(&emptyBar[s]);
+            }
+            if (ok && n > 0) tc_commit(&doneBar);
+        }
+        __syncwarp();
+        float* part = reinterpret_cast<float*>(ring);  // free: every chunk was copied and multiplied before doneBar completed
+        if (warp < 4) {
+            if (n > 0) ok = ok && mbar_wait_bounded(&doneBar, 0, &abortFlag);
+            __syncwarp();
+            tc_fence_after();
+            float* to = part + threadIdx.x * kPitch;
+#pragma unroll
+            for (int c0 = 0; c0 < R; c0 += 32) {
+                uint32_t v[32];
+                if (n > 0) {
+                    tmem_ld_32x32b_x32(tmemSlot + (static_cast<uint32_t>(warp * 32) << 16) + c0, v);
+                    tmem_ld_wait();
+                }
+#pragma unroll
+                for (int c = 0; c < 32; ++c)
+                    if (c0 + c < R) to[c0 + c] = n > 0 ? __uint_as_float(v[c]) : 0.f;
+            }
+        }
+        __syncthreads();
+        cluster_arrive();
+        cluster_wait();
+        if (warp < 4) {
+            const float scale = p.scale ? p.scale[adapter] : 1.0f;
+            const int step = clusterCtas * 4;
+            for (int row0 = rank * 4 + warp; row0 < tokens; row0 += 4 * step) {
+                float v[4][VP / 32] = {}, top[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int row = min(row0 + u * step, kRows - 1);
+#pragma unroll
+                    for (int i = 0; i < VP / 32; ++i) {
+                        const int col = lane + 32 * i;
+                        if (col < R) {
+                            const uint32_t at = smem_u32(part + row * kPitch + col);
+                            for (int q = 0; q < clusterCtas; ++q) v[u][i] += ld_cluster_f32(mapa_u32(at, q));
+                        }
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    top[u] = 0.f;
+#pragma unroll
+                    for (int i = 0; i < VP / 32; ++i) {
+                        v[u][i] *= scale;
+                        top[u] = fmaxf(top[u], fabsf(v[u][i]));
+                    }
+#pragma unroll
+                    for (int s = 16; s > 0; s >>= 1) top[u] = fmaxf(top[u], __shfl_xor_sync(0xFFFFFFFFu, top[u], s));
+                    const int row = row0 + u * step;
+                    if (row >= tokens) continue;
+                    const int shift = range_shift(top[u]);
+                    const float down = exp2_int(-shift);
+                    if (lane == 0) o.unit[start + row] = exp2_int(shift);
+                    unsigned short* to = static_cast<unsigned short*>(o.v) + static_cast<size_t>(start + row) * 2 * VP;
+#pragma unroll
+                    for (int i = 0; i < VP / 32; ++i) {
+                        const uint2 h = split16<T>(v[u][i] * down);
+                        to[lane + 32 * i] = static_cast<unsigned short>(h.x);
+                        to[VP + lane + 32 * i] = static_cast<unsigned short>(h.y);
+                    }
+                }
+            }
+        }
+        __syncwarp();
+        cluster_arrive();  // no CTA ends while another reads its sums
+        cluster_wait();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 4) {
+        tc_fence_after();
+        tmem_dealloc(tmemSlot, C::kTmemCols);
+    }
+    if (threadIdx.x == 0 && abortFlag) atomicExch(&g_low_rank_status, 1);
+}
+
+// Shared memory of the outer kernel: V's two terms, three blocks of 64 columns of B, three of base (which dst's values replace).
+template <int NB> struct Outer {
+    static constexpr int kAtoms = rank_pitch(NB) > 64 ? 2 : 1;
+    static constexpr int kVBytes = 2 * kAtoms * kAtomBytes, kBBytes = kAtoms * kBlockCols * 128, kYBytes = kRows * 128;
+    static constexpr int kBytes = kVBytes + 3 * (kBBytes + kYBytes) + 1024;
+};
+
+template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_rank_outer_kernel(const LowRankArgs p, const LowRankScratch o)
+{
+    using C = Outer<NB>;
+    constexpr int VP = rank_pitch(NB);
+    extern __shared__ uint8_t raw[];
+    __shared__ uint64_t inBar[3], outBar[2];
+    __shared__ uint32_t tmemSlot;
+    __shared__ int abortFlag;
+    uint8_t* sV = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+    uint8_t *sB = sV + C::kVBytes, *sY = sB + 3 * C::kBBytes;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 3; ++i) mbar_init(&inBar[i], kLoaders);
+        mbar_init(&outBar[0], 1);
+        mbar_init(&outBar[1], 1);
+        fence_barrier_init();
+        abortFlag = 0;
+    }
+    if (warp == 4) {
+        tmem_alloc(&tmemSlot, 2 * kBlockCols);
+        tmem_relinquish();
+    }
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int4 tile = static_cast<const int4*>(o.tiles)[blockIdx.y];
+    const int adapter = tile.x, start = tile.y, tokens = tile.z;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const int col0 = blockIdx.x * kColumns, colEnd = min(p.N, col0 + kColumns), blocks = (colEnd - col0 + kBlockCols - 1) / kBlockCols;
+    const bool has = adapter >= 0 && adapter < p.L;
+    bool ok = true;
+    if (adapter == p.L) {
+        // tokens without an adapter: base as it is
+        if (p.base != p.dst)
+            for (int row = warp; row < tokens; row += 5) {
+                const int64_t t = p.order[start + row];
+                for (int col = col0 + lane * 8; col < colEnd; col += 256) {
+                    const uint4 v = p.base ? *reinterpret_cast<const uint4*>(static_cast<const T*>(p.base) + t * p.ldBase + col) : make_uint4(0u, 0u, 0u, 0u);
+                    *reinterpret_cast<uint4*>(static_cast<T*>(p.dst) + t * p.ldDst + col) = v;
+                }
+            }
+    } else if (has && warp < 4) {
+        const int piece = threadIdx.x & 7, row0 = threadIdx.x >> 3;
+        // V, 16 rows at a time
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int row = row0 + 16 * i;
+            if (row < tokens) {
+                const T* v = static_cast<const T*>(o.v) + static_cast<size_t>(start + row) * 2 * VP + piece * 8;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int ka = 0; ka < C::kAtoms; ++ka)
+                        if (VP >= 64 || piece < 4)
+                            cp_async16(smem_u32(sV) + (h * C::kAtoms + ka) * kAtomBytes + row * 128 + ((piece ^ (row & 7)) << 4), v + h * VP + ka * 64, true);
+            }
+        }
+        // the lanes' tokens: lane l of the warp holds row 32 w + l, and moves piece l % 8 of the rows l / 8 + 4 i
+        const int myRow = warp * 32 + lane;
+        const bool mine = myRow < tokens;
+        const int token = mine ? p.order[start + myRow] : -1;
+        const float unit = mine ? o.unit[start + myRow] : 0.f;
+        const T* bRow = static_cast<const T*>(p.b) + (static_cast<size_t>(adapter) * p.N + row0) * p.r + piece * 8;
+        auto request = [&](int b) {
+            if (b < blocks) {
+                const int n0 = col0 + b * kBlockCols, s = b % 3;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int n = row0 + 16 * i;
+#pragma unroll
+                    for (int ka = 0; ka < C::kAtoms; ++ka) {
+                        const bool in = n0 + n < p.N && ka * 64 + piece * 8 < p.r;
+                        cp_async16(smem_u32(sB) + s * C::kBBytes + ka * kBlockCols * 128 + n * 128 + ((piece ^ (n & 7)) << 4),
+                                   in ? bRow + static_cast<size_t>(n0 + 16 * i) * p.r + ka * 64 : p.b, in);
+                    }
+                }
+                if (p.base) {
+                    const int col = n0 + piece * 8;
+                    const uint32_t y = smem_u32(sY) + s * C::kYBytes + warp * 32 * 128;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int r = i * 4 + (lane >> 3);
+                        const int t = __shfl_sync(0xFFFFFFFFu, token, r);
+                        if (t >= 0 && col < colEnd)
+                            cp_async16(y + r * 128 + ((piece ^ (r & 7)) << 4), static_cast<const T*>(p.base) + static_cast<int64_t>(t) * p.ldBase + col, true);
+                    }
+                }
+            }
+            cp_commit();
+        };
+        request(0);
+        request(1);
+        cp_wait<1>();
+        publish(&inBar[0]);
+        for (int b = 0; b < blocks; ++b) {
+            __syncwarp();  // the warp has read the values of block b - 1 out of the slot that is filled now
+            request(b + 2);
+            cp_wait<1>();
+            if (b + 1 < blocks) publish(&inBar[(b + 1) % 3]);
+            __syncwarp();  // base's values of block b, copied by the warp's lanes, are there for all of them
+            if (!(ok = mbar_wait_bounded(&outBar[b & 1], (b >> 1) & 1, &abortFlag))) break;
+            __syncwarp();
+            tc_fence_after();
+            uint8_t* y = sY + (b % 3) * C::kYBytes + myRow * 128;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                uint32_t acc[32];
+                tmem_ld_32x32b_x32(tmemSlot + (static_cast<uint32_t>(warp * 32) << 16) + (b & 1) * kBlockCols + half * 32, acc);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint4* at = reinterpret_cast<uint4*>(y + (((half * 4 + j) ^ (myRow & 7)) << 4));
+                    const uint4 was = p.base ? *at : make_uint4(0u, 0u, 0u, 0u);
+                    const uint32_t w[4] = {was.x, was.y, was.z, was.w};
+                    uint32_t r[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const float2 f = unpack2<T>(w[q]);
+                        r[q] = pack_sat<T>(fmaf(__uint_as_float(acc[j * 8 + 2 * q]), unit, f.x), fmaf(__uint_as_float(acc[j * 8 + 2 * q + 1]), unit, f.y));
+                    }
+                    *at = make_uint4(r[0], r[1], r[2], r[3]);
+                }
+            }
+            tc_fence_before();  // the next arrival on inBar lets the MMAs overwrite this accumulator
+            __syncwarp();
+            const int col = col0 + b * kBlockCols + piece * 8;
+            const uint8_t* out = sY + (b % 3) * C::kYBytes + warp * 32 * 128;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = i * 4 + (lane >> 3);
+                const int t = __shfl_sync(0xFFFFFFFFu, token, r);
+                if (t >= 0 && col < colEnd)
+                    __stcs(reinterpret_cast<uint4*>(static_cast<T*>(p.dst) + static_cast<int64_t>(t) * p.ldDst + col),
+                           *reinterpret_cast<const uint4*>(out + r * 128 + ((piece ^ (r & 7)) << 4)));
+            }
+        }
+        cp_wait<0>();
+    } else if (has && elect_one()) {
+        constexpr uint32_t idesc = idesc_f16(kRows, kBlockCols, std::is_same<T, __half>::value ? 0 : 1);
+        const int steps = (p.r + 15) / 16;
+        for (int b = 0; b < blocks; ++b) {
+            if (!(ok = mbar_wait_bounded(&inBar[b % 3], (b / 3) & 1, &abortFlag))) break;
+            tc_fence_after();
+            const uint32_t v = smem_u32(sV), w = smem_u32(sB) + (b % 3) * C::kBBytes;
+            for (int h = 0; h < 2; ++h)
+                for (int k = 0; k < steps; ++k)
+                    mma_f16(tmemSlot + (b & 1) * kBlockCols, smem_desc_sw128(v + (h * C::kAtoms + (k >> 2)) * kAtomBytes) + 2 * (k & 3),
+                            smem_desc_sw128(w + (k >> 2) * kBlockCols * 128) + 2 * (k & 3), idesc, (h | k) != 0);
+            tc_commit(&outBar[b & 1]);
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 4) {
+        tc_fence_after();
+        tmem_dealloc(tmemSlot, 2 * kBlockCols);
+    }
+    if (threadIdx.x == 0 && abortFlag) atomicExch(&g_low_rank_status, 1);
+}
+
+template <typename K, typename... Args>
+cudaError_t launch_pdl(K kernel, dim3 grid, unsigned block, size_t smem, int cluster, cudaStream_t st, Args... args)
+{
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(block, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+template <typename T, int NB> ascq_status launch_long(const LowRankArgs& p, const LowRankScratch& o, unsigned tiles, cudaStream_t st)
+{
+    static PerDeviceOnce once;
+    const int dev = current_device();
+    if (!once.done(dev)) {
+        ASCQ_CUDA_CHECK(cudaFuncSetAttribute(low_rank_inner_kernel<T, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<NB>::kBytes));
+        ASCQ_CUDA_CHECK(cudaFuncSetAttribute(low_rank_outer_kernel<T, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, Outer<NB>::kBytes));
+        once.mark(dev);
+    }
+    // K is split until there are about two CTAs per SM; a CTA keeps at least four chunks of 64
+    int cluster = 8;
+    while (cluster > 1 && (static_cast<uint64_t>(tiles) * cluster > 2ull * sm_count() || p.K < cluster * 256)) cluster /= 2;
+    ASCQ_CUDA_CHECK(launch_pdl(low_rank_inner_kernel<T, NB>, dim3(tiles * cluster), kThreads, Ring<NB>::kBytes, cluster, st, p, o, cluster));
+    ASCQ_CUDA_CHECK(launch_pdl(low_rank_outer_kernel<T, NB>, dim3((p.N + kColumns - 1) / kColumns, tiles), kThreads, Outer<NB>::kBytes, 1, st, p, o));
+    return ASCQ_OK;
+}
+template <typename T> ascq_status launch_long_typed(const LowRankArgs& p, const LowRankScratch& o, unsigned tiles, cudaStream_t st)
+{
+    switch (rank_blocks(p.r)) {
+        case 2: return launch_long<T, 2>(p, o, tiles, st);
+        case 4: return launch_long<T, 4>(p, o, tiles, st);
+        case 8: return launch_long<T, 8>(p, o, tiles, st);
+        default: return launch_long<T, 16>(p, o, tiles, st);
+    }
+}
+
+}  // namespace
+
+size_t low_rank_long_tiles_bytes(int64_t tiles) { return static_cast<size_t>(tiles) * 16; }
+size_t low_rank_long_inner_bytes(int M, int r) { return static_cast<size_t>(M) * 2 * rank_pitch(rank_blocks(r)) * 2; }
+
+ascq_status low_rank_long(const LowRankArgs& p, bool half, const LowRankScratch& o, unsigned tiles, ::CUstream_st* st)
+{
+    return half ? launch_long_typed<__half>(p, o, tiles, st) : launch_long_typed<__nv_bfloat16>(p, o, tiles, st);
+}
+
+// Reads and clears this unit's device status word (used by ascq_matmul_status).
+ascq_status low_rank_read_status(::CUstream_st* st)
+{
+    int v = 0, zero = 0;
+    ASCQ_CUDA_CHECK(cudaMemcpyFromSymbolAsync(&v, g_low_rank_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st));
+    ASCQ_CUDA_CHECK(cudaStreamSynchronize(st));
+    if (v != 0) {
+        ASCQ_CUDA_CHECK(cudaMemcpyToSymbolAsync(g_low_rank_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st));
+        return fail(ASCQ_ERR_TIMEOUT, "a bounded wait inside the low-rank adapter kernels expired (status %d)", v);
+    }
+    return ASCQ_OK;
+}
+ascq_status low_rank_set_wait_cycles(long long cycles)
+{
+    ASCQ_CUDA_CHECK(cudaMemcpyToSymbol(ptx::c_waitCycles, &cycles, sizeof(cycles)));
+    return ASCQ_OK;
+}
+}  // namespace ascq
