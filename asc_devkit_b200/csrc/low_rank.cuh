@@ -84,6 +84,23 @@ template <typename T> __device__ __forceinline__ uint32_t pack_sat(float lo, flo
     if constexpr (std::is_same<T, __half>::value) return pack_f16x2_sat(lo, hi);
     else return pack_bf16x2_sat(lo, hi);
 }
+// eight floats -> eight 16-bit values, finite overflow saturating: one test for all of them
+template <typename T> __device__ __forceinline__ uint4 pack8_sat(const float (&f)[8])
+{
+    constexpr float kMost = std::is_same<T, __half>::value ? 65504.0f : 3.3895313892515355e38f;
+    uint32_t r[4];
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        r[i] = pack2<T>(f[2 * i], f[2 * i + 1]);
+        asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(top) : "f"(top), "f"(f[2 * i]), "f"(f[2 * i + 1]));
+    }
+    if (__builtin_expect(!(top <= kMost), 0)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = pack_sat<T>(f[2 * i], f[2 * i + 1]);
+    }
+    return make_uint4(r[0], r[1], r[2], r[3]);
+}
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr)
 {
     float f;

@@ -16,8 +16,8 @@ namespace ascq {
 namespace {
 
 constexpr int kRows = kLongTile;
-constexpr int kLoaders = 128;              // threads of the four warps that copy and finish; a fifth warp issues the MMAs
-constexpr int kThreads = kLoaders + 32;
+constexpr int kLoaders = 128, kThreads = kLoaders + 32;         // inner: four warps that copy and finish; one more issues the MMAs
+constexpr int kFinishers = 256, kOuterThreads = kFinishers + 32;  // outer: eight and one
 constexpr int kAtomBytes = kRows * 128;    // 128 rows x 64 elements
 constexpr int kBlockCols = 64, kColumns = 512, kBlocks = kColumns / kBlockCols;  // outer: columns of an MMA, of a CTA
 
@@ -43,8 +43,8 @@ __device__ __forceinline__ void publish(uint64_t* bar)
 // Chunks of 64 k in flight.  A copy is announced LAG chunks after it was requested; its slot is asked for again two chunks after
 // that, so the MMAs that read it have had a chunk's time.
 template <int NB> struct Ring {
-    static constexpr int kStages = 4, kLag = 2;
     static constexpr int kABytes = NB * 8 * 128, kStageBytes = kAtomBytes + kABytes;
+    static constexpr int kStages = NB <= 8 ? 8 : 6, kLag = kStages - 2;
     static constexpr int kSumBytes = kRows * (NB * 8 + 1) * 4;
     static constexpr int kBytes = (kStages * kStageBytes > kSumBytes ? kStages * kStageBytes : kSumBytes) + 1024;  // + alignment
     static constexpr uint32_t kTmemCols = NB * 8 < 32 ? 32 : NB * 8;
@@ -220,7 +220,7 @@ template <int NB> struct Outer {
     static constexpr int kBytes = kVBytes + 3 * (kBBytes + kYBytes) + 1024;
 };
 
-template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_rank_outer_kernel(const LowRankArgs p, const LowRankScratch o)
+template <typename T, int NB> __global__ void __launch_bounds__(kOuterThreads, NB <= 8 ? 2 : 1) low_rank_outer_kernel(const LowRankArgs p, const LowRankScratch o)
 {
     using C = Outer<NB>;
     constexpr int VP = rank_pitch(NB);
@@ -232,13 +232,13 @@ template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_ra
     uint8_t *sB = sV + C::kVBytes, *sY = sB + 3 * C::kBBytes;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 3; ++i) mbar_init(&inBar[i], kLoaders);
+        for (int i = 0; i < 3; ++i) mbar_init(&inBar[i], kFinishers);
         mbar_init(&outBar[0], 1);
         mbar_init(&outBar[1], 1);
         fence_barrier_init();
         abortFlag = 0;
     }
-    if (warp == 4) {
+    if (warp == 8) {
         tmem_alloc(&tmemSlot, 2 * kBlockCols);
         tmem_relinquish();
     }
@@ -255,58 +255,63 @@ template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_ra
     if (adapter == p.L) {
         // tokens without an adapter: base as it is
         if (p.base != p.dst)
-            for (int row = warp; row < tokens; row += 5) {
+            for (int row = warp; row < tokens; row += 9) {
                 const int64_t t = p.order[start + row];
                 for (int col = col0 + lane * 8; col < colEnd; col += 256) {
                     const uint4 v = p.base ? *reinterpret_cast<const uint4*>(static_cast<const T*>(p.base) + t * p.ldBase + col) : make_uint4(0u, 0u, 0u, 0u);
                     *reinterpret_cast<uint4*>(static_cast<T*>(p.dst) + t * p.ldDst + col) = v;
                 }
             }
-    } else if (has && warp < 4) {
-        const int piece = threadIdx.x & 7, row0 = threadIdx.x >> 3;
-        // V, 16 rows at a time
+    } else if (has && warp < 8) {
+        {   // V: row (t / 8) + 32 i, piece t % 8
+            const int piece = threadIdx.x & 7, row0 = threadIdx.x >> 3;
+            const uint32_t at = smem_u32(sV) + row0 * 128 + ((piece ^ (row0 & 7)) << 4);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int row = row0 + 16 * i;
-            if (row < tokens) {
-                const T* v = static_cast<const T*>(o.v) + static_cast<size_t>(start + row) * 2 * VP + piece * 8;
+            for (int i = 0; i < 4; ++i)
+                if (row0 + 32 * i < tokens && (VP >= 64 || piece < 4)) {
+                    const T* v = static_cast<const T*>(o.v) + static_cast<size_t>(start + row0 + 32 * i) * 2 * VP + piece * 8;
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                    for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int ka = 0; ka < C::kAtoms; ++ka)
-                        if (VP >= 64 || piece < 4)
-                            cp_async16(smem_u32(sV) + (h * C::kAtoms + ka) * kAtomBytes + row * 128 + ((piece ^ (row & 7)) << 4), v + h * VP + ka * 64, true);
-            }
+                        for (int ka = 0; ka < C::kAtoms; ++ka) cp_async16(at + (h * C::kAtoms + ka) * kAtomBytes + i * 4096, v + h * VP + ka * 64, true);
+                }
         }
-        // the lanes' tokens: lane l of the warp holds row 32 w + l, and moves piece l % 8 of the rows l / 8 + 4 i
-        const int myRow = warp * 32 + lane;
-        const bool mine = myRow < tokens;
-        const int token = mine ? p.order[start + myRow] : -1;
-        const float unit = mine ? o.unit[start + myRow] : 0.f;
-        const T* bRow = static_cast<const T*>(p.b) + (static_cast<size_t>(adapter) * p.N + row0) * p.r + piece * 8;
+        // B: row (t / 8) + 32 i of a block, piece t % 8
+        const int bPiece = threadIdx.x & 7, bRow0 = threadIdx.x >> 3;
+        const uint32_t bAt = smem_u32(sB) + bRow0 * 128 + ((bPiece ^ (bRow0 & 7)) << 4);
+        const T* b0 = static_cast<const T*>(p.b) + (static_cast<size_t>(adapter) * p.N + col0 + bRow0) * p.r + bPiece * 8;
+        // A warp owns 32 rows (its quarter of tensor memory) and 32 of a block's 64 columns.  It moves base and dst in 16-byte pieces, four lanes a
+        // row; neighbouring quads take rows that differ in bit 2, so that eight lanes meet all banks of the swizzled layout.
+        const int quarter = warp & 3, half = warp >> 2, quad = lane >> 2;
+        const int moveRow = quarter * 32 + ((quad & 1) << 2 | quad >> 1), movePiece = half * 4 + (lane & 3);
+        const uint32_t moveAt = moveRow * 128 + ((movePiece ^ (moveRow & 7)) << 4);
+        const T* from[4];
+        T* to[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = moveRow + 8 * i;
+            const int64_t t = row < tokens ? p.order[start + row] : -1;
+            from[i] = t >= 0 && p.base ? static_cast<const T*>(p.base) + t * p.ldBase + col0 + movePiece * 8 : nullptr;
+            to[i] = t >= 0 ? static_cast<T*>(p.dst) + t * p.ldDst + col0 + movePiece * 8 : nullptr;
+        }
+        const int myRow = quarter * 32 + lane;
+        const float unit = myRow < tokens ? o.unit[start + myRow] : 0.f;
+        const int bCols = p.N - col0 - bRow0, moveCols = colEnd - col0 - movePiece * 8;  // a piece is inside while its block's column is below
         auto request = [&](int b) {
             if (b < blocks) {
-                const int n0 = col0 + b * kBlockCols, s = b % 3;
+                const int c0 = b * kBlockCols, s = b % 3;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int n = row0 + 16 * i;
+                for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int ka = 0; ka < C::kAtoms; ++ka) {
-                        const bool in = n0 + n < p.N && ka * 64 + piece * 8 < p.r;
-                        cp_async16(smem_u32(sB) + s * C::kBBytes + ka * kBlockCols * 128 + n * 128 + ((piece ^ (n & 7)) << 4),
-                                   in ? bRow + static_cast<size_t>(n0 + 16 * i) * p.r + ka * 64 : p.b, in);
+                        const bool in = c0 + 32 * i < bCols && ka * 64 + bPiece * 8 < p.r;
+                        cp_async16(bAt + s * C::kBBytes + ka * kBlockCols * 128 + i * 4096, in ? b0 + static_cast<size_t>(c0 + 32 * i) * p.r + ka * 64 : p.b, in);
                     }
-                }
-                if (p.base) {
-                    const int col = n0 + piece * 8;
-                    const uint32_t y = smem_u32(sY) + s * C::kYBytes + warp * 32 * 128;
+                if (c0 < moveCols) {
+                    const uint32_t y = smem_u32(sY) + s * C::kYBytes + moveAt;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int r = i * 4 + (lane >> 3);
-                        const int t = __shfl_sync(0xFFFFFFFFu, token, r);
-                        if (t >= 0 && col < colEnd)
-                            cp_async16(y + r * 128 + ((piece ^ (r & 7)) << 4), static_cast<const T*>(p.base) + static_cast<int64_t>(t) * p.ldBase + col, true);
-                    }
+                    for (int i = 0; i < 4; ++i)
+                        if (from[i]) cp_async16(y + i * 1024, from[i] + c0, true);
                 }
             }
             cp_commit();
@@ -320,41 +325,33 @@ template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_ra
             request(b + 2);
             cp_wait<1>();
             if (b + 1 < blocks) publish(&inBar[(b + 1) % 3]);
-            __syncwarp();  // base's values of block b, copied by the warp's lanes, are there for all of them
             if (!(ok = mbar_wait_bounded(&outBar[b & 1], (b >> 1) & 1, &abortFlag))) break;
-            __syncwarp();
+            __syncwarp();  // base's values of block b, copied by the warp's lanes, are there for all of them
             tc_fence_after();
-            uint8_t* y = sY + (b % 3) * C::kYBytes + myRow * 128;
+            uint32_t acc[32];
+            tmem_ld_32x32b_x32(tmemSlot + (static_cast<uint32_t>(quarter * 32) << 16) + (b & 1) * kBlockCols + half * 32, acc);
+            uint8_t* y = sY + (b % 3) * C::kYBytes;
+            tmem_ld_wait();
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                uint32_t acc[32];
-                tmem_ld_32x32b_x32(tmemSlot + (static_cast<uint32_t>(warp * 32) << 16) + (b & 1) * kBlockCols + half * 32, acc);
-                tmem_ld_wait();
+            for (int j = 0; j < 4; ++j) {
+                uint4* at = reinterpret_cast<uint4*>(y + myRow * 128 + (((half * 4 + j) ^ (lane & 7)) << 4));
+                const uint4 was = p.base ? *at : make_uint4(0u, 0u, 0u, 0u);
+                const uint32_t w[4] = {was.x, was.y, was.z, was.w};
+                float f[8];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    uint4* at = reinterpret_cast<uint4*>(y + (((half * 4 + j) ^ (myRow & 7)) << 4));
-                    const uint4 was = p.base ? *at : make_uint4(0u, 0u, 0u, 0u);
-                    const uint32_t w[4] = {was.x, was.y, was.z, was.w};
-                    uint32_t r[4];
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const float2 f = unpack2<T>(w[q]);
-                        r[q] = pack_sat<T>(fmaf(__uint_as_float(acc[j * 8 + 2 * q]), unit, f.x), fmaf(__uint_as_float(acc[j * 8 + 2 * q + 1]), unit, f.y));
-                    }
-                    *at = make_uint4(r[0], r[1], r[2], r[3]);
+                for (int q = 0; q < 4; ++q) {
+                    const float2 v = unpack2<T>(w[q]);
+                    f[2 * q] = fmaf(__uint_as_float(acc[j * 8 + 2 * q]), unit, v.x);
+                    f[2 * q + 1] = fmaf(__uint_as_float(acc[j * 8 + 2 * q + 1]), unit, v.y);
                 }
+                *at = pack8_sat<T>(f);
             }
             tc_fence_before();  // the next arrival on inBar lets the MMAs overwrite this accumulator
             __syncwarp();
-            const int col = col0 + b * kBlockCols + piece * 8;
-            const uint8_t* out = sY + (b % 3) * C::kYBytes + warp * 32 * 128;
+            if (b * kBlockCols < moveCols) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int r = i * 4 + (lane >> 3);
-                const int t = __shfl_sync(0xFFFFFFFFu, token, r);
-                if (t >= 0 && col < colEnd)
-                    __stcs(reinterpret_cast<uint4*>(static_cast<T*>(p.dst) + static_cast<int64_t>(t) * p.ldDst + col),
-                           *reinterpret_cast<const uint4*>(out + r * 128 + ((piece ^ (r & 7)) << 4)));
+                for (int i = 0; i < 4; ++i)
+                    if (to[i]) __stcs(reinterpret_cast<uint4*>(to[i] + b * kBlockCols), *reinterpret_cast<const uint4*>(y + moveAt + i * 1024));
             }
         }
         cp_wait<0>();
@@ -375,7 +372,7 @@ template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_ra
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (warp == 4) {
+    if (warp == 8) {
         tc_fence_after();
         tmem_dealloc(tmemSlot, 2 * kBlockCols);
     }
@@ -410,11 +407,12 @@ template <typename T, int NB> ascq_status launch_long(const LowRankArgs& p, cons
         ASCQ_CUDA_CHECK(cudaFuncSetAttribute(low_rank_outer_kernel<T, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, Outer<NB>::kBytes));
         once.mark(dev);
     }
-    // K is split until there are about two CTAs per SM; a CTA keeps at least four chunks of 64
+    // K is split until there is about one CTA per SM (the ring takes most of the shared memory; the bound on the tiles is rarely
+    // reached); a CTA keeps at least four chunks of 64
     int cluster = 8;
-    while (cluster > 1 && (static_cast<uint64_t>(tiles) * cluster > 2ull * sm_count() || p.K < cluster * 256)) cluster /= 2;
+    while (cluster > 1 && (static_cast<uint64_t>(tiles) * cluster > (9ull * sm_count()) / 8 || p.K < cluster * 256)) cluster /= 2;
     ASCQ_CUDA_CHECK(launch_pdl(low_rank_inner_kernel<T, NB>, dim3(tiles * cluster), kThreads, Ring<NB>::kBytes, cluster, st, p, o, cluster));
-    ASCQ_CUDA_CHECK(launch_pdl(low_rank_outer_kernel<T, NB>, dim3((p.N + kColumns - 1) / kColumns, tiles), kThreads, Outer<NB>::kBytes, 1, st, p, o));
+    ASCQ_CUDA_CHECK(launch_pdl(low_rank_outer_kernel<T, NB>, dim3((p.N + kColumns - 1) / kColumns, tiles), kOuterThreads, Outer<NB>::kBytes, 1, st, p, o));
     return ASCQ_OK;
 }
 template <typename T> ascq_status launch_long_typed(const LowRankArgs& p, const LowRankScratch& o, unsigned tiles, cudaStream_t st)
