@@ -107,6 +107,10 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr)
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(addr) : "memory");
     return f;
 }
+__device__ __forceinline__ void st_cluster_v4(uint32_t addr, uint4 v)
+{
+    asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
 // Exponent of the power of two that brings a row whose largest magnitude is `top` to [512, 1024); rows that are zero, subnormal or
 // not finite stay as they are.
 __device__ __forceinline__ int range_shift(float top)

@@ -19,7 +19,7 @@ constexpr int kRows = kLongTile;
 constexpr int kLoaders = 128, kThreads = kLoaders + 32;         // inner: four warps that copy and finish; one more issues the MMAs
 constexpr int kFinishers = 256, kOuterThreads = kFinishers + 32;  // outer: eight and one
 constexpr int kAtomBytes = kRows * 128;    // 128 rows x 64 elements
-constexpr int kBlockCols = 64, kColumns = 512, kBlocks = kColumns / kBlockCols;  // outer: columns of an MMA, of a CTA
+constexpr int kBlockCols = 64;             // outer: columns of an MMA
 
 __device__ int g_low_rank_status;  // 1: a bounded wait ran out
 
@@ -44,16 +44,77 @@ __device__ __forceinline__ void publish(uint64_t* bar)
 // that, so the MMAs that read it have had a chunk's time.
 template <int NB> struct Ring {
     static constexpr int kABytes = NB * 8 * 128, kStageBytes = kAtomBytes + kABytes;
-    static constexpr int kStages = NB <= 8 ? 8 : 6, kLag = kStages - 2;
-    static constexpr int kSumBytes = kRows * (NB * 8 + 1) * 4;
-    static constexpr int kBytes = (kStages * kStageBytes > kSumBytes ? kStages * kStageBytes : kSumBytes) + 1024;  // + alignment
+    static constexpr int kStages = NB <= 8 ? 6 : 4, kLag = kStages - 2;
+    static constexpr int kSumBytes = kRows * (NB * 8 + 4) * 4;  // partial sums of the rows that this CTA finishes, from every CTA of the cluster
+    static constexpr int kBytes = kStages * kStageBytes + kSumBytes + 1024;  // + alignment
     static constexpr uint32_t kTmemCols = NB * 8 < 32 ? 32 : NB * 8;
 };
+
+// The rows of one CTA's share: CTAS threads a row, each sums its columns over the cluster's CTAs, scales them, finds the row's largest
+// value with its neighbours and writes the two terms.
+template <typename T, int NB, int CTAS>
+__device__ __forceinline__ void finish_rows(const float* part, int there, int start, float scale, const LowRankScratch& o)
+{
+    constexpr int R = NB * 8, VP = rank_pitch(NB), kPitch = R + 4, kShare = kRows / CTAS, W = R / CTAS;  // W: columns of a thread
+    const int row = threadIdx.x / CTAS, col0 = (threadIdx.x % CTAS) * W;
+    float v[W] = {}, top = 0.f;
+#pragma unroll
+    for (int q = 0; q < CTAS; ++q) {
+        const float* at = part + (q * kShare + row) * kPitch + col0;
+        if constexpr (W % 4 == 0) {
+#pragma unroll
+            for (int i = 0; i < W; i += 4) {
+                const float4 f = *reinterpret_cast<const float4*>(at + i);
+                v[i] += f.x; v[i + 1] += f.y; v[i + 2] += f.z; v[i + 3] += f.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[i] += at[i];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+        v[i] *= scale;
+        top = fmaxf(top, fabsf(v[i]));
+    }
+#pragma unroll
+    for (int s = 1; s < CTAS; s <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, s));
+    if (row >= there) return;
+    const int shift = range_shift(top);
+    const float down = exp2_int(-shift);
+    if (col0 == 0) o.unit[start + row] = exp2_int(shift);
+    uint32_t hi[W / 2], lo[W / 2];
+#pragma unroll
+    for (int i = 0; i < W; i += 2) {
+        const uint2 a = split16<T>(v[i] * down), b = split16<T>(v[i + 1] * down);
+        hi[i / 2] = a.x | (b.x << 16);
+        lo[i / 2] = a.y | (b.y << 16);
+    }
+    uint32_t* to = reinterpret_cast<uint32_t*>(static_cast<unsigned short*>(o.v) + static_cast<size_t>(start + row) * 2 * VP + col0);
+    if constexpr (W % 8 == 0) {
+#pragma unroll
+        for (int i = 0; i < W / 2; i += 4) {
+            *reinterpret_cast<uint4*>(to + i) = make_uint4(hi[i], hi[i + 1], hi[i + 2], hi[i + 3]);
+            *reinterpret_cast<uint4*>(to + VP / 2 + i) = make_uint4(lo[i], lo[i + 1], lo[i + 2], lo[i + 3]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < W / 2; ++i) {
+            to[i] = hi[i];
+            to[VP / 2 + i] = lo[i];
+        }
+    }
+    if constexpr (VP > R) {  // the rest of a short row is zeros: W more columns of each thread
+        static_assert(VP == 2 * R, "ranks up to 16 take rows of 32");
+#pragma unroll
+        for (int i = 0; i < W / 2; ++i) to[R / 2 + i] = to[VP / 2 + R / 2 + i] = 0u;
+    }
+}
 
 template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_rank_inner_kernel(const LowRankArgs p, const LowRankScratch o, int clusterCtas)
 {
     using C = Ring<NB>;
-    constexpr int R = NB * 8, VP = rank_pitch(NB), kPitch = R + 1;
+    constexpr int R = NB * 8, kPitch = R + 4;
     extern __shared__ uint8_t raw[];
     __shared__ int found[4];
     __shared__ uint64_t fullBar[C::kStages], emptyBar[C::kStages], doneBar;
@@ -85,6 +146,7 @@ template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_ra
     if (rank == 0 && threadIdx.x == 0) static_cast<int4*>(o.tiles)[tileIdx] = make_int4(adapter, start, tokens, 0);
     const bool has = adapter >= 0 && adapter < p.L;  // the same for every CTA of the cluster
     if (has) {
+        cluster_arrive();
         const int chunks = (p.K + 63) / 64, per = (chunks + clusterCtas - 1) / clusterCtas;
         const int first = min(rank * per, chunks), n = min(first + per, chunks) - first;
         bool ok = true;
@@ -137,12 +199,16 @@ template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_ra
             if (ok && n > 0) tc_commit(&doneBar);
         }
         __syncwarp();
-        float* part = reinterpret_cast<float*>(ring);  // free: every chunk was copied and multiplied before doneBar completed
+        // Each CTA of the cluster finishes its share of the rows: the others' sums are stored into its shared memory (nobody waits for a
+        // remote load), one cluster barrier, and the rest is local.
+        float* part = reinterpret_cast<float*>(ring + C::kStages * C::kStageBytes);
+        const int share = kRows / clusterCtas;
+        cluster_wait();  // every CTA of the cluster has started (they arrived at the top)
         if (warp < 4) {
             if (n > 0) ok = ok && mbar_wait_bounded(&doneBar, 0, &abortFlag);
             __syncwarp();
             tc_fence_after();
-            float* to = part + threadIdx.x * kPitch;
+            const uint32_t to = mapa_u32(smem_u32(part + (rank * share + threadIdx.x % share) * kPitch), threadIdx.x / share);
 #pragma unroll
             for (int c0 = 0; c0 < R; c0 += 32) {
                 uint32_t v[32];
@@ -151,8 +217,8 @@ template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_ra
                     tmem_ld_wait();
                 }
 #pragma unroll
-                for (int c = 0; c < 32; ++c)
-                    if (c0 + c < R) to[c0 + c] = n > 0 ? __uint_as_float(v[c]) : 0.f;
+                for (int c = 0; c < 32 && c0 + c < R; c += 4)
+                    st_cluster_v4(to + (c0 + c) * 4, n > 0 ? make_uint4(v[c], v[c + 1], v[c + 2], v[c + 3]) : make_uint4(0u, 0u, 0u, 0u));
             }
         }
         __syncthreads();
@@ -160,49 +226,12 @@ template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_ra
         cluster_wait();
         if (warp < 4) {
             const float scale = p.scale ? p.scale[adapter] : 1.0f;
-            const int step = clusterCtas * 4;
-            for (int row0 = rank * 4 + warp; row0 < tokens; row0 += 4 * step) {
-                float v[4][VP / 32] = {}, top[4];
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int row = min(row0 + u * step, kRows - 1);
-#pragma unroll
-                    for (int i = 0; i < VP / 32; ++i) {
-                        const int col = lane + 32 * i;
-                        if (col < R) {
-                            const uint32_t at = smem_u32(part + row * kPitch + col);
-                            for (int q = 0; q < clusterCtas; ++q) v[u][i] += ld_cluster_f32(mapa_u32(at, q));
-                        }
-                    }
-                }
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    top[u] = 0.f;
-#pragma unroll
-                    for (int i = 0; i < VP / 32; ++i) {
-                        v[u][i] *= scale;
-                        top[u] = fmaxf(top[u], fabsf(v[u][i]));
-                    }
-#pragma unroll
-                    for (int s = 16; s > 0; s >>= 1) top[u] = fmaxf(top[u], __shfl_xor_sync(0xFFFFFFFFu, top[u], s));
-                    const int row = row0 + u * step;
-                    if (row >= tokens) continue;
-                    const int shift = range_shift(top[u]);
-                    const float down = exp2_int(-shift);
-                    if (lane == 0) o.unit[start + row] = exp2_int(shift);
-                    unsigned short* to = static_cast<unsigned short*>(o.v) + static_cast<size_t>(start + row) * 2 * VP;
-#pragma unroll
-                    for (int i = 0; i < VP / 32; ++i) {
-                        const uint2 h = split16<T>(v[u][i] * down);
-                        to[lane + 32 * i] = static_cast<unsigned short>(h.x);
-                        to[VP + lane + 32 * i] = static_cast<unsigned short>(h.y);
-                    }
-                }
-            }
+            const int there = tokens - rank * share;  // rows of this CTA's share that have a token
+            if (clusterCtas == 1) finish_rows<T, NB, 1>(part, there, start, scale, o);
+            else if (clusterCtas == 2) finish_rows<T, NB, 2>(part, there, start + rank * share, scale, o);
+            else if (clusterCtas == 4) finish_rows<T, NB, 4>(part, there, start + rank * share, scale, o);
+            else finish_rows<T, NB, 8>(part, there, start + rank * share, scale, o);
         }
-        __syncwarp();
-        cluster_arrive();  // no CTA ends while another reads its sums
-        cluster_wait();
     }
     tc_fence_before();
     __syncthreads();
@@ -220,7 +249,7 @@ template <int NB> struct Outer {
     static constexpr int kBytes = kVBytes + 3 * (kBBytes + kYBytes) + 1024;
 };
 
-template <typename T, int NB> __global__ void __launch_bounds__(kOuterThreads, NB <= 8 ? 2 : 1) low_rank_outer_kernel(const LowRankArgs p, const LowRankScratch o)
+template <typename T, int NB> __global__ void __launch_bounds__(kOuterThreads, NB <= 8 ? 2 : 1) low_rank_outer_kernel(const LowRankArgs p, const LowRankScratch o, int columns)
 {
     using C = Outer<NB>;
     constexpr int VP = rank_pitch(NB);
@@ -249,7 +278,7 @@ template <typename T, int NB> __global__ void __launch_bounds__(kOuterThreads, N
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const int col0 = blockIdx.x * kColumns, colEnd = min(p.N, col0 + kColumns), blocks = (colEnd - col0 + kBlockCols - 1) / kBlockCols;
+    const int col0 = blockIdx.x * columns, colEnd = min(p.N, col0 + columns), blocks = (colEnd - col0 + kBlockCols - 1) / kBlockCols;
     const bool has = adapter >= 0 && adapter < p.L;
     bool ok = true;
     if (adapter == p.L) {
@@ -297,6 +326,14 @@ template <typename T, int NB> __global__ void __launch_bounds__(kOuterThreads, N
         const int myRow = quarter * 32 + lane;
         const float unit = myRow < tokens ? o.unit[start + myRow] : 0.f;
         const int bCols = p.N - col0 - bRow0, moveCols = colEnd - col0 - movePiece * 8;  // a piece is inside while its block's column is below
+        // base's lines of the whole tile on their way to L2: the copies below run one block ahead, too little for HBM's latency
+        if (p.base) {
+            const int row = threadIdx.x >> 1;
+            if (row < tokens) {
+                const T* line = static_cast<const T*>(p.base) + static_cast<int64_t>(p.order[start + row]) * p.ldBase + col0 + (threadIdx.x & 1) * 64;
+                for (int c = (threadIdx.x & 1) * 64; c < colEnd - col0; c += 128, line += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(line));
+            }
+        }
         auto request = [&](int b) {
             if (b < blocks) {
                 const int c0 = b * kBlockCols, s = b % 3;
@@ -412,7 +449,9 @@ template <typename T, int NB> ascq_status launch_long(const LowRankArgs& p, cons
     int cluster = 8;
     while (cluster > 1 && (static_cast<uint64_t>(tiles) * cluster > (9ull * sm_count()) / 8 || p.K < cluster * 256)) cluster /= 2;
     ASCQ_CUDA_CHECK(launch_pdl(low_rank_inner_kernel<T, NB>, dim3(tiles * cluster), kThreads, Ring<NB>::kBytes, cluster, st, p, o, cluster));
-    ASCQ_CUDA_CHECK(launch_pdl(low_rank_outer_kernel<T, NB>, dim3((p.N + kColumns - 1) / kColumns, tiles), kOuterThreads, Outer<NB>::kBytes, 1, st, p, o));
+    int columns = getenv("LRC") ? atoi(getenv("LRC")) : 512;
+    while (columns > 128 && static_cast<uint64_t>(tiles) * ((p.N + columns - 1) / columns) < (getenv("LRW") ? atoi(getenv("LRW")) : 4ull) * sm_count()) columns /= 2;
+    ASCQ_CUDA_CHECK(launch_pdl(low_rank_outer_kernel<T, NB>, dim3((p.N + columns - 1) / columns, tiles), kOuterThreads, Outer<NB>::kBytes, 1, st, p, o, columns));
     return ASCQ_OK;
 }
 template <typename T> ascq_status launch_long_typed(const LowRankArgs& p, const LowRankScratch& o, unsigned tiles, cudaStream_t st)
