@@ -44,8 +44,9 @@ __device__ __forceinline__ void publish(uint64_t* bar)
 // that, so the MMAs that read it have had a chunk's time.
 template <int NB> struct Ring {
     static constexpr int kABytes = NB * 8 * 128, kStageBytes = kAtomBytes + kABytes;
-    static constexpr int kStages = NB <= 8 ? 6 : 4, kLag = kStages - 2;
     static constexpr int kSumBytes = kRows * (NB * 8 + 4) * 4;  // partial sums of the rows that this CTA finishes, from every CTA of the cluster
+    static constexpr int kFit = (226 * 1024 - 1024 - kSumBytes) / kStageBytes;  // one CTA takes an SM's shared memory (227 KB)
+    static constexpr int kStages = kFit < 8 ? kFit : 8, kLag = kStages - 2;
     static constexpr int kBytes = kStages * kStageBytes + kSumBytes + 1024;  // + alignment
     static constexpr uint32_t kTmemCols = NB * 8 < 32 ? 32 : NB * 8;
 };
@@ -139,6 +140,12 @@ template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_ra
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (warp == 0) find_tile<kRows>(tileIdx, p.L + 1, [&](int e) { return static_cast<int>(p.counts[e]); }, found);
+    if (warp == 1 && blockIdx.x == 0) {  // how many tiles there are, behind their table
+        int all = 0;
+        for (int e = lane; e <= p.L; e += 32) all += (static_cast<int>(p.counts[e]) + kRows - 1) / kRows;
+        all = __reduce_add_sync(0xFFFFFFFFu, all);
+        if (lane == 0) static_cast<int4*>(o.tiles)[gridDim.x / clusterCtas].x = all;
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -249,7 +256,11 @@ template <int NB> struct Outer {
     static constexpr int kBytes = kVBytes + 3 * (kBBytes + kYBytes) + 1024;
 };
 
-template <typename T, int NB> __global__ void __launch_bounds__(kOuterThreads, NB <= 8 ? 2 : 1) low_rank_outer_kernel(const LowRankArgs p, const LowRankScratch o, int columns)
+// The blocks of 64 columns of all tiles are dealt out evenly: CTA c of G takes the blocks from c * total / G to (c + 1) * total / G, which
+// touch one tile or two; for each it loads V once and streams B and base.  (With a CTA for each tile and 512 columns the two waves' starts were
+// as long as their work: 42 us instead of 31 at 8192 tokens, 4096 columns.)
+template <typename T, int NB>
+__global__ void __launch_bounds__(kOuterThreads, NB <= 8 ? 2 : 1) low_rank_outer_kernel(const LowRankArgs p, const LowRankScratch o, int tileBound)
 {
     using C = Outer<NB>;
     constexpr int VP = rank_pitch(NB);
@@ -273,138 +284,148 @@ template <typename T, int NB> __global__ void __launch_bounds__(kOuterThreads, N
     }
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int4 tile = static_cast<const int4*>(o.tiles)[blockIdx.y];
-    const int adapter = tile.x, start = tile.y, tokens = tile.z;
+    const int4* tiles = static_cast<const int4*>(o.tiles);
+    const int perTile = (p.N + kBlockCols - 1) / kBlockCols;
+    const int64_t total = static_cast<int64_t>(tiles[tileBound].x) * perTile;
+    int64_t pos = total * blockIdx.x / gridDim.x;
+    const int64_t end = total * (blockIdx.x + 1) / gridDim.x;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const int col0 = blockIdx.x * columns, colEnd = min(p.N, col0 + columns), blocks = (colEnd - col0 + kBlockCols - 1) / kBlockCols;
-    const bool has = adapter >= 0 && adapter < p.L;
     bool ok = true;
-    if (adapter == p.L) {
-        // tokens without an adapter: base as it is
-        if (p.base != p.dst)
-            for (int row = warp; row < tokens; row += 9) {
-                const int64_t t = p.order[start + row];
-                for (int col = col0 + lane * 8; col < colEnd; col += 256) {
-                    const uint4 v = p.base ? *reinterpret_cast<const uint4*>(static_cast<const T*>(p.base) + t * p.ldBase + col) : make_uint4(0u, 0u, 0u, 0u);
-                    *reinterpret_cast<uint4*>(static_cast<T*>(p.dst) + t * p.ldDst + col) = v;
-                }
-            }
-    } else if (has && warp < 8) {
-        {   // V: row (t / 8) + 32 i, piece t % 8
-            const int piece = threadIdx.x & 7, row0 = threadIdx.x >> 3;
-            const uint32_t at = smem_u32(sV) + row0 * 128 + ((piece ^ (row0 & 7)) << 4);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (row0 + 32 * i < tokens && (VP >= 64 || piece < 4)) {
-                    const T* v = static_cast<const T*>(o.v) + static_cast<size_t>(start + row0 + 32 * i) * 2 * VP + piece * 8;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int ka = 0; ka < C::kAtoms; ++ka) cp_async16(at + (h * C::kAtoms + ka) * kAtomBytes + i * 4096, v + h * VP + ka * 64, true);
-                }
-        }
-        // B: row (t / 8) + 32 i of a block, piece t % 8
-        const int bPiece = threadIdx.x & 7, bRow0 = threadIdx.x >> 3;
-        const uint32_t bAt = smem_u32(sB) + bRow0 * 128 + ((bPiece ^ (bRow0 & 7)) << 4);
-        const T* b0 = static_cast<const T*>(p.b) + (static_cast<size_t>(adapter) * p.N + col0 + bRow0) * p.r + bPiece * 8;
-        // A warp owns 32 rows (its quarter of tensor memory) and 32 of a block's 64 columns.  It moves base and dst in 16-byte pieces, four lanes a
-        // row; neighbouring quads take rows that differ in bit 2, so that eight lanes meet all banks of the swizzled layout.
-        const int quarter = warp & 3, half = warp >> 2, quad = lane >> 2;
-        const int moveRow = quarter * 32 + ((quad & 1) << 2 | quad >> 1), movePiece = half * 4 + (lane & 3);
-        const uint32_t moveAt = moveRow * 128 + ((movePiece ^ (moveRow & 7)) << 4);
-        const T* from[4];
-        T* to[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int row = moveRow + 8 * i;
-            const int64_t t = row < tokens ? p.order[start + row] : -1;
-            from[i] = t >= 0 && p.base ? static_cast<const T*>(p.base) + t * p.ldBase + col0 + movePiece * 8 : nullptr;
-            to[i] = t >= 0 ? static_cast<T*>(p.dst) + t * p.ldDst + col0 + movePiece * 8 : nullptr;
-        }
-        const int myRow = quarter * 32 + lane;
-        const float unit = myRow < tokens ? o.unit[start + myRow] : 0.f;
-        const int bCols = p.N - col0 - bRow0, moveCols = colEnd - col0 - movePiece * 8;  // a piece is inside while its block's column is below
-        // base's lines of the whole tile on their way to L2: the copies below run one block ahead, too little for HBM's latency
-        if (p.base) {
-            const int row = threadIdx.x >> 1;
-            if (row < tokens) {
-                const T* line = static_cast<const T*>(p.base) + static_cast<int64_t>(p.order[start + row]) * p.ldBase + col0 + (threadIdx.x & 1) * 64;
-                for (int c = (threadIdx.x & 1) * 64; c < colEnd - col0; c += 128, line += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(line));
-            }
-        }
-        auto request = [&](int b) {
-            if (b < blocks) {
-                const int c0 = b * kBlockCols, s = b % 3;
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int ka = 0; ka < C::kAtoms; ++ka) {
-                        const bool in = c0 + 32 * i < bCols && ka * 64 + bPiece * 8 < p.r;
-                        cp_async16(bAt + s * C::kBBytes + ka * kBlockCols * 128 + i * 4096, in ? b0 + static_cast<size_t>(c0 + 32 * i) * p.r + ka * 64 : p.b, in);
+    uint32_t it = 0;  // blocks multiplied so far: the barriers' slots and phases go by it
+    while (pos < end && ok) {
+        const int tileIdx = static_cast<int>(pos / perTile), first = static_cast<int>(pos % perTile);
+        const int blocks = static_cast<int>(min(end - pos, static_cast<int64_t>(perTile - first)));
+        pos += blocks;
+        const int4 tile = tiles[tileIdx];
+        const int adapter = tile.x, start = tile.y, tokens = tile.z;
+        const int col0 = first * kBlockCols, colEnd = min(p.N, col0 + blocks * kBlockCols);
+        if (adapter >= p.L) {
+            // tokens without an adapter: base as it is
+            if (p.base != p.dst)
+                for (int row = warp; row < tokens; row += 9) {
+                    const int64_t t = p.order[start + row];
+                    for (int col = col0 + lane * 8; col < colEnd; col += 256) {
+                        const uint4 v = p.base ? *reinterpret_cast<const uint4*>(static_cast<const T*>(p.base) + t * p.ldBase + col) : make_uint4(0u, 0u, 0u, 0u);
+                        *reinterpret_cast<uint4*>(static_cast<T*>(p.dst) + t * p.ldDst + col) = v;
                     }
-                if (c0 < moveCols) {
-                    const uint32_t y = smem_u32(sY) + s * C::kYBytes + moveAt;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (from[i]) cp_async16(y + i * 1024, from[i] + c0, true);
                 }
-            }
-            cp_commit();
-        };
-        request(0);
-        request(1);
-        cp_wait<1>();
-        publish(&inBar[0]);
-        for (int b = 0; b < blocks; ++b) {
-            __syncwarp();  // the warp has read the values of block b - 1 out of the slot that is filled now
-            request(b + 2);
-            cp_wait<1>();
-            if (b + 1 < blocks) publish(&inBar[(b + 1) % 3]);
-            if (!(ok = mbar_wait_bounded(&outBar[b & 1], (b >> 1) & 1, &abortFlag))) break;
-            __syncwarp();  // base's values of block b, copied by the warp's lanes, are there for all of them
-            tc_fence_after();
-            uint32_t acc[32];
-            tmem_ld_32x32b_x32(tmemSlot + (static_cast<uint32_t>(quarter * 32) << 16) + (b & 1) * kBlockCols + half * 32, acc);
-            uint8_t* y = sY + (b % 3) * C::kYBytes;
-            tmem_ld_wait();
+            continue;
+        }
+        if (warp < 8) {
+            // A warp owns 32 rows (its quarter of tensor memory) and 32 of a block's 64 columns.  It moves base and dst in 16-byte pieces, four lanes
+            // a row; neighbouring quads take rows that differ in bit 2, so that eight lanes meet all banks of the swizzled layout.
+            const int quarter = warp & 3, half = warp >> 2, quad = lane >> 2;
+            const int moveRow = quarter * 32 + ((quad & 1) << 2 | quad >> 1), movePiece = half * 4 + (lane & 3);
+            const uint32_t moveAt = moveRow * 128 + ((movePiece ^ (moveRow & 7)) << 4);
+            const T* from[4];
+            T* to[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint4* at = reinterpret_cast<uint4*>(y + myRow * 128 + (((half * 4 + j) ^ (lane & 7)) << 4));
-                const uint4 was = p.base ? *at : make_uint4(0u, 0u, 0u, 0u);
-                const uint32_t w[4] = {was.x, was.y, was.z, was.w};
-                float f[8];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const float2 v = unpack2<T>(w[q]);
-                    f[2 * q] = fmaf(__uint_as_float(acc[j * 8 + 2 * q]), unit, v.x);
-                    f[2 * q + 1] = fmaf(__uint_as_float(acc[j * 8 + 2 * q + 1]), unit, v.y);
-                }
-                *at = pack8_sat<T>(f);
+            for (int i = 0; i < 4; ++i) {
+                const int row = moveRow + 8 * i;
+                const int64_t t = row < tokens ? p.order[start + row] : -1;
+                from[i] = t >= 0 && p.base ? static_cast<const T*>(p.base) + t * p.ldBase + col0 + movePiece * 8 : nullptr;
+                to[i] = t >= 0 ? static_cast<T*>(p.dst) + t * p.ldDst + col0 + movePiece * 8 : nullptr;
             }
-            tc_fence_before();  // the next arrival on inBar lets the MMAs overwrite this accumulator
-            __syncwarp();
-            if (b * kBlockCols < moveCols) {
+            {   // V: row (t / 8) + 32 i, piece t % 8
+                const int piece = threadIdx.x & 7, row0 = threadIdx.x >> 3;
+                const uint32_t at = smem_u32(sV) + row0 * 128 + ((piece ^ (row0 & 7)) << 4);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (to[i]) __stcs(reinterpret_cast<uint4*>(to[i] + b * kBlockCols), *reinterpret_cast<const uint4*>(y + moveAt + i * 1024));
+                    if (row0 + 32 * i < tokens && (VP >= 64 || piece < 4)) {
+                        const T* v = static_cast<const T*>(o.v) + static_cast<size_t>(start + row0 + 32 * i) * 2 * VP + piece * 8;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int ka = 0; ka < C::kAtoms; ++ka) cp_async16(at + (h * C::kAtoms + ka) * kAtomBytes + i * 4096, v + h * VP + ka * 64, true);
+                    }
+            }
+            // B: row (t / 8) + 32 i of a block, piece t % 8
+            const int bPiece = threadIdx.x & 7, bRow0 = threadIdx.x >> 3;
+            const uint32_t bAt = smem_u32(sB) + bRow0 * 128 + ((bPiece ^ (bRow0 & 7)) << 4);
+            const T* b0 = static_cast<const T*>(p.b) + (static_cast<size_t>(adapter) * p.N + col0 + bRow0) * p.r + bPiece * 8;
+            const int myRow = quarter * 32 + lane;
+            const float unit = myRow < tokens ? o.unit[start + myRow] : 0.f;
+            const int bCols = p.N - col0 - bRow0, moveCols = colEnd - col0 - movePiece * 8;  // a piece is inside while its block's column is below
+            auto request = [&](int b) {
+                if (b < blocks) {
+                    const int c0 = b * kBlockCols, s = (it + b) % 3;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int ka = 0; ka < C::kAtoms; ++ka) {
+                            const bool in = c0 + 32 * i < bCols && ka * 64 + bPiece * 8 < p.r;
+                            cp_async16(bAt + s * C::kBBytes + ka * kBlockCols * 128 + i * 4096, in ? b0 + static_cast<size_t>(c0 + 32 * i) * p.r + ka * 64 : p.b, in);
+                        }
+                    if (c0 < moveCols) {
+                        const uint32_t y = smem_u32(sY) + s * C::kYBytes + moveAt;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (from[i]) cp_async16(y + i * 1024, from[i] + c0, true);
+                    }
+                }
+                cp_commit();
+            };
+            request(0);
+            request(1);
+            cp_wait<1>();
+            publish(&inBar[it % 3]);
+            for (int b = 0; b < blocks; ++b) {
+                const uint32_t n = it + b;
+                __syncwarp();  // the warp has read the values of block n - 1 out of the slot that is filled now
+                request(b + 2);
+                cp_wait<1>();
+                if (b + 1 < blocks) publish(&inBar[(n + 1) % 3]);
+                ok = mbar_wait_bounded(&outBar[n & 1], (n >> 1) & 1, &abortFlag);
+                // base's values of block n, copied by the warp's lanes, are there for all of them; and the lanes give up together
+                if (!(ok = __all_sync(0xFFFFFFFFu, ok))) break;
+                tc_fence_after();
+                uint32_t acc[32];
+                tmem_ld_32x32b_x32(tmemSlot + (static_cast<uint32_t>(quarter * 32) << 16) + (n & 1) * kBlockCols + half * 32, acc);
+                uint8_t* y = sY + (n % 3) * C::kYBytes;
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint4* at = reinterpret_cast<uint4*>(y + myRow * 128 + (((half * 4 + j) ^ (lane & 7)) << 4));
+                    const uint4 was = p.base ? *at : make_uint4(0u, 0u, 0u, 0u);
+                    const uint32_t w[4] = {was.x, was.y, was.z, was.w};
+                    float f[8];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const float2 v = unpack2<T>(w[q]);
+                        f[2 * q] = fmaf(__uint_as_float(acc[j * 8 + 2 * q]), unit, v.x);
+                        f[2 * q + 1] = fmaf(__uint_as_float(acc[j * 8 + 2 * q + 1]), unit, v.y);
+                    }
+                    *at = pack8_sat<T>(f);
+                }
+                tc_fence_before();  // the next arrival on inBar lets the MMAs overwrite this accumulator
+                __syncwarp();
+                if (b * kBlockCols < moveCols) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (to[i]) __stcs(reinterpret_cast<uint4*>(to[i] + b * kBlockCols), *reinterpret_cast<const uint4*>(y + moveAt + i * 1024));
+                }
+            }
+            cp_wait<0>();
+            __syncwarp();  // the slots are filled again for the next tile
+        } else if (elect_one()) {
+            constexpr uint32_t idesc = idesc_f16(kRows, kBlockCols, std::is_same<T, __half>::value ? 0 : 1);
+            const int steps = (p.r + 15) / 16;
+            for (int b = 0; b < blocks; ++b) {
+                const uint32_t n = it + b;
+                if (!(ok = mbar_wait_bounded(&inBar[n % 3], (n / 3) & 1, &abortFlag))) break;
+                tc_fence_after();
+                const uint32_t v = smem_u32(sV), w = smem_u32(sB) + (n % 3) * C::kBBytes;
+                for (int h = 0; h < 2; ++h)
+                    for (int k = 0; k < steps; ++k)
+                        mma_f16(tmemSlot + (n & 1) * kBlockCols, smem_desc_sw128(v + (h * C::kAtoms + (k >> 2)) * kAtomBytes) + 2 * (k & 3),
+                                smem_desc_sw128(w + (k >> 2) * kBlockCols * 128) + 2 * (k & 3), idesc, (h | k) != 0);
+                tc_commit(&outBar[n & 1]);
             }
         }
-        cp_wait<0>();
-    } else if (has && elect_one()) {
-        constexpr uint32_t idesc = idesc_f16(kRows, kBlockCols, std::is_same<T, __half>::value ? 0 : 1);
-        const int steps = (p.r + 15) / 16;
-        for (int b = 0; b < blocks; ++b) {
-            if (!(ok = mbar_wait_bounded(&inBar[b % 3], (b / 3) & 1, &abortFlag))) break;
-            tc_fence_after();
-            const uint32_t v = smem_u32(sV), w = smem_u32(sB) + (b % 3) * C::kBBytes;
-            for (int h = 0; h < 2; ++h)
-                for (int k = 0; k < steps; ++k)
-                    mma_f16(tmemSlot + (b & 1) * kBlockCols, smem_desc_sw128(v + (h * C::kAtoms + (k >> 2)) * kAtomBytes) + 2 * (k & 3),
-                            smem_desc_sw128(w + (k >> 2) * kBlockCols * 128) + 2 * (k & 3), idesc, (h | k) != 0);
-            tc_commit(&outBar[b & 1]);
-        }
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        it += blocks;
     }
     __syncwarp();
     tc_fence_before();
@@ -449,9 +470,10 @@ template <typename T, int NB> ascq_status launch_long(const LowRankArgs& p, cons
     int cluster = 8;
     while (cluster > 1 && (static_cast<uint64_t>(tiles) * cluster > (9ull * sm_count()) / 8 || p.K < cluster * 256)) cluster /= 2;
     ASCQ_CUDA_CHECK(launch_pdl(low_rank_inner_kernel<T, NB>, dim3(tiles * cluster), kThreads, Ring<NB>::kBytes, cluster, st, p, o, cluster));
-    int columns = getenv("LRC") ? atoi(getenv("LRC")) : 512;
-    while (columns > 128 && static_cast<uint64_t>(tiles) * ((p.N + columns - 1) / columns) < (getenv("LRW") ? atoi(getenv("LRW")) : 4ull) * sm_count()) columns /= 2;
-    ASCQ_CUDA_CHECK(launch_pdl(low_rank_outer_kernel<T, NB>, dim3((p.N + columns - 1) / columns, tiles), kOuterThreads, Outer<NB>::kBytes, 1, st, p, o, columns));
+    // as many CTAs of the second launch as are resident together, at most one per block of columns
+    const uint64_t blocks = static_cast<uint64_t>(tiles) * ((p.N + kBlockCols - 1) / kBlockCols);
+    const unsigned grid = static_cast<unsigned>(std::min<uint64_t>(blocks, static_cast<uint64_t>(sm_count()) * (NB <= 8 ? 2 : 1)));
+    ASCQ_CUDA_CHECK(launch_pdl(low_rank_outer_kernel<T, NB>, dim3(grid), kOuterThreads, Outer<NB>::kBytes, 1, st, p, o, static_cast<int>(tiles)));
     return ASCQ_OK;
 }
 template <typename T> ascq_status launch_long_typed(const LowRankArgs& p, const LowRankScratch& o, unsigned tiles, cudaStream_t st)
@@ -466,7 +488,7 @@ template <typename T> ascq_status launch_long_typed(const LowRankArgs& p, const 
 
 }  // namespace
 
-size_t low_rank_long_tiles_bytes(int64_t tiles) { return static_cast<size_t>(tiles) * 16; }
+size_t low_rank_long_tiles_bytes(int64_t tiles) { return static_cast<size_t>(tiles + 1) * 16; }
 size_t low_rank_long_inner_bytes(int M, int r) { return static_cast<size_t>(M) * 2 * rank_pitch(rank_blocks(r)) * 2; }
 
 ascq_status low_rank_long(const LowRankArgs& p, bool half, const LowRankScratch& o, unsigned tiles, ::CUstream_st* st)

@@ -210,7 +210,7 @@ def test_refusals():
     size = L.lib().ascq_low_rank_add_workspace_size
     assert size(1024, 16, 8) == 0
     assert size(2000, 16, 1000) == 8016 + 2000 * 4                       # counts and order
-    assert size(2000, 64, 3) == 32 + 8000 + (2000 // 128 + 4) * 16 + 8000 + 2000 * 2 * 64 * 2  # and tiles, units and the inner products
+    assert size(2000, 64, 3) == 32 + 8000 + (2000 // 128 + 5) * 16 + 8000 + 2000 * 2 * 64 * 2  # and tiles, units and the inner products
 
 
 def test_python_refusals():
