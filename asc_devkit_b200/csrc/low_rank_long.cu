@@ -16,7 +16,7 @@ namespace ascq {
 namespace {
 
 constexpr int kRows = kLongTile;
-constexpr int kLoaders = 128, kThreads = kLoaders + 32;         // inner: four warps that copy and finish; one more issues the MMAs
+constexpr int kLoaders = 128, kThreads = 2 * kLoaders + 32;     // inner: two groups of four warps copy, the first finishes too; one more warp issues the MMAs
 constexpr int kFinishers = 256, kOuterThreads = kFinishers + 32;  // outer: eight and one
 constexpr int kAtomBytes = kRows * 128;    // 128 rows x 64 elements
 constexpr int kBlockCols = 64;             // outer: columns of an MMA
@@ -40,13 +40,14 @@ __device__ __forceinline__ void publish(uint64_t* bar)
     mbar_arrive(bar);
 }
 
-// Chunks of 64 k in flight.  A copy is announced LAG chunks after it was requested; its slot is asked for again two chunks after
-// that, so the MMAs that read it have had a chunk's time.
+// Chunks of 64 k in flight.  The two groups of loading warps take alternate chunks: waiting for a chunk's copies, making them visible to the
+// tensor cores and announcing them takes a few hundred cycles, and the other group requests meanwhile.  A group announces a chunk
+// kLag of its own chunks after it was requested (2 kLag < kStages: the slot that it waits for next was announced before).
 template <int NB> struct Ring {
     static constexpr int kABytes = NB * 8 * 128, kStageBytes = kAtomBytes + kABytes;
     static constexpr int kSumBytes = kRows * (NB * 8 + 4) * 4;  // partial sums of the rows that this CTA finishes, from every CTA of the cluster
     static constexpr int kFit = (226 * 1024 - 1024 - kSumBytes) / kStageBytes;  // one CTA takes an SM's shared memory (227 KB)
-    static constexpr int kStages = kFit < 8 ? kFit : 8, kLag = kStages - 2;
+    static constexpr int kStages = kFit < 8 ? kFit : 8, kLag = (kStages - 1) / 2;
     static constexpr int kBytes = kStages * kStageBytes + kSumBytes + 1024;  // + alignment
     static constexpr uint32_t kTmemCols = NB * 8 < 32 ? 32 : NB * 8;
 };
@@ -133,7 +134,7 @@ template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_ra
         fence_barrier_init();
         abortFlag = 0;
     }
-    if (warp == 4) {
+    if (warp == 8) {
         tmem_alloc(&tmemSlot, C::kTmemCols);
         tmem_relinquish();
     }
@@ -157,9 +158,9 @@ template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_ra
         const int chunks = (p.K + 63) / 64, per = (chunks + clusterCtas - 1) / clusterCtas;
         const int first = min(rank * per, chunks), n = min(first + per, chunks) - first;
         bool ok = true;
-        if (warp < 4) {
+        if (warp < 8) {
             // 16 rows at a time, eight lanes a row: row (t / 8) + 16 i, piece t % 8; the swizzle exchanges pieces by the row's low three bits
-            const int piece = threadIdx.x & 7, row0 = threadIdx.x >> 3;
+            const int group = warp >> 2, piece = threadIdx.x & 7, row0 = (threadIdx.x & (kLoaders - 1)) >> 3;
             const uint32_t at = smem_u32(ring) + row0 * 128 + ((piece ^ (row0 & 7)) << 4);
             const T* x[8];
 #pragma unroll
@@ -168,7 +169,7 @@ template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_ra
                 x[i] = row < tokens ? static_cast<const T*>(p.x) + static_cast<int64_t>(p.order[start + row]) * p.ldX + first * 64 + piece * 8 : nullptr;
             }
             const T* a = static_cast<const T*>(p.a) + (static_cast<size_t>(adapter) * p.r + row0) * p.K + first * 64 + piece * 8;
-            for (int i = 0; i < n && ok; ++i) {
+            for (int i = group; i < n; i += 2) {
                 const int s = i % C::kStages;
                 if (i >= C::kStages && !(ok = mbar_wait_bounded(&emptyBar[s], (i / C::kStages - 1) & 1, &abortFlag))) break;
                 const bool kIn = (first + i) * 64 + piece * 8 < p.K;
@@ -183,14 +184,16 @@ template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_ra
                     cp_async16(slot + kAtomBytes + j * 2048, in ? a + static_cast<size_t>(16 * j) * p.K + i * 64 : p.a, in);
                 }
                 cp_commit();
-                if (i >= C::kLag) {
+                if (i >= 2 * C::kLag) {
                     cp_wait<C::kLag>();
-                    publish(&fullBar[(i - C::kLag) % C::kStages]);
+                    publish(&fullBar[(i - 2 * C::kLag) % C::kStages]);
                 }
             }
             cp_wait<0>();
-            if (ok)
-                for (int i = max(n - C::kLag, 0); i < n; ++i) publish(&fullBar[i % C::kStages]);
+            if (ok) {  // the group's last chunks
+                const int count = (n - group + 1) / 2;
+                for (int j = max(count - C::kLag, 0); j < count; ++j) publish(&fullBar[(2 * j + group) % C::kStages]);
+            }
         } else if (elect_one()) {
             constexpr uint32_t idesc = idesc_f16(kRows, R, std::is_same<T, __half>::value ? 0 : 1);
             for (int i = 0; i < n && ok; ++i) {
@@ -242,7 +245,7 @@ template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_ra
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 4) {
+    if (warp == 8) {
         tc_fence_after();
         tmem_dealloc(tmemSlot, C::kTmemCols);
     }
