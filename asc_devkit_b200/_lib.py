@@ -99,7 +99,7 @@ SIGNATURES = {
     "ascq_test_withhold_after": (_i, [_i]),
     "ascq_measure_tensor_rate": (_i, [_i, _i, C.POINTER(C.c_double), _vp]),
     "ascq_low_rank_add": (_i, [_vp, C.c_int64, _vp, C.c_int64, _vp, C.c_int64, _vp, _vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _vp, C.c_size_t, _vp]),
-    "ascq_low_rank_add_workspace_size": (C.c_size_t, [_i, _i, _i]),
+    "ascq_low_rank_add_workspace_size": (C.c_size_t, [_i, _i, _i, _i, _i]),
     "ascq_expert_sort": (_i, [_vp, _vp, _vp, _vp, _i, C.c_int64, _i, _vp]),
     "ascq_expert_dispatch": (_i, [_vp, _vp, C.c_size_t, C.c_size_t, _vp, _vp, C.c_size_t, _vp, C.c_int64, _i, C.c_int64, _vp]),
     "ascq_expert_combine": (_i, [_vp, _vp, _i, _vp, _vp, C.c_int64, _i, C.c_int64, C.c_int64, _vp]),

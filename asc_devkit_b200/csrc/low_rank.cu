@@ -23,6 +23,7 @@ using namespace ascq::ptx;
 namespace ascq {
 namespace {
 
+constexpr int kMaxRank = 128;
 constexpr int kTile = 16;         // tokens of one adapter that share a tile
 constexpr int kWarps = 8;
 constexpr int kInlineTokens = 1024;  // up to here every CTA finds its tile in the adapter numbers itself; beyond, they are sorted first
@@ -55,29 +56,48 @@ __device__ __forceinline__ Tile take_tile(const LowRankArgs& p, int tile, int* l
         __syncthreads();
         return t;
     }
+    // each warp owns a contiguous run of tokens and keeps their adapters in registers
+    constexpr int kSteps = kInlineTokens / (32 * kWarps);
+    const int run = (p.M + 32 * kWarps - 1) / (32 * kWarps) * 32, begin = warp * run;
+    int key[kSteps];
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+        const int t = begin + i * 32 + lane;
+        key[i] = i * 32 < run && t < p.M ? adapter_of(p, t) : -1;
+    }
     int* hist = work;
     int* perWarp = work + keys;
     for (int e = threadIdx.x; e < keys; e += blockDim.x) hist[e] = 0;
     __syncthreads();
-    for (int t = threadIdx.x; t < p.M; t += blockDim.x) atomicAdd(&hist[adapter_of(p, t)], 1);  // counts: the order does not show
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+        // counts: the order of the additions does not show; a run of one request's tokens is one addition
+        const int first = __shfl_sync(0xFFFFFFFFu, key[i], 0);
+        if (__all_sync(0xFFFFFFFFu, key[i] == first)) {
+            if (lane == 0 && first >= 0) atomicAdd(&hist[first], 32);
+        } else if (key[i] >= 0) {
+            atomicAdd(&hist[key[i]], 1);
+        }
+    }
     __syncthreads();
     if (warp == 0) find_tile<kTile>(tile, keys, [&](int e) { return hist[e]; }, found);
     __syncthreads();
     const Tile t{found[0], found[0] < 0 ? 0 : found[1]};
     if (t.adapter < 0) return t;
-    // the adapter's tokens in ascending order: each warp owns a contiguous run of them
-    const int run = (p.M + 32 * kWarps - 1) / (32 * kWarps) * 32, begin = warp * run, end = begin + run < p.M ? begin + run : p.M;
+    // the adapter's tokens in ascending order
     int mine = 0;
-    for (int s = begin; s < end; s += 32) mine += __popc(__ballot_sync(0xFFFFFFFFu, s + lane < end && adapter_of(p, s + lane) == t.adapter));
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) mine += __popc(__ballot_sync(0xFFFFFFFFu, key[i] == t.adapter));
     if (lane == 0) perWarp[warp] = mine;
     __syncthreads();
     int at = -found[2];
     for (int w = 0; w < warp; ++w) at += perWarp[w];
-    for (int s = begin; s < end && at < kTile; s += 32) {
-        const bool hit = s + lane < end && adapter_of(p, s + lane) == t.adapter;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+        const bool hit = key[i] == t.adapter;
         const uint32_t all = __ballot_sync(0xFFFFFFFFu, hit);
-        const int i = at + __popc(all & ((1u << lane) - 1u));
-        if (hit && i >= 0 && i < kTile) list[i] = s + lane;
+        const int slot = at + __popc(all & ((1u << lane) - 1u));
+        if (hit && slot >= 0 && slot < kTile) list[slot] = begin + i * 32 + lane;
         at += __popc(all);
     }
     __syncthreads();
@@ -95,7 +115,8 @@ template <typename T> __device__ __forceinline__ void mma16816(float (&d)[4], co
 }
 
 __host__ __device__ constexpr int padded_rank(int nb) { return nb * 8 < 32 ? 32 : nb * 8; }  // whole 32-wide k steps of the second product
-// float words of dynamic shared memory: the warps' sums (the tile finder's scratch before that), this CTA's sum, and the split result
+// float words of dynamic shared memory: the warps' sums (the tile finder's scratch before that), the cluster's partial sums (every CTA's
+// copy of all of them), and the split result
 __host__ __device__ constexpr int red_words(int nb, int L)
 {
     const int sums = kWarps * kTile * nb * 8, finder = (L + 1 + kWarps + 3) / 4 * 4;
@@ -105,15 +126,16 @@ __host__ __device__ constexpr int part_words(int nb) { return kTile * nb * 8; }
 __host__ __device__ constexpr int split_words(int nb) { return kTile * (padded_rank(nb) / 2 + 4) * 2; }
 
 // NB: blocks of 8 of the rank (r <= 8 NB)
-template <typename T, int NB> __global__ void __launch_bounds__(32 * kWarps) low_rank_kernel(const LowRankArgs p, int clusterCtas)
+template <typename T, int NB> __global__ void __launch_bounds__(32 * kWarps, NB <= 8 ? 2 : 1) low_rank_kernel(const LowRankArgs p, int clusterCtas)
 {
     extern __shared__ float smem[];
     __shared__ int list[kTile], found[4];
     __shared__ float unit[kTile];  // the power of two that brings a token's row back
     constexpr int R = NB * 8, KS = padded_rank(NB) / 32, VP = padded_rank(NB) / 2 + 4;  // VP: row pitch of the split result in words
+    constexpr bool kAhead = KS == 1;  // B's and base's first columns are requested together with x and A (registers allow it up to rank 32)
     float* red = smem;
-    float* part = red + red_words(NB, p.L);
-    uint32_t* hi = reinterpret_cast<uint32_t*>(part + part_words(NB));
+    float* part = red + red_words(NB, p.L);  // [clusterCtas][kTile][R]
+    uint32_t* hi = reinterpret_cast<uint32_t*>(part + clusterCtas * part_words(NB));
     uint32_t* lo = hi + kTile * VP;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int rank = blockIdx.x % clusterCtas;
@@ -122,53 +144,83 @@ template <typename T, int NB> __global__ void __launch_bounds__(32 * kWarps) low
     const Tile tile = take_tile(p, blockIdx.x / clusterCtas, list, found, reinterpret_cast<int*>(red));
     if (tile.adapter < 0) return;  // the same for every CTA of the cluster
     const bool has = tile.adapter < p.L;
+    if (has) cluster_arrive();     // this CTA runs: its shared memory can be written from the others
     const int units = clusterCtas * kWarps, unitIdx = rank * kWarps + warp;
+    const int t0 = list[g], t1 = list[g + 8];
+    const bool in0 = g < tile.tokens, in1 = g + 8 < tile.tokens;
+    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+
+    // second product: this warp's groups of 32 columns; lane c of a row owns 8 consecutive ones
+    const T* b = static_cast<const T*>(p.b) + static_cast<size_t>(has ? tile.adapter : 0) * p.N * p.r;
+    auto load_columns = [&](int n0, uint4 (&w)[4][KS], uint4& y0, uint4& y1) {
+        const int col = n0 + c * 8;  // N is a multiple of 8
+        y0 = p.base && in0 && col < p.N ? *reinterpret_cast<const uint4*>(static_cast<const T*>(p.base) + static_cast<int64_t>(t0) * p.ldBase + col) : zero;
+        y1 = p.base && in1 && col < p.N ? *reinterpret_cast<const uint4*>(static_cast<const T*>(p.base) + static_cast<int64_t>(t1) * p.ldBase + col) : zero;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            // column g of MMA j is column 8 (g / 2) + 2 j + (g & 1) of the group, so that accumulators 2c, 2c + 1 of the four MMAs are a
+            // lane's 8 neighbours
+            const int n = n0 + 8 * (g >> 1) + 2 * j + (g & 1);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const int k = s * 32 + c * 8;
+                w[j][s] = has && n < p.N && k < p.r ? __ldg(reinterpret_cast<const uint4*>(b + static_cast<size_t>(n) * p.r + k)) : zero;
+            }
+        }
+    };
+    uint4 w[4][KS], y0, y1;
 
     if (has) {
         // ---- inner product: this warp's chunks of 32 k
         const T* a = static_cast<const T*>(p.a) + static_cast<size_t>(tile.adapter) * p.r * p.K;
-        const T* x0 = static_cast<const T*>(p.x) + static_cast<int64_t>(list[g]) * p.ldX;
-        const T* x1 = static_cast<const T*>(p.x) + static_cast<int64_t>(list[g + 8]) * p.ldX;
-        const bool in0 = g < tile.tokens, in1 = g + 8 < tile.tokens;
+        const T* x0 = static_cast<const T*>(p.x) + static_cast<int64_t>(t0) * p.ldX;
+        const T* x1 = static_cast<const T*>(p.x) + static_cast<int64_t>(t1) * p.ldX;
         float acc[NB][4] = {};
-        const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+        if constexpr (kAhead) load_columns(unitIdx * 32, w, y0, y1);
 #pragma unroll 2
         for (int k = unitIdx * 32 + c * 8; k - c * 8 < p.K; k += units * 32) {
             const bool kIn = k < p.K;
             const uint4 u0 = in0 && kIn ? __ldg(reinterpret_cast<const uint4*>(x0 + k)) : zero;
             const uint4 u1 = in1 && kIn ? __ldg(reinterpret_cast<const uint4*>(x1 + k)) : zero;
-            uint4 w[NB];
+            uint4 v[NB];
 #pragma unroll
             for (int n = 0; n < NB; ++n)
-                w[n] = kIn && n * 8 + g < p.r ? __ldg(reinterpret_cast<const uint4*>(a + static_cast<size_t>(n * 8 + g) * p.K + k)) : zero;
+                v[n] = kIn && n * 8 + g < p.r ? __ldg(reinterpret_cast<const uint4*>(a + static_cast<size_t>(n * 8 + g) * p.K + k)) : zero;
             const uint32_t f0[4] = {u0.x, u1.x, u0.y, u1.y}, f1[4] = {u0.z, u1.z, u0.w, u1.w};
 #pragma unroll
-            for (int n = 0; n < NB; ++n) mma16816<T>(acc[n], f0, w[n].x, w[n].y);
+            for (int n = 0; n < NB; ++n) mma16816<T>(acc[n], f0, v[n].x, v[n].y);
 #pragma unroll
-            for (int n = 0; n < NB; ++n) mma16816<T>(acc[n], f1, w[n].z, w[n].w);
+            for (int n = 0; n < NB; ++n) mma16816<T>(acc[n], f1, v[n].z, v[n].w);
         }
-        __syncthreads();  // the tile finder's scratch is read no more
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
             float* to = red + warp * kTile * R + n * 8 + 2 * c;
-            to[g * R] = acc[n][0];
-            to[g * R + 1] = acc[n][1];
-            to[(g + 8) * R] = acc[n][2];
-            to[(g + 8) * R + 1] = acc[n][3];
+            *reinterpret_cast<float2*>(to + g * R) = make_float2(acc[n][0], acc[n][1]);
+            *reinterpret_cast<float2*>(to + (g + 8) * R) = make_float2(acc[n][2], acc[n][3]);
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < kTile * R; i += blockDim.x) {
-            float s = red[i];
+        // the CTA's sum goes to every CTA of the cluster (stores, which nobody waits for, rather than loads): one cluster barrier, then all
+        // of them add up the same partial sums in the same order
+        cluster_wait();
+        for (int i = threadIdx.x * 4; i < kTile * R; i += blockDim.x * 4) {
+            float4 s = *reinterpret_cast<const float4*>(red + i);
 #pragma unroll
-            for (int w = 1; w < kWarps; ++w) s += red[w * kTile * R + i];
-            part[i] = s;
+            for (int q = 1; q < kWarps; ++q) {
+                const float4 f = *reinterpret_cast<const float4*>(red + q * kTile * R + i);
+                s.x += f.x; s.y += f.y; s.z += f.z; s.w += f.w;
+            }
+            const uint32_t at = smem_u32(part + rank * part_words(NB) + i);
+            const uint4 bits = make_uint4(__float_as_uint(s.x), __float_as_uint(s.y), __float_as_uint(s.z), __float_as_uint(s.w));
+            for (int q = 0; q < clusterCtas; ++q) st_cluster_v4(mapa_u32(at, q), bits);
         }
+        const float scale = p.scale ? p.scale[tile.adapter] : 1.0f;
         __syncwarp();
         cluster_arrive();
         cluster_wait();
         // ---- the cluster's sum, scaled, brought to a common range per token and split; a warp takes two tokens
-        const float scale = p.scale ? p.scale[tile.adapter] : 1.0f;
-        for (int row = warp; row < kTile; row += kWarps) {
+#pragma unroll
+        for (int u = 0; u < kTile / kWarps; ++u) {
+            const int row = warp + u * kWarps;
             float v[(R + 31) / 32];
             float top = 0.f;
 #pragma unroll
@@ -176,8 +228,7 @@ template <typename T, int NB> __global__ void __launch_bounds__(32 * kWarps) low
                 const int col = lane + 32 * i;
                 v[i] = 0.f;
                 if (col < R) {
-                    const uint32_t at = smem_u32(part + row * R + col);
-                    for (int q = 0; q < clusterCtas; ++q) v[i] += ld_cluster_f32(mapa_u32(at, q));
+                    for (int q = 0; q < clusterCtas; ++q) v[i] += part[q * part_words(NB) + row * R + col];
                     v[i] *= scale;
                 }
                 top = fmaxf(top, fabsf(v[i]));
@@ -189,17 +240,18 @@ template <typename T, int NB> __global__ void __launch_bounds__(32 * kWarps) low
             if (lane == 0) unit[row] = exp2_int(shift);
             unsigned short* h = reinterpret_cast<unsigned short*>(hi + row * VP);
             unsigned short* l = reinterpret_cast<unsigned short*>(lo + row * VP);
-            for (int col = lane; col < padded_rank(NB); col += 32) {
-                const uint2 two = split16<T>(col < R ? v[col / 32] * down : 0.f);
+#pragma unroll
+            for (int i = 0; i < padded_rank(NB) / 32; ++i) {
+                const int col = lane + 32 * i;
+                const uint2 two = split16<T>(col < R ? v[i] * down : 0.f);
                 h[col] = static_cast<unsigned short>(two.x);
                 l[col] = static_cast<unsigned short>(two.y);
             }
         }
         __syncthreads();
-        cluster_arrive();  // this CTA has read the others' sums; the wait is at the end
     }
 
-    // ---- second product: this warp's groups of 32 columns; lane c of a row owns 8 consecutive ones
+    // ---- second product
     uint32_t fh[KS][2][4], fl[KS][2][4];
     float back0 = 0.f, back1 = 0.f;
     if (has) {
@@ -215,60 +267,50 @@ template <typename T, int NB> __global__ void __launch_bounds__(32 * kWarps) low
         back0 = unit[g];
         back1 = unit[g + 8];
     }
-    const T* b = static_cast<const T*>(p.b) + static_cast<size_t>(has ? tile.adapter : 0) * p.N * p.r;
+    if (!kAhead || !has) load_columns(unitIdx * 32, w, y0, y1);
     for (int n0 = unitIdx * 32; n0 < p.N; n0 += units * 32) {
         float acc[4][4] = {};
         const int col = n0 + c * 8;
-        const bool nIn = col < p.N;  // N is a multiple of 8
-        uint4 y0 = make_uint4(0u, 0u, 0u, 0u), y1 = y0;
-        if (p.base && nIn) {
-            if (g < tile.tokens) y0 = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.base) + static_cast<int64_t>(list[g]) * p.ldBase + col);
-            if (g + 8 < tile.tokens) y1 = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.base) + static_cast<int64_t>(list[g + 8]) * p.ldBase + col);
-        }
         if (has) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                // column g of MMA j is column 8 (g / 2) + 2 j + (g & 1) of the group, so that accumulators 2c, 2c + 1 of the four MMAs are a
-                // lane's 8 neighbours
-                const int n = n0 + 8 * (g >> 1) + 2 * j + (g & 1);
+            for (int s = 0; s < KS; ++s)
 #pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                    const int k = s * 32 + c * 8;
-                    const uint4 w = n < p.N && k < p.r ? __ldg(reinterpret_cast<const uint4*>(b + static_cast<size_t>(n) * p.r + k)) : make_uint4(0u, 0u, 0u, 0u);
-                    mma16816<T>(acc[j], fh[s][0], w.x, w.y);
-                    mma16816<T>(acc[j], fh[s][1], w.z, w.w);
-                    mma16816<T>(acc[j], fl[s][0], w.x, w.y);
-                    mma16816<T>(acc[j], fl[s][1], w.z, w.w);
-                }
-            }
+                for (int q = 0; q < 2; ++q)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        mma16816<T>(acc[j], fh[s][q], q ? w[j][s].z : w[j][s].x, q ? w[j][s].w : w[j][s].y);
+                        mma16816<T>(acc[j], fl[s][q], q ? w[j][s].z : w[j][s].x, q ? w[j][s].w : w[j][s].y);
+                    }
         }
-        if (!nIn) continue;
-        uint32_t o0[4], o1[4];
         const uint32_t i0[4] = {y0.x, y0.y, y0.z, y0.w}, i1[4] = {y1.x, y1.y, y1.z, y1.w};
+        if (n0 + units * 32 < p.N) load_columns(n0 + units * 32, w, y0, y1);
+        if (col >= p.N) continue;
+        uint4 o0 = make_uint4(i0[0], i0[1], i0[2], i0[3]), o1 = make_uint4(i1[0], i1[1], i1[2], i1[3]);
+        if (has) {
+            float f0[8], f1[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 v0 = unpack2<T>(i0[j]), v1 = unpack2<T>(i1[j]);
-            const float r0 = fmaf(acc[j][0], back0, v0.x), r1 = fmaf(acc[j][1], back0, v0.y), r2 = fmaf(acc[j][2], back1, v1.x), r3 = fmaf(acc[j][3], back1, v1.y);
-            o0[j] = has ? pack_sat<T>(r0, r1) : i0[j];
-            o1[j] = has ? pack_sat<T>(r2, r3) : i1[j];
+            for (int j = 0; j < 4; ++j) {
+                const float2 v0 = unpack2<T>(i0[j]), v1 = unpack2<T>(i1[j]);
+                f0[2 * j] = fmaf(acc[j][0], back0, v0.x);
+                f0[2 * j + 1] = fmaf(acc[j][1], back0, v0.y);
+                f1[2 * j] = fmaf(acc[j][2], back1, v1.x);
+                f1[2 * j + 1] = fmaf(acc[j][3], back1, v1.y);
+            }
+            o0 = pack8_sat<T>(f0);
+            o1 = pack8_sat<T>(f1);
         }
-        if (g < tile.tokens) *reinterpret_cast<uint4*>(static_cast<T*>(p.dst) + static_cast<int64_t>(list[g]) * p.ldDst + col) = make_uint4(o0[0], o0[1], o0[2], o0[3]);
-        if (g + 8 < tile.tokens)
-            *reinterpret_cast<uint4*>(static_cast<T*>(p.dst) + static_cast<int64_t>(list[g + 8]) * p.ldDst + col) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
-    }
-    if (has) {
-        __syncwarp();
-        cluster_wait();
+        if (in0) *reinterpret_cast<uint4*>(static_cast<T*>(p.dst) + static_cast<int64_t>(t0) * p.ldDst + col) = o0;
+        if (in1) *reinterpret_cast<uint4*>(static_cast<T*>(p.dst) + static_cast<int64_t>(t1) * p.ldDst + col) = o1;
     }
 }
 
 template <typename T, int NB> ascq_status launch_low_rank(const LowRankArgs& p, int cluster, unsigned tiles, cudaStream_t st)
 {
-    const size_t smem = (static_cast<size_t>(red_words(NB, p.L)) + part_words(NB) + split_words(NB)) * 4;
+    const size_t smem = (static_cast<size_t>(red_words(NB, p.L)) + static_cast<size_t>(cluster) * part_words(NB) + split_words(NB)) * 4;
     static PerDeviceOnce once;
     const int dev = current_device();
     if (!once.done(dev)) {
-        const int most = (red_words(NB, kMaxSortKeys) + part_words(NB) + split_words(NB)) * 4;
+        const int most = (red_words(NB, kMaxSortKeys) + 8 * part_words(NB) + split_words(NB)) * 4;
         ASCQ_CUDA_CHECK(cudaFuncSetAttribute(low_rank_kernel<T, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
         once.mark(dev);
     }
@@ -298,8 +340,14 @@ template <typename T> ascq_status launch_low_rank_typed(const LowRankArgs& p, in
     return launch_low_rank<T, 16>(p, cluster, tiles, st);
 }
 
-// Tiles of 128 tokens pay when an adapter has enough tokens to fill them.
-bool long_tiles(int M, int L) { return M > kInlineTokens && M / (L + 1) >= 16; }
+// Tiles of 128 tokens pay for their second and third launch when there is enough to do and adapters have tokens to fill them.  Measured, us,
+// tiles of 16 / of 128 tokens: K + N = 15104, rank 64, 4 adapters 24 / 33 at 1024 tokens, 44 / 33 at 1500; K = N = 4096, rank 64, 16 adapters 32 / 35 at
+// 2048, 59 / 55 at 4096, but 62 / 86 with 64 adapters; rank 128, K + N = 15104, 4 adapters 55 / 31 at 512 (16 adapters: 33 / 42).
+bool long_tiles(int M, int N, int K, int r, int L)
+{
+    const int64_t work = static_cast<int64_t>(M) * (static_cast<int64_t>(K) + N) * (r > 64 ? 3 : 1);
+    return work >= 16'000'000 && M / (L + 1) >= (r > 64 ? 48 : 96);
+}
 
 // Every adapter with tokens, and the tokens without one, can leave one tile partly filled.
 int64_t tile_bound(int M, int L, int size) { return M / size + std::min(L + 1, M); }
@@ -307,14 +355,16 @@ int64_t tile_bound(int M, int L, int size) { return M / size + std::min(L + 1, M
 struct Workspace {
     size_t order, tiles, unit, v, bytes;  // offsets; the counts come first
 };
-Workspace workspace_of(int M, int r, int L)
+Workspace workspace_of(int M, int N, int K, int r, int L)
 {
     Workspace w{};
-    if (M <= kInlineTokens || r <= 0 || r > 128 || L <= 0) return w;
+    if (M <= 0 || N <= 0 || K <= 0 || r <= 0 || r > kMaxRank || L <= 0) return w;
+    const bool tiled = long_tiles(M, N, K, r, L);
+    if (M <= kInlineTokens && !tiled) return w;
     auto up = [](size_t n) { return (n + 15) / 16 * 16; };
     w.order = up((static_cast<size_t>(L) + 1) * 8);
     w.bytes = w.order + up(static_cast<size_t>(M) * 4);
-    if (long_tiles(M, L)) {
+    if (tiled) {
         w.tiles = w.bytes;
         w.unit = w.tiles + low_rank_long_tiles_bytes(tile_bound(M, L, kLongTile));
         w.v = w.unit + up(static_cast<size_t>(M) * 4);
@@ -323,12 +373,10 @@ Workspace workspace_of(int M, int r, int L)
     return w;
 }
 
-constexpr int kMaxRank = 128;
-
 }  // namespace
 }  // namespace ascq
 
-extern "C" size_t ascq_low_rank_add_workspace_size(int M, int r, int L) { return workspace_of(M, r, L).bytes; }
+extern "C" size_t ascq_low_rank_add_workspace_size(int M, int N, int K, int r, int L) { return workspace_of(M, N, K, r, L).bytes; }
 
 extern "C" ascq_status ascq_low_rank_add(void* dst, int64_t ldDst, const void* base, int64_t ldBase, const void* x, int64_t ldX, const void* A, const void* B,
                                          ascq_dtype T, const void* adapterIds, ascq_dtype idT, const float* scale, int M, int N, int K, int r, int L,
@@ -352,7 +400,7 @@ extern "C" ascq_status ascq_low_rank_add(void* dst, int64_t ldDst, const void* b
     if ((reinterpret_cast<uintptr_t>(adapterIds) & (idT == ASCQ_DT_I64 ? 7u : 3u)) || (reinterpret_cast<uintptr_t>(scale) & 3u))
         return fail(ASCQ_ERR_ALIGNMENT, "a tensor is not aligned to its element type");
     const size_t rows = static_cast<size_t>(M);
-    const Workspace ws = workspace_of(M, r, L);
+    const Workspace ws = workspace_of(M, N, K, r, L);
     const size_t need = ws.bytes;
     if (need && (!workspace || workspaceBytes < need)) return fail(ASCQ_ERR_INVALID_ARG, "the workspace has %zu bytes, %zu are needed", workspaceBytes, need);
     if (need && !aligned16(workspace)) return fail(ASCQ_ERR_ALIGNMENT, "the workspace must be 16-byte aligned");

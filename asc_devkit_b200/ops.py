@@ -534,7 +534,7 @@ def LowRankAdd(dstTensor: torch.Tensor, base: Optional[torch.Tensor], X: torch.T
     code, idc = dtype_code(X), _id_code(adapterIds)
     dev = _cuda_index(X)
     if workspace is None:
-        need = L.lib().ascq_low_rank_add_workspace_size(M, r, Lo)
+        need = L.lib().ascq_low_rank_add_workspace_size(M, N, K, r, Lo)
         if need:
             workspace = _workspace(need, X.device, stream)
     (dp, ldd), (bp, ldb), (xp, ldx) = _rows(dstTensor, dev), _rows(base, dev), _rows(X, dev)

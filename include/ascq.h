@@ -499,14 +499,14 @@ ascq_status ascq_matmul_w4a16(void* C, ascq_dtype cT, const void* A, ascq_dtype 
  * contiguous; A and B contiguous), adapterIds [M] of idT = int32 or int64 in any order, scale fp32 [L] or NULL (1).  A token whose number is
  * outside [0, L) keeps base[t].  base may be dst itself (same pitch) or NULL (0).  Both products accumulate in fp32 and the inner one is not
  * rounded to T in between.  N % 8 == 0, K % 8 == 0, r % 8 == 0, r <= 128, L <= 1023; tensors 16-byte aligned.
- * workspace: ascq_low_rank_add_workspace_size(M, r, L) bytes (0 for M <= 1024), 16-byte aligned, private to this call until the
+ * workspace: ascq_low_rank_add_workspace_size(M, N, K, r, L) bytes (0 for small calls), 16-byte aligned, private to this call until the
  * stream reaches the end of it.
  */
 ascq_status ascq_low_rank_add(void* dst, int64_t ldDst, const void* base, int64_t ldBase, const void* x, int64_t ldX,
                               const void* A, const void* B, ascq_dtype T, const void* adapterIds, ascq_dtype idT,
                               const float* scale, int M, int N, int K, int r, int L, void* workspace, size_t workspaceBytes,
                               void* stream);
-size_t ascq_low_rank_add_workspace_size(int M, int r, int L);
+size_t ascq_low_rank_add_workspace_size(int M, int N, int K, int r, int L);
 
 /*
  * The grouped MX matmul with 8-bit operands (fp8_e4m3fn / fp8_e5m2 in any combination, one E8M0 scale per 32 elements

@@ -57,7 +57,10 @@ def check(got, x, base, a, b, scale, ids):
 SHAPES = [  # m, n, k, r, adapters, tokens of a request
     (1, 8, 8, 8, 1, 1), (1, 4096, 4096, 16, 16, 1), (32, 4096, 4096, 16, 16, 1), (5, 264, 520, 8, 3, 1), (17, 1000, 72, 24, 2, 1), (16, 96, 2048, 40, 40, 1),
     (64, 512, 1024, 64, 64, 1), (200, 2048, 512, 128, 5, 33), (1024, 256, 512, 16, 1000, 1), (1025, 256, 512, 32, 1023, 1), (1337, 640, 1376, 32, 8, 97),
-    (2500, 264, 136, 64, 3, 700), (3000, 520, 1032, 104, 7, 1), (1100, 4096, 256, 128, 4, 300), (4096, 1024, 1024, 64, 16, 256)]
+    (2500, 264, 136, 64, 3, 700), (3000, 520, 1032, 104, 7, 1), (1100, 4096, 256, 128, 4, 300), (4096, 1024, 1024, 64, 16, 256),
+    # tiles of 128 tokens: more than 16 million of m (n + k), a third of that for ranks above 64
+    (1500, 4104, 8200, 16, 3, 1), (2000, 8200, 72, 32, 5, 130), (4100, 4096, 264, 64, 16, 300), (1030, 200, 5000, 128, 2, 1030), (520, 5000, 5000, 104, 2, 7), (6000, 8, 2760, 8, 20, 1),
+    (2100, 8000, 8, 24, 1, 2100), (3000, 3000, 3000, 48, 4, 129)]
 
 
 @gpu
@@ -208,9 +211,11 @@ def test_refusals():
                 dict(m=2000, ws=0x7000008, wsb=1 << 20)):
         assert call(**bad) == L.ERR_ALIGNMENT, bad
     size = L.lib().ascq_low_rank_add_workspace_size
-    assert size(1024, 16, 8) == 0
-    assert size(2000, 16, 1000) == 8016 + 2000 * 4                       # counts and order
-    assert size(2000, 64, 3) == 32 + 8000 + (2000 // 128 + 5) * 16 + 8000 + 2000 * 2 * 64 * 2  # and tiles, units and the inner products
+    assert size(1024, 4096, 4096, 16, 8) == 0
+    assert size(2000, 4096, 4096, 16, 1000) == 8016 + 2000 * 4                    # counts and order
+    # many tokens of few adapters: tiles (and their number), units and the inner products too
+    assert size(2000, 8192, 4096, 64, 3) == 32 + 8000 + (2000 // 128 + 5) * 16 + 8000 + 2000 * 2 * 64 * 2
+    assert size(512, 11008, 4096, 128, 3) > 0 and size(512, 11008, 4096, 64, 3) == 0
 
 
 def test_python_refusals():
