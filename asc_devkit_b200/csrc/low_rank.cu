@@ -341,12 +341,12 @@ template <typename T> ascq_status launch_low_rank_typed(const LowRankArgs& p, in
 }
 
 // Tiles of 128 tokens pay for their second and third launch when there is enough to do and adapters have tokens to fill them.  Measured, us,
-// tiles of 16 / of 128 tokens: K + N = 15104, rank 64, 4 adapters 24 / 33 at 1024 tokens, 44 / 33 at 1500; K = N = 4096, rank 64, 16 adapters 32 / 35 at
-// 2048, 59 / 55 at 4096, but 62 / 86 with 64 adapters; rank 128, K + N = 15104, 4 adapters 55 / 31 at 512 (16 adapters: 33 / 42).
+// tiles of 16 / of 128 tokens, 4 adapters: K + N = 15104, rank 64: 23 / 30 at 1024 tokens, 43 / 31 at 1500; K = N = 4096, rank 64: 29 / 30 at 2048,
+// 47 / 31 at 2800; rank 16: 20 / 26, 35 / 27; rank 128: 25 / 24 at 512, 39 / 27 at 1024.  64 adapters, rank 64, 4096 tokens: 62 / 86.
 bool long_tiles(int M, int N, int K, int r, int L)
 {
     const int64_t work = static_cast<int64_t>(M) * (static_cast<int64_t>(K) + N) * (r > 64 ? 3 : 1);
-    return work >= 16'000'000 && M / (L + 1) >= (r > 64 ? 48 : 96);
+    return work >= 20'000'000 && M / (L + 1) >= (r > 64 ? 24 : 64) && static_cast<int64_t>(L) * N <= 0x7FFFFFFF;  // (the copies' coordinates are int)
 }
 
 // Every adapter with tokens, and the tokens without one, can leave one tile partly filled.
@@ -437,6 +437,8 @@ extern "C" ascq_status ascq_low_rank_add(void* dst, int64_t ldDst, const void* b
     }
     const unsigned tiles = static_cast<unsigned>(tile_bound(M, L, kTile));
     int cluster = 8;
-    while (cluster > 1 && static_cast<uint64_t>(tiles) * cluster > 2ull * sm_count()) cluster /= 2;
+    // as many CTAs as are resident together: two per SM, above rank 64 one (and clusters of 8 do not fill every SM)
+    const uint64_t limit = r > 64 ? sm_count() * 7 / 8 : 2 * sm_count();
+    while (cluster > 1 && static_cast<uint64_t>(tiles) * cluster > limit) cluster /= 2;
     return T == ASCQ_DT_F16 ? launch_low_rank_typed<__half>(p, cluster, tiles, st) : launch_low_rank_typed<__nv_bfloat16>(p, cluster, tiles, st);
 }

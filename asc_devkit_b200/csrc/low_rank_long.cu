@@ -4,10 +4,12 @@
 //           terms, [M][2][pitch] in sorted order, with one power of two per token
 //   outer   dst = base + V . B^T for a tile and a range of columns
 // What bounds both is HBM: the inner launch reads x once, the outer one reads base and writes dst; A and B come from L2 once per 128
-// tokens.  The tokens of a tile lie anywhere, so rows are gathered with 16-byte cp.async into the 128-byte-swizzled layout that the
-// tensor cores read; 64 elements of a row are 128 bytes, and the eight lanes that share a row fill a whole line.
+// tokens.  The tokens of a tile lie anywhere, so their rows are gathered with 16-byte cp.async into the 128-byte-swizzled layout that the
+// tensor cores read; 64 elements of a row are 128 bytes, and the lanes that share a row fill a whole line.  What lies in order -- A, B, V -- comes
+// by TMA: one thread asks for a tile, and no warp has to wait for it and make it visible to the tensor cores.
 #include "low_rank.cuh"
 #include "sm100_ptx.cuh"
+#include "tma_host.h"
 
 using namespace ascq;
 using namespace ascq::ptx;
@@ -16,14 +18,15 @@ namespace ascq {
 namespace {
 
 constexpr int kRows = kLongTile;
-constexpr int kLoaders = 128, kThreads = 2 * kLoaders + 32;     // inner: two groups of four warps copy, the first finishes too; one more warp issues the MMAs
-constexpr int kFinishers = 256, kOuterThreads = kFinishers + 32;  // outer: eight and one
+constexpr int kLoaders = 128, kThreads = 2 * kLoaders + 64;      // inner: two groups of four warps gather x, the first finishes too; one warp
+                                                               // issues the MMAs, one the loads of A
+constexpr int kFinishers = 256, kOuterThreads = kFinishers + 32;  // outer: eight warps move base and dst, one issues loads and MMAs
 constexpr int kAtomBytes = kRows * 128;    // 128 rows x 64 elements
 constexpr int kBlockCols = 64;             // outer: columns of an MMA
 
 __device__ int g_low_rank_status;  // 1: a bounded wait ran out
 
-__host__ __device__ constexpr int rank_pitch(int nb) { return nb * 8 < 32 ? 32 : nb * 8; }  // elements of the hi (or lo) part of a row of V
+__host__ __device__ constexpr int rank_pitch(int nb) { return nb * 8 < 64 ? 64 : nb * 8; }  // elements of the hi (or lo) part of a row of V
 constexpr int rank_blocks(int r) { return r <= 16 ? 2 : r <= 32 ? 4 : r <= 64 ? 8 : 16; }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool in)
@@ -33,6 +36,12 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool i
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// Waits, bounded, for a copy that is on its way although the CTA gives up.
+__device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity)
+{
+    const long long t0 = clock64();
+    while (!mbar_try_wait(bar, parity) && clock64() - t0 < c_waitCycles) {}
+}
 // this thread's finished copies become visible to the tensor cores, and the barrier learns of it
 __device__ __forceinline__ void publish(uint64_t* bar)
 {
@@ -55,7 +64,7 @@ template <int NB> struct Ring {
 // The rows of one CTA's share: CTAS threads a row, each sums its columns over the cluster's CTAs, scales them, finds the row's largest
 // value with its neighbours and writes the two terms.
 template <typename T, int NB, int CTAS>
-__device__ __forceinline__ void finish_rows(const float* part, int there, int start, float scale, const LowRankScratch& o)
+__device__ __forceinline__ void finish_rows(const float* part, int there, int start, int r, float scale, const LowRankScratch& o)
 {
     constexpr int R = NB * 8, VP = rank_pitch(NB), kPitch = R + 4, kShare = kRows / CTAS, W = R / CTAS;  // W: columns of a thread
     const int row = threadIdx.x / CTAS, col0 = (threadIdx.x % CTAS) * W;
@@ -76,7 +85,7 @@ __device__ __forceinline__ void finish_rows(const float* part, int there, int st
     }
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-        v[i] *= scale;
+        v[i] = col0 + i < r ? v[i] * scale : 0.f;
         top = fmaxf(top, fabsf(v[i]));
     }
 #pragma unroll
@@ -106,20 +115,22 @@ __device__ __forceinline__ void finish_rows(const float* part, int there, int st
             to[VP / 2 + i] = lo[i];
         }
     }
-    if constexpr (VP > R) {  // the rest of a short row is zeros: W more columns of each thread
-        static_assert(VP == 2 * R, "ranks up to 16 take rows of 32");
+    if constexpr (VP > R) {  // the rest of a short row is zeros: every thread fills its share
+        constexpr int kRest = (VP - R) / CTAS / 2;
+        uint32_t* rest = reinterpret_cast<uint32_t*>(static_cast<unsigned short*>(o.v) + static_cast<size_t>(start + row) * 2 * VP + R) + (threadIdx.x % CTAS) * kRest;
 #pragma unroll
-        for (int i = 0; i < W / 2; ++i) to[R / 2 + i] = to[VP / 2 + R / 2 + i] = 0u;
+        for (int i = 0; i < kRest; ++i) rest[i] = rest[VP / 2 + i] = 0u;
     }
 }
 
-template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_rank_inner_kernel(const LowRankArgs p, const LowRankScratch o, int clusterCtas)
+template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_rank_inner_kernel(const LowRankArgs p, const LowRankScratch o, int clusterCtas,
+                                                                                          const __grid_constant__ CUtensorMap mapA)
 {
     using C = Ring<NB>;
     constexpr int R = NB * 8, kPitch = R + 4;
     extern __shared__ uint8_t raw[];
     __shared__ int found[4];
-    __shared__ uint64_t fullBar[C::kStages], emptyBar[C::kStages], doneBar;
+    __shared__ uint64_t fullBar[C::kStages], aBar[C::kStages], emptyBar[C::kStages], doneBar;  // x gathered, A loaded, both read
     __shared__ uint32_t tmemSlot;
     __shared__ int abortFlag;
     uint8_t* ring = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
@@ -128,6 +139,7 @@ template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_ra
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::kStages; ++i) {
             mbar_init(&fullBar[i], kLoaders);
+            mbar_init(&aBar[i], 1);
             mbar_init(&emptyBar[i], 1);
         }
         mbar_init(&doneBar, 1);
@@ -168,7 +180,6 @@ template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_ra
                 const int row = row0 + 16 * i;
                 x[i] = row < tokens ? static_cast<const T*>(p.x) + static_cast<int64_t>(p.order[start + row]) * p.ldX + first * 64 + piece * 8 : nullptr;
             }
-            const T* a = static_cast<const T*>(p.a) + (static_cast<size_t>(adapter) * p.r + row0) * p.K + first * 64 + piece * 8;
             for (int i = group; i < n; i += 2) {
                 const int s = i % C::kStages;
                 if (i >= C::kStages && !(ok = mbar_wait_bounded(&emptyBar[s], (i / C::kStages - 1) & 1, &abortFlag))) break;
@@ -178,11 +189,6 @@ template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_ra
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     if (x[j]) cp_async16(slot + j * 2048, kIn ? x[j] + i * 64 : p.x, kIn);
-#pragma unroll
-                for (int j = 0; j < NB / 2; ++j) {
-                    const bool in = kIn && row0 + 16 * j < p.r;
-                    cp_async16(slot + kAtomBytes + j * 2048, in ? a + static_cast<size_t>(16 * j) * p.K + i * 64 : p.a, in);
-                }
                 cp_commit();
                 if (i >= 2 * C::kLag) {
                     cp_wait<C::kLag>();
@@ -194,11 +200,24 @@ template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_ra
                 const int count = (n - group + 1) / 2;
                 for (int j = max(count - C::kLag, 0); j < count; ++j) publish(&fullBar[(2 * j + group) % C::kStages]);
             }
+        } else if (warp == 9) {
+            if (elect_one()) {
+                int i = 0;
+                for (; i < n; ++i) {
+                    const int s = i % C::kStages;
+                    if (i >= C::kStages && !(ok = mbar_wait_bounded(&emptyBar[s], (i / C::kStages - 1) & 1, &abortFlag))) break;
+                    // rows behind the adapter's rank are the next adapter's (or zeros): columns of D that finish_rows leaves out
+                    mbar_arrive_expect_tx(&aBar[s], C::kABytes);
+                    tma_load_2d(ring + s * C::kStageBytes + kAtomBytes, &mapA, &aBar[s], (first + i) * 64, adapter * p.r);
+                }
+                if (!ok)  // no copy may be on its way when the CTA ends
+                    for (int j = max(i - C::kStages, 0); j < i; ++j) drain(&aBar[j % C::kStages], (j / C::kStages) & 1);
+            }
         } else if (elect_one()) {
             constexpr uint32_t idesc = idesc_f16(kRows, R, std::is_same<T, __half>::value ? 0 : 1);
             for (int i = 0; i < n && ok; ++i) {
                 const int s = i % C::kStages;
-                if (!(ok = mbar_wait_bounded(&fullBar[s], (i / C::kStages) & 1, &abortFlag))) break;
+                if (!(ok = mbar_wait_bounded(&aBar[s], (i / C::kStages) & 1, &abortFlag) && mbar_wait_bounded(&fullBar[s], (i / C::kStages) & 1, &abortFlag))) break;
                 tc_fence_after();
                 const uint32_t at = smem_u32(ring) + s * C::kStageBytes;
                 const uint64_t descX = smem_desc_sw128(at), descA = smem_desc_sw128(at + kAtomBytes);
@@ -237,10 +256,10 @@ template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_ra
         if (warp < 4) {
             const float scale = p.scale ? p.scale[adapter] : 1.0f;
             const int there = tokens - rank * share;  // rows of this CTA's share that have a token
-            if (clusterCtas == 1) finish_rows<T, NB, 1>(part, there, start, scale, o);
-            else if (clusterCtas == 2) finish_rows<T, NB, 2>(part, there, start + rank * share, scale, o);
-            else if (clusterCtas == 4) finish_rows<T, NB, 4>(part, there, start + rank * share, scale, o);
-            else finish_rows<T, NB, 8>(part, there, start + rank * share, scale, o);
+            if (clusterCtas == 1) finish_rows<T, NB, 1>(part, there, start, p.r, scale, o);
+            else if (clusterCtas == 2) finish_rows<T, NB, 2>(part, there, start + rank * share, p.r, scale, o);
+            else if (clusterCtas == 4) finish_rows<T, NB, 4>(part, there, start + rank * share, p.r, scale, o);
+            else finish_rows<T, NB, 8>(part, there, start + rank * share, p.r, scale, o);
         }
     }
     tc_fence_before();
@@ -263,21 +282,25 @@ template <int NB> struct Outer {
 // touch one tile or two; for each it loads V once and streams B and base.  (With a CTA for each tile and 512 columns the two waves' starts were
 // as long as their work: 42 us instead of 31 at 8192 tokens, 4096 columns.)
 template <typename T, int NB>
-__global__ void __launch_bounds__(kOuterThreads, NB <= 8 ? 2 : 1) low_rank_outer_kernel(const LowRankArgs p, const LowRankScratch o, int tileBound)
+__global__ void __launch_bounds__(kOuterThreads, NB <= 8 ? 2 : 1) low_rank_outer_kernel(const LowRankArgs p, const LowRankScratch o, int tileBound, const __grid_constant__ CUtensorMap mapB,
+                          const __grid_constant__ CUtensorMap mapV)
 {
     using C = Outer<NB>;
     constexpr int VP = rank_pitch(NB);
     extern __shared__ uint8_t raw[];
-    __shared__ uint64_t inBar[3], outBar[2];
+    __shared__ uint64_t vBar, bBar[3], freeBar[2], outBar[2];
     __shared__ uint32_t tmemSlot;
     __shared__ int abortFlag;
     uint8_t* sV = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
     uint8_t *sB = sV + C::kVBytes, *sY = sB + 3 * C::kBBytes;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 3; ++i) mbar_init(&inBar[i], kFinishers);
-        mbar_init(&outBar[0], 1);
-        mbar_init(&outBar[1], 1);
+        mbar_init(&vBar, 1);
+        for (int i = 0; i < 3; ++i) mbar_init(&bBar[i], 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&freeBar[i], 8);  // the warps that have read an accumulator
+            mbar_init(&outBar[i], 1);
+        }
         fence_barrier_init();
         abortFlag = 0;
     }
@@ -296,7 +319,7 @@ __global__ void __launch_bounds__(kOuterThreads, NB <= 8 ? 2 : 1) low_rank_outer
     __syncthreads();
     tc_fence_after();
     bool ok = true;
-    uint32_t it = 0;  // blocks multiplied so far: the barriers' slots and phases go by it
+    uint32_t it = 0, segment = 0;  // blocks multiplied so far, and tiles: the barriers' slots and phases go by them
     while (pos < end && ok) {
         const int tileIdx = static_cast<int>(pos / perTile), first = static_cast<int>(pos % perTile);
         const int blocks = static_cast<int>(min(end - pos, static_cast<int64_t>(perTile - first)));
@@ -331,63 +354,36 @@ __global__ void __launch_bounds__(kOuterThreads, NB <= 8 ? 2 : 1) low_rank_outer
                 from[i] = t >= 0 && p.base ? static_cast<const T*>(p.base) + t * p.ldBase + col0 + movePiece * 8 : nullptr;
                 to[i] = t >= 0 ? static_cast<T*>(p.dst) + t * p.ldDst + col0 + movePiece * 8 : nullptr;
             }
-            {   // V: row (t / 8) + 32 i, piece t % 8
-                const int piece = threadIdx.x & 7, row0 = threadIdx.x >> 3;
-                const uint32_t at = smem_u32(sV) + row0 * 128 + ((piece ^ (row0 & 7)) << 4);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (row0 + 32 * i < tokens && (VP >= 64 || piece < 4)) {
-                        const T* v = static_cast<const T*>(o.v) + static_cast<size_t>(start + row0 + 32 * i) * 2 * VP + piece * 8;
-#pragma unroll
-                        for (int h = 0; h < 2; ++h)
-#pragma unroll
-                            for (int ka = 0; ka < C::kAtoms; ++ka) cp_async16(at + (h * C::kAtoms + ka) * kAtomBytes + i * 4096, v + h * VP + ka * 64, true);
-                    }
-            }
-            // B: row (t / 8) + 32 i of a block, piece t % 8
-            const int bPiece = threadIdx.x & 7, bRow0 = threadIdx.x >> 3;
-            const uint32_t bAt = smem_u32(sB) + bRow0 * 128 + ((bPiece ^ (bRow0 & 7)) << 4);
-            const T* b0 = static_cast<const T*>(p.b) + (static_cast<size_t>(adapter) * p.N + col0 + bRow0) * p.r + bPiece * 8;
             const int myRow = quarter * 32 + lane;
             const float unit = myRow < tokens ? o.unit[start + myRow] : 0.f;
-            const int bCols = p.N - col0 - bRow0, moveCols = colEnd - col0 - movePiece * 8;  // a piece is inside while its block's column is below
+            const int moveCols = colEnd - col0 - movePiece * 8;  // the piece is inside while its block's column is below
             auto request = [&](int b) {
-                if (b < blocks) {
-                    const int c0 = b * kBlockCols, s = (it + b) % 3;
+                if (b * kBlockCols < moveCols) {
+                    const uint32_t y = smem_u32(sY) + (it + b) % 3 * C::kYBytes + moveAt;
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int ka = 0; ka < C::kAtoms; ++ka) {
-                            const bool in = c0 + 32 * i < bCols && ka * 64 + bPiece * 8 < p.r;
-                            cp_async16(bAt + s * C::kBBytes + ka * kBlockCols * 128 + i * 4096, in ? b0 + static_cast<size_t>(c0 + 32 * i) * p.r + ka * 64 : p.b, in);
-                        }
-                    if (c0 < moveCols) {
-                        const uint32_t y = smem_u32(sY) + s * C::kYBytes + moveAt;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (from[i]) cp_async16(y + i * 1024, from[i] + c0, true);
-                    }
+                    for (int i = 0; i < 4; ++i)
+                        if (from[i]) cp_async16(y + i * 1024, from[i] + b * kBlockCols, true);
                 }
                 cp_commit();
             };
             request(0);
             request(1);
-            cp_wait<1>();
-            publish(&inBar[it % 3]);
             for (int b = 0; b < blocks; ++b) {
                 const uint32_t n = it + b;
                 __syncwarp();  // the warp has read the values of block n - 1 out of the slot that is filled now
                 request(b + 2);
-                cp_wait<1>();
-                if (b + 1 < blocks) publish(&inBar[(n + 1) % 3]);
+                cp_wait<2>();
                 ok = mbar_wait_bounded(&outBar[n & 1], (n >> 1) & 1, &abortFlag);
                 // base's values of block n, copied by the warp's lanes, are there for all of them; and the lanes give up together
                 if (!(ok = __all_sync(0xFFFFFFFFu, ok))) break;
+                __syncwarp();
                 tc_fence_after();
                 uint32_t acc[32];
                 tmem_ld_32x32b_x32(tmemSlot + (static_cast<uint32_t>(quarter * 32) << 16) + (n & 1) * kBlockCols + half * 32, acc);
                 uint8_t* y = sY + (n % 3) * C::kYBytes;
                 tmem_ld_wait();
+                tc_fence_before();
+                if (lane == 0) mbar_arrive(&freeBar[n & 1]);  // (all lanes have their values: the load is the warp's)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     uint4* at = reinterpret_cast<uint4*>(y + myRow * 128 + (((half * 4 + j) ^ (lane & 7)) << 4));
@@ -402,7 +398,6 @@ __global__ void __launch_bounds__(kOuterThreads, NB <= 8 ? 2 : 1) low_rank_outer
                     }
                     *at = pack8_sat<T>(f);
                 }
-                tc_fence_before();  // the next arrival on inBar lets the MMAs overwrite this accumulator
                 __syncwarp();
                 if (b * kBlockCols < moveCols) {
 #pragma unroll
@@ -415,9 +410,34 @@ __global__ void __launch_bounds__(kOuterThreads, NB <= 8 ? 2 : 1) low_rank_outer
         } else if (elect_one()) {
             constexpr uint32_t idesc = idesc_f16(kRows, kBlockCols, std::is_same<T, __half>::value ? 0 : 1);
             const int steps = (p.r + 15) / 16;
-            for (int b = 0; b < blocks; ++b) {
+            auto done = [&](uint32_t n) { return mbar_wait_bounded(&outBar[n & 1], (n >> 1) & 1, &abortFlag); };  // block n's MMAs
+            int asked = 0;  // blocks of B asked for
+            auto load_b = [&](int b) {
+                if (b >= blocks) return;
+                asked = b + 1;
+                const uint32_t s = (it + b) % 3;
+                mbar_arrive_expect_tx(&bBar[s], C::kBBytes);
+#pragma unroll
+                for (int ka = 0; ka < C::kAtoms; ++ka)
+                    tma_load_2d(sB + s * C::kBBytes + ka * kBlockCols * 128, &mapB, &bBar[s], ka * 64, adapter * p.N + col0 + b * kBlockCols);
+            };
+            if (it > 0) ok = done(it - 1);  // V and the slots of B are read no more
+            if (ok) {
+                mbar_arrive_expect_tx(&vBar, C::kVBytes);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int ka = 0; ka < C::kAtoms; ++ka) tma_load_2d(sV + (h * C::kAtoms + ka) * kAtomBytes, &mapV, &vBar, h * VP + ka * 64, start);
+                load_b(0);
+                load_b(1);
+                ok = mbar_wait_bounded(&vBar, segment & 1, &abortFlag);
+            }
+            for (int b = 0; b < blocks && ok; ++b) {
                 const uint32_t n = it + b;
-                if (!(ok = mbar_wait_bounded(&inBar[n % 3], (n / 3) & 1, &abortFlag))) break;
+                if (b > 0 && !(ok = done(n - 1))) break;
+                load_b(b + 2);
+                if (!(ok = mbar_wait_bounded(&bBar[n % 3], (n / 3) & 1, &abortFlag))) break;
+                if (n >= 2 && !(ok = mbar_wait_bounded(&freeBar[n & 1], ((n >> 1) & 1) ^ 1, &abortFlag))) break;
                 tc_fence_after();
                 const uint32_t v = smem_u32(sV), w = smem_u32(sB) + (n % 3) * C::kBBytes;
                 for (int h = 0; h < 2; ++h)
@@ -426,7 +446,12 @@ __global__ void __launch_bounds__(kOuterThreads, NB <= 8 ? 2 : 1) low_rank_outer
                                 smem_desc_sw128(w + (k >> 2) * kBlockCols * 128) + 2 * (k & 3), idesc, (h | k) != 0);
                 tc_commit(&outBar[n & 1]);
             }
+            if (!ok && asked > 0) {  // no copy may be on its way when the CTA ends
+                drain(&vBar, segment & 1);
+                for (int b = max(asked - 3, 0); b < asked; ++b) drain(&bBar[(it + b) % 3], ((it + b) / 3) & 1);
+            }
         }
+        ++segment;
         ok = __all_sync(0xFFFFFFFFu, ok);
         it += blocks;
     }
@@ -472,11 +497,22 @@ template <typename T, int NB> ascq_status launch_long(const LowRankArgs& p, cons
     // reached); a CTA keeps at least four chunks of 64
     int cluster = 8;
     while (cluster > 1 && (static_cast<uint64_t>(tiles) * cluster > (9ull * sm_count()) / 8 || p.K < cluster * 256)) cluster /= 2;
-    ASCQ_CUDA_CHECK(launch_pdl(low_rank_inner_kernel<T, NB>, dim3(tiles * cluster), kThreads, Ring<NB>::kBytes, cluster, st, p, o, cluster));
+    constexpr CUtensorMapDataType kType = CU_TENSOR_MAP_DATA_TYPE_UINT16;  // copies only
+    CUtensorMap mapA, mapB, mapV;
+    ascq_status rc = encode_2d(&mapA, kType, p.a, p.K, static_cast<uint64_t>(p.L) * p.r, static_cast<uint64_t>(p.K) * 2, 64, NB * 8, CU_TENSOR_MAP_SWIZZLE_128B,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, "A");
+    if (rc == ASCQ_OK)
+        rc = encode_2d(&mapB, kType, p.b, p.r, static_cast<uint64_t>(p.L) * p.N, static_cast<uint64_t>(p.r) * 2, 64, kBlockCols, CU_TENSOR_MAP_SWIZZLE_128B,
+                       CU_TENSOR_MAP_L2_PROMOTION_L2_128B, "B");
+    if (rc == ASCQ_OK)
+        rc = encode_2d(&mapV, kType, o.v, 2 * rank_pitch(NB), p.M, 4 * rank_pitch(NB), 64, kRows, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                       "inner products");
+    if (rc != ASCQ_OK) return rc;
+    ASCQ_CUDA_CHECK(launch_pdl(low_rank_inner_kernel<T, NB>, dim3(tiles * cluster), kThreads, Ring<NB>::kBytes, cluster, st, p, o, cluster, mapA));
     // as many CTAs of the second launch as are resident together, at most one per block of columns
     const uint64_t blocks = static_cast<uint64_t>(tiles) * ((p.N + kBlockCols - 1) / kBlockCols);
     const unsigned grid = static_cast<unsigned>(std::min<uint64_t>(blocks, static_cast<uint64_t>(sm_count()) * (NB <= 8 ? 2 : 1)));
-    ASCQ_CUDA_CHECK(launch_pdl(low_rank_outer_kernel<T, NB>, dim3(grid), kOuterThreads, Outer<NB>::kBytes, 1, st, p, o, static_cast<int>(tiles)));
+    ASCQ_CUDA_CHECK(launch_pdl(low_rank_outer_kernel<T, NB>, dim3(grid), kOuterThreads, Outer<NB>::kBytes, 1, st, p, o, static_cast<int>(tiles), mapB, mapV));
     return ASCQ_OK;
 }
 template <typename T> ascq_status launch_long_typed(const LowRankArgs& p, const LowRankScratch& o, unsigned tiles, cudaStream_t st)

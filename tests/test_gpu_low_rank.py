@@ -58,9 +58,9 @@ SHAPES = [  # m, n, k, r, adapters, tokens of a request
     (1, 8, 8, 8, 1, 1), (1, 4096, 4096, 16, 16, 1), (32, 4096, 4096, 16, 16, 1), (5, 264, 520, 8, 3, 1), (17, 1000, 72, 24, 2, 1), (16, 96, 2048, 40, 40, 1),
     (64, 512, 1024, 64, 64, 1), (200, 2048, 512, 128, 5, 33), (1024, 256, 512, 16, 1000, 1), (1025, 256, 512, 32, 1023, 1), (1337, 640, 1376, 32, 8, 97),
     (2500, 264, 136, 64, 3, 700), (3000, 520, 1032, 104, 7, 1), (1100, 4096, 256, 128, 4, 300), (4096, 1024, 1024, 64, 16, 256),
-    # tiles of 128 tokens: more than 16 million of m (n + k), a third of that for ranks above 64
-    (1500, 4104, 8200, 16, 3, 1), (2000, 8200, 72, 32, 5, 130), (4100, 4096, 264, 64, 16, 300), (1030, 200, 5000, 128, 2, 1030), (520, 5000, 5000, 104, 2, 7), (6000, 8, 2760, 8, 20, 1),
-    (2100, 8000, 8, 24, 1, 2100), (3000, 3000, 3000, 48, 4, 129)]
+    # tiles of 128 tokens: more than 20 million of m (n + k), a third of that for ranks above 64
+    (1700, 4104, 8200, 16, 3, 1), (2500, 8200, 72, 32, 5, 130), (4700, 4096, 264, 64, 16, 300), (1400, 200, 5000, 128, 2, 1030), (700, 5000, 5000, 104, 2, 7), (8000, 8, 2760, 8, 20, 1),
+    (2600, 8000, 8, 24, 1, 2100), (3500, 3000, 3000, 48, 4, 129), (1500, 8200, 6000, 40, 8, 1500)]
 
 
 @gpu
@@ -75,17 +75,17 @@ def test_against_the_formula(m, n, k, r, lo, span, dt):
 
 
 @gpu
-@pytest.mark.parametrize("m", [1, 16, 40, 1500])
-def test_one_adapter_or_none_for_all(m):
+@pytest.mark.parametrize("m,n", [(1, 136), (16, 136), (40, 136), (1500, 136), (1500, 14000)])
+def test_one_adapter_or_none_for_all(m, n):
     for value in (0, 2, -1, 3, 2 ** 31 - 1):
-        x, base, a, b, scale, ids = case(m, 136, 264, 16, 3, torch.bfloat16, ids=torch.full((m,), value))
+        x, base, a, b, scale, ids = case(m, n, 264, 16, 3, torch.bfloat16, ids=torch.full((m,), value))
         got = torch.empty_like(base)
         ops.LowRankAdd(got, base, x, a, b, ids, scale=scale)
         check(got, x, base, a, b, scale, ids)
 
 
 @gpu
-@pytest.mark.parametrize("m", [48, 1200])
+@pytest.mark.parametrize("m", [48, 1200, 27000])
 def test_in_place_pitched_rows_and_repeated_calls(m):
     x, base, a, b, scale, ids = case(m, 256, 512, 32, 6, torch.float16)
     want = torch.empty_like(base)
@@ -103,9 +103,10 @@ def test_in_place_pitched_rows_and_repeated_calls(m):
 
 
 @gpu
-def test_large_and_small_inner_products():
+@pytest.mark.parametrize("m,n", [(40, 128), (1200, 20000)])
+def test_large_and_small_inner_products(m, n):
     """Inner products beyond fp16's range and among its subnormals: the second product brings them back."""
-    x, base, a, b, scale, ids = case(40, 128, 256, 16, 2, torch.float16, ids=torch.zeros(40))
+    x, base, a, b, scale, ids = case(m, n, 256, 16, 2, torch.float16, ids=torch.zeros(m))
     for fx, fb in ((2000.0, 2.0 ** -14), (2.0 ** -14, 1000.0)):
         xs, bs = (x.float() * fx).to(torch.float16), (b.float() * fb).to(torch.float16)
         got = torch.empty_like(base)
@@ -114,8 +115,9 @@ def test_large_and_small_inner_products():
 
 
 @gpu
-def test_values_that_are_not_finite_stay_in_their_token():
-    x, base, a, b, scale, ids = case(60, 64, 128, 16, 3, torch.bfloat16)
+@pytest.mark.parametrize("m,n", [(60, 64), (1300, 16384)])
+def test_values_that_are_not_finite_stay_in_their_token(m, n):
+    x, base, a, b, scale, ids = case(m, n, 128, 16, 3, torch.bfloat16)
     want = torch.empty_like(base)
     ops.LowRankAdd(want, base, x, a, b, ids, scale=scale)
     t = int((ids >= 0).nonzero()[3])
@@ -123,7 +125,7 @@ def test_values_that_are_not_finite_stay_in_their_token():
     x2[t, 5] = float("nan")
     got = torch.empty_like(base)
     ops.LowRankAdd(got, base, x2, a, b, ids, scale=scale)
-    rest = torch.arange(60, device=DEV) != t
+    rest = torch.arange(m, device=DEV) != t
     assert torch.equal(got[rest], want[rest]) and torch.isnan(got[t]).all()
     # NaN in the input of a token without an adapter, and in an adapter that no token uses
     none = int((ids < 0).nonzero()[0])
@@ -146,7 +148,7 @@ def test_result_that_overflows_saturates():
 
 
 @gpu
-@pytest.mark.parametrize("m", [64, 1100])
+@pytest.mark.parametrize("m", [64, 1100, 27000])
 def test_other_stream_and_capture(m):
     x, base, a, b, scale, ids = case(m, 256, 512, 16, 8, torch.bfloat16)
     want = torch.empty_like(base)
