@@ -328,15 +328,30 @@ __global__ void __launch_bounds__(kOuterThreads, NB <= 8 ? 2 : 1) low_rank_outer
         const int adapter = tile.x, start = tile.y, tokens = tile.z;
         const int col0 = first * kBlockCols, colEnd = min(p.N, col0 + blocks * kBlockCols);
         if (adapter >= p.L) {
-            // tokens without an adapter: base as it is
-            if (p.base != p.dst)
-                for (int row = warp; row < tokens; row += 9) {
-                    const int64_t t = p.order[start + row];
-                    for (int col = col0 + lane * 8; col < colEnd; col += 256) {
-                        const uint4 v = p.base ? *reinterpret_cast<const uint4*>(static_cast<const T*>(p.base) + t * p.ldBase + col) : make_uint4(0u, 0u, 0u, 0u);
-                        *reinterpret_cast<uint4*>(static_cast<T*>(p.dst) + t * p.ldDst + col) = v;
+            // tokens without an adapter: base as it is, eight pieces of 16 bytes in flight per thread
+            if (p.base != p.dst) {
+                const int pieces = (colEnd - col0) / 8, all = tokens * pieces;
+                constexpr int kFlight = 8;
+                for (int i0 = threadIdx.x; i0 < all; i0 += kOuterThreads * kFlight) {
+                    uint4 v[kFlight];
+                    T* to[kFlight];
+#pragma unroll
+                    for (int u = 0; u < kFlight; ++u) {
+                        const int i = i0 + u * kOuterThreads;
+                        to[u] = nullptr;
+                        v[u] = make_uint4(0u, 0u, 0u, 0u);
+                        if (i < all) {
+                            const int64_t t = p.order[start + i / pieces];
+                            const int col = col0 + i % pieces * 8;
+                            to[u] = static_cast<T*>(p.dst) + t * p.ldDst + col;
+                            if (p.base) v[u] = __ldcs(reinterpret_cast<const uint4*>(static_cast<const T*>(p.base) + t * p.ldBase + col));
+                        }
                     }
+#pragma unroll
+                    for (int u = 0; u < kFlight; ++u)
+                        if (to[u]) __stcs(reinterpret_cast<uint4*>(to[u]), v[u]);
                 }
+            }
             continue;
         }
         if (warp < 8) {
@@ -484,19 +499,52 @@ cudaError_t launch_pdl(K kernel, dim3 grid, unsigned block, size_t smem, int clu
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+// Clusters of `size` CTAs of the first launch that are resident together (a cluster lies inside one group of SMs, and a CTA takes an SM).
+template <typename T, int NB> int resident_clusters(int size)
+{
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(size), 1, 1);
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = Ring<NB>::kBytes;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(size);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, low_rank_inner_kernel<T, NB>, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        n = 0;
+    }
+    return n;
+}
+
 template <typename T, int NB> ascq_status launch_long(const LowRankArgs& p, const LowRankScratch& o, unsigned tiles, cudaStream_t st)
 {
     static PerDeviceOnce once;
+    static std::atomic<int> resident[kMaxDevices][4];  // clusters of 1, 2, 4, 8
     const int dev = current_device();
     if (!once.done(dev)) {
         ASCQ_CUDA_CHECK(cudaFuncSetAttribute(low_rank_inner_kernel<T, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<NB>::kBytes));
         ASCQ_CUDA_CHECK(cudaFuncSetAttribute(low_rank_outer_kernel<T, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, Outer<NB>::kBytes));
+        for (int i = 0; i < 4; ++i) resident[dev][i].store(resident_clusters<T, NB>(1 << i), std::memory_order_relaxed);
         once.mark(dev);
     }
-    // K is split until there is about one CTA per SM (the ring takes most of the shared memory; the bound on the tiles is rarely
-    // reached); a CTA keeps at least four chunks of 64
-    int cluster = 8;
-    while (cluster > 1 && (static_cast<uint64_t>(tiles) * cluster > (9ull * sm_count()) / 8 || p.K < cluster * 256)) cluster /= 2;
+    // K is split over a cluster so that the waves of clusters take the least time: a wave's chunks, and about ten more for its start and its end.  How many
+    // tiles there are only the device knows; half of the adapters are taken to leave a tile partly filled.
+    const int64_t chunks = (p.K + 63) / 64, expected = p.M / kRows + std::min(p.L + 1, p.M) / 2 + 1;
+    int cluster = 1;
+    int64_t best = INT64_MAX;
+    for (int i = 0; i < 4; ++i) {
+        const int fit = resident[dev][i].load(std::memory_order_relaxed);
+        if (fit <= 0) continue;
+        const int64_t cost = (expected + fit - 1) / fit * ((chunks + (1 << i) - 1) / (1 << i) + 10);
+        if (cost < best) {
+            best = cost;
+            cluster = 1 << i;
+        }
+    }
     constexpr CUtensorMapDataType kType = CU_TENSOR_MAP_DATA_TYPE_UINT16;  // copies only
     CUtensorMap mapA, mapB, mapV;
     ascq_status rc = encode_2d(&mapA, kType, p.a, p.K, static_cast<uint64_t>(p.L) * p.r, static_cast<uint64_t>(p.K) * 2, 64, NB * 8, CU_TENSOR_MAP_SWIZZLE_128B,
