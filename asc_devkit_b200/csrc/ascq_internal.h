@@ -38,6 +38,22 @@ inline bool spans_overlap(const void* a, size_t an, const void* b, size_t bn)
     return a && b && an && bn && x < y + bn && y < x + an;
 }
 
+// The same for matrices whose rows of `width` bytes are `pitch` bytes apart.  Two of one pitch may lie in each other's gaps (column
+// slices of one buffer); of matrices of different pitches that interleave the rows are not compared, they count as overlapping.
+struct PitchedSpan {
+    const void* p;
+    size_t rows, width, pitch;
+};
+inline bool spans_overlap(const PitchedSpan& a, const PitchedSpan& b)
+{
+    if (!a.p || !b.p || !a.rows || !b.rows) return false;
+    if (!spans_overlap(a.p, (a.rows - 1) * a.pitch + a.width, b.p, (b.rows - 1) * b.pitch + b.width)) return false;
+    if (a.pitch != b.pitch || a.pitch == 0) return true;
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+    const size_t ahead = x >= y ? (x - y) % a.pitch : (a.pitch - (y - x) % a.pitch) % a.pitch;  // where a's rows begin inside b's pitch
+    return ahead < b.width || a.pitch - ahead < a.width;
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // gemm_w8a16_small.cu: the weight-only-quantised matmul for at most kW8A16SmallMaxM activation rows

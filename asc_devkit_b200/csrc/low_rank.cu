@@ -404,17 +404,17 @@ extern "C" ascq_status ascq_low_rank_add(void* dst, int64_t ldDst, const void* b
     const size_t need = ws.bytes;
     if (need && (!workspace || workspaceBytes < need)) return fail(ASCQ_ERR_INVALID_ARG, "the workspace has %zu bytes, %zu are needed", workspaceBytes, need);
     if (need && !aligned16(workspace)) return fail(ASCQ_ERR_ALIGNMENT, "the workspace must be 16-byte aligned");
-    const size_t dstBytes = ((rows - 1) * ldDst + N) * 2;
-    const void* q[7] = {x, A, B, adapterIds, scale, need ? workspace : nullptr, base};
-    const size_t b[7] = {((rows - 1) * ldX + K) * 2, static_cast<size_t>(L) * r * K * 2, static_cast<size_t>(L) * N * r * 2, rows * (idT == ASCQ_DT_I64 ? 8 : 4),
-                         scale ? static_cast<size_t>(L) * 4 : 0, need, base ? ((rows - 1) * ldBase + N) * 2 : 0};
-    for (int i = 0; i < 7; ++i) {
-        if (i == 6 && base == dst && ldBase == ldDst) continue;
-        if (spans_overlap(dst, dstBytes, q[i], b[i])) return fail(ASCQ_ERR_INVALID_ARG, "dst overlaps another tensor of the call (only base may be dst itself, with the same pitch)");
+    auto matrix = [&](const void* q, int64_t cols, int64_t ld) { return PitchedSpan{q, rows, static_cast<size_t>(cols) * 2, static_cast<size_t>(ld) * 2}; };
+    auto flat = [](const void* q, size_t bytes) { return PitchedSpan{q, 1, bytes, 0}; };
+    const PitchedSpan out = matrix(dst, N, ldDst), scratch = flat(need ? workspace : nullptr, need);
+    const PitchedSpan in[6] = {matrix(x, K, ldX), matrix(base, N, ldBase), flat(A, static_cast<size_t>(L) * r * K * 2), flat(B, static_cast<size_t>(L) * N * r * 2),
+                               flat(adapterIds, rows * (idT == ASCQ_DT_I64 ? 8 : 4)), flat(scale, static_cast<size_t>(L) * 4)};
+    for (int i = 0; i < 6; ++i) {
+        const bool same = i == 1 && base == dst && ldBase == ldDst;
+        if (!same && spans_overlap(out, in[i])) return fail(ASCQ_ERR_INVALID_ARG, "dst overlaps another tensor of the call (only base may be dst itself, with the same pitch)");
+        if (spans_overlap(scratch, in[i])) return fail(ASCQ_ERR_INVALID_ARG, "the workspace overlaps another tensor of the call");
     }
-    if (need)
-        for (int i = 0; i < 7; ++i)
-            if (i != 5 && spans_overlap(workspace, need, q[i], b[i])) return fail(ASCQ_ERR_INVALID_ARG, "the workspace overlaps another tensor of the call");
+    if (spans_overlap(scratch, out)) return fail(ASCQ_ERR_INVALID_ARG, "the workspace overlaps another tensor of the call");
 
     LowRankArgs p{};
     p.x = x; p.a = A; p.b = B; p.base = base; p.dst = dst; p.ids = adapterIds; p.scale = scale;

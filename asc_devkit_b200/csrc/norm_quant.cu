@@ -476,9 +476,6 @@ template <typename T, typename G> cudaError_t launch_norm_typed(const NormArgs& 
     }
 }
 
-// Bytes from the first element of a pitched matrix to the end of its last row
-size_t extent(uint32_t rows, uint32_t cols, int64_t ld, int size) { return (static_cast<size_t>(rows - 1) * static_cast<size_t>(ld) + cols) * size; }
-
 }  // namespace
 }  // namespace ascq
 
@@ -518,22 +515,22 @@ extern "C" ascq_status ascq_residual_rms_norm_quant(void* dst, ascq_dtype dstT, 
         return fail(ASCQ_ERR_ALIGNMENT, "a tensor is not aligned to its element type");
     // outputs overlap nothing, except that residualOut may be src or residual itself (the same matrix with the same pitch)
     const size_t elems = static_cast<size_t>(p->m) * p->n;
-    struct Span { const void* p; size_t bytes; int64_t ld; };
-    const Span in[3] = {{src, extent(p->m, p->n, a.ldSrc, es), a.ldSrc},
-                        {residual, residual ? extent(p->m, p->n, a.ldResidual, es) : 0, a.ldResidual},
-                        {gamma, static_cast<size_t>(p->n) * dtype_size(gammaT), 0}};
-    const Span out[4] = {{residualOut, residualOut ? extent(p->m, p->n, a.ldResidualOut, es) : 0, a.ldResidualOut},
-                         {normOut, normOut ? extent(p->m, p->n, a.ldNormOut, es) : 0, a.ldNormOut},
-                         {dst, a.out == kOutE2M1 ? elems / 2 : elems, 0},
-                         {scaleOut, a.out == kOutI8 ? p->m * size_t{4} : elems / 32, 0}};
+    const size_t width = static_cast<size_t>(p->n) * es, rows = p->m;
+    const PitchedSpan in[3] = {{src, rows, width, static_cast<size_t>(a.ldSrc) * es},
+                               {residual, rows, width, static_cast<size_t>(a.ldResidual) * es},
+                               {gamma, 1, static_cast<size_t>(p->n) * dtype_size(gammaT), 0}};
+    const PitchedSpan out[4] = {{residualOut, rows, width, static_cast<size_t>(a.ldResidualOut) * es},
+                                {normOut, rows, width, static_cast<size_t>(a.ldNormOut) * es},
+                                {dst, 1, a.out == kOutE2M1 ? elems / 2 : elems, 0},
+                                {scaleOut, 1, a.out == kOutI8 ? rows * 4 : elems / 32, 0}};
     for (int i = 0; i < 4; ++i) {
         for (int j = 0; j < 3; ++j) {
-            const bool same = i == 0 && j < 2 && out[i].p == in[j].p && out[i].ld == in[j].ld;
-            if (!same && spans_overlap(out[i].p, out[i].bytes, in[j].p, in[j].bytes))
+            const bool same = i == 0 && j < 2 && out[i].p == in[j].p && out[i].pitch == in[j].pitch;
+            if (!same && spans_overlap(out[i], in[j]))
                 return fail(ASCQ_ERR_INVALID_ARG, "an output overlaps an input (only residualOut may be src or residual, with the same pitch)");
         }
         for (int j = 0; j < i; ++j)
-            if (spans_overlap(out[i].p, out[i].bytes, out[j].p, out[j].bytes)) return fail(ASCQ_ERR_INVALID_ARG, "two outputs overlap");
+            if (spans_overlap(out[i], out[j])) return fail(ASCQ_ERR_INVALID_ARG, "two outputs overlap");
     }
 
     a.dst = dst; a.scaleOut = scaleOut; a.residualOut = residualOut; a.normOut = normOut;

@@ -179,11 +179,6 @@ def _launch(fn, dev: int, stream: Optional[torch.cuda.Stream], *args):
         L.check(rc)
 
 
-def _need(cond: bool, what: str):
-    if not cond:
-        raise ValueError(what)
-
-
 _MX_TARGETS = {L.DT_FP8_E4M3: 1, L.DT_FP8_E5M2: 1, L.DT_FP4X2_E2M1: 2}
 
 
@@ -197,18 +192,23 @@ def ResidualRmsNormQuant(dstTensor: torch.Tensor, scaleOut: torch.Tensor, srcTen
     ``DT_FP8_E4M3`` / ``DT_FP8_E5M2``: dst uint8 [m, n], scaleOut uint8 [m, n/32] (e8m0); ``DT_FP4X2_E2M1``: dst uint8
     [m, n/2].  ``residualOut`` takes ``h`` and ``normOut`` takes ``y`` in src's dtype; ``residualOut`` may be ``residual``
     or ``srcTensor`` itself.  src, residual, residualOut and normOut are 2-D and may have a row pitch."""
-    m, n = srcTensor.shape
+    shape, dt = srcTensor.shape, srcTensor.dtype
+    m, n = shape
     for t in (residual, residualOut, normOut):
-        _need(t is None or (t.shape == srcTensor.shape and t.dtype == srcTensor.dtype),
-              "residual, residualOut and normOut must have srcTensor's shape and dtype")
-    _need(gamma.shape == (n,), "gamma must have one element per column")
+        if t is not None and (t.dtype != dt or t.shape != shape):
+            raise ValueError("residual, residualOut and normOut must have srcTensor's shape and dtype")
+    if gamma.shape != (n,):
+        raise ValueError("gamma must have one element per column")
     if dst_dtype == L.DT_I8:
-        _need(dstTensor.dtype == torch.int8 and dstTensor.shape == (m, n), "dstTensor must be int8 of srcTensor's shape")
-        _need(scaleOut.dtype == torch.float32 and scaleOut.numel() == m, "scaleOut must hold one float per row")
+        if dstTensor.dtype != torch.int8 or dstTensor.shape != shape:
+            raise ValueError("dstTensor must be int8 of srcTensor's shape")
+        if scaleOut.dtype != torch.float32 or scaleOut.numel() != m:
+            raise ValueError("scaleOut must hold one float per row")
     elif dst_dtype in _MX_TARGETS:
-        _need(dstTensor.element_size() == 1 and dstTensor.shape == (m, n // _MX_TARGETS[dst_dtype]),
-              "dstTensor must hold one byte per code (fp4: per two codes)")
-        _need(scaleOut.element_size() == 1 and scaleOut.numel() == m * (n // 32), "scaleOut must hold one byte per 32 elements")
+        if dstTensor.element_size() != 1 or dstTensor.shape != (m, n // _MX_TARGETS[dst_dtype]):
+            raise ValueError("dstTensor must hold one byte per code (fp4: per two codes)")
+        if scaleOut.element_size() != 1 or scaleOut.numel() != m * (n // 32):
+            raise ValueError("scaleOut must hold one byte per 32 elements")
     dev = _cuda_index(srcTensor)
     (sp, ls), (rp, lr), (ro, lro), (no, lno) = _rows(srcTensor, dev), _rows(residual, dev), _rows(residualOut, dev), _rows(normOut, dev)
     _launch(L.lib().ascq_residual_rms_norm_quant, dev, stream, _whole(dstTensor, dev), dst_dtype, _whole(scaleOut, dev), ro, no, sp, rp, _whole(gamma, dev),
@@ -449,11 +449,13 @@ def ExpertSort(counts: torch.Tensor, rowOfSlot: torch.Tensor, expertIds: torch.T
     int32 / int64, usually [tokens, k]; numbers outside ``[0, counts.numel())`` get no row.  counts int64 [experts] = rows per
     expert (``counts.tolist()`` is the groupList of the grouped matmuls); rowOfSlot int32 of expertIds' shape (-1: no row); slotOfRow
     int32 with as many elements (-1 behind the last row)."""
-    n = expertIds.numel()
-    _need(counts.dtype == torch.int64 and counts.dim() == 1, "counts must be an int64 vector with one element per expert")
-    _need(rowOfSlot.dtype == torch.int32 and rowOfSlot.numel() == n, "rowOfSlot must be int32 with one element per slot")
-    _need(slotOfRow is None or (slotOfRow.dtype == torch.int32 and slotOfRow.numel() == n), "slotOfRow must be int32 with one element per slot")
-    code = _id_code(expertIds)
+    n, code = expertIds.numel(), _id_code(expertIds)
+    if counts.dtype != torch.int64 or counts.dim() != 1:
+        raise ValueError("counts must be an int64 vector with one element per expert")
+    if rowOfSlot.dtype != torch.int32 or rowOfSlot.numel() != n:
+        raise ValueError("rowOfSlot must be int32 with one element per slot")
+    if slotOfRow is not None and (slotOfRow.dtype != torch.int32 or slotOfRow.numel() != n):
+        raise ValueError("slotOfRow must be int32 with one element per slot")
     dev = _cuda_index(expertIds)
     _launch(L.lib().ascq_expert_sort, dev, stream, _whole(counts, dev), _whole(rowOfSlot, dev), _whole(slotOfRow, dev), _whole(expertIds, dev), code, n,
             counts.numel())
@@ -461,9 +463,16 @@ def ExpertSort(counts: torch.Tensor, rowOfSlot: torch.Tensor, expertIds: torch.T
 
 
 def _slots(rowOfSlot: torch.Tensor, tokens: int) -> int:
-    _need(rowOfSlot.dtype == torch.int32 and rowOfSlot.dim() == 2 and rowOfSlot.shape[0] == tokens and rowOfSlot.shape[1] > 0,
-          "rowOfSlot must be int32 [tokens, k]")
-    return rowOfSlot.shape[1]
+    if rowOfSlot.dtype == torch.int32 and rowOfSlot.dim() == 2:
+        t, k = rowOfSlot.shape
+        if t == tokens and k > 0:
+            return k
+    raise ValueError("rowOfSlot must be int32 [tokens, k]")
+
+
+def _check_weights(weights: Optional[torch.Tensor], rowOfSlot: torch.Tensor):
+    if weights is not None and (weights.dtype != torch.float32 or weights.shape != rowOfSlot.shape):
+        raise ValueError("weights must be float32 of rowOfSlot's shape")
 
 
 def ExpertDispatch(dstTensor: torch.Tensor, srcTensor: torch.Tensor, rowOfSlot: torch.Tensor, *, dstScale: Optional[torch.Tensor] = None,
@@ -472,13 +481,19 @@ def ExpertDispatch(dstTensor: torch.Tensor, srcTensor: torch.Tensor, rowOfSlot: 
     [tokens, width] of any dtype (it may have a row pitch), dst [rows, width] of the same; srcScale / dstScale, a float per
     token or a row of e8m0 scales per token, go along.  Rows that no slot names are left as they were."""
     tokens, width = srcTensor.shape
-    _need(dstTensor.dim() == 2 and dstTensor.shape[1] == width and dstTensor.dtype == srcTensor.dtype, "dstTensor must be [rows, width] of srcTensor's dtype")
-    k, rows = _slots(rowOfSlot, tokens), dstTensor.shape[0]
+    if dstTensor.dim() != 2 or dstTensor.dtype != srcTensor.dtype:
+        raise ValueError("dstTensor must be [rows, width] of srcTensor's dtype")
+    rows, dw = dstTensor.shape
+    if dw != width:
+        raise ValueError("dstTensor must be [rows, width] of srcTensor's dtype")
+    k = _slots(rowOfSlot, tokens)
     scaleBytes = 0
-    _need((dstScale is None) == (srcScale is None), "dstScale and srcScale go together")
+    if (dstScale is None) != (srcScale is None):
+        raise ValueError("dstScale and srcScale go together")
     if srcScale is not None:
-        _need(srcScale.dtype == dstScale.dtype and srcScale.shape[:1] == (tokens,) and dstScale.shape == (rows,) + tuple(srcScale.shape[1:]),
-              "srcScale must be [tokens, ...] and dstScale [rows, ...] of the same dtype")
+        ss = srcScale.shape
+        if srcScale.dtype != dstScale.dtype or ss[:1] != (tokens,) or dstScale.shape != (rows,) + tuple(ss[1:]):
+            raise ValueError("srcScale must be [tokens, ...] and dstScale [rows, ...] of the same dtype")
         scaleBytes = srcScale.numel() // tokens * srcScale.element_size() if tokens else 0
     dev = _cuda_index(srcTensor)
     sp, ld = _rows(srcTensor, dev)
@@ -492,9 +507,10 @@ def ExpertCombine(dstTensor: torch.Tensor, rows: torch.Tensor, rowOfSlot: torch.
     """Brings the experts' rows back to their tokens (``ascq_expert_combine``): ``dst[t] = sum_j weights[t, j] *
     rows[rowOfSlot[t, j]]`` in fp32.  ``weights`` fp32 [tokens, k]; without them it is the gradient of ExpertDispatch."""
     tokens, h = dstTensor.shape
-    _need(rows.dim() == 2 and rows.shape[1] == h and rows.dtype == dstTensor.dtype, "rows must be [rows, h] of dstTensor's dtype")
+    if rows.dim() != 2 or rows.shape[1] != h or rows.dtype != dstTensor.dtype:
+        raise ValueError("rows must be [rows, h] of dstTensor's dtype")
     k = _slots(rowOfSlot, tokens)
-    _need(weights is None or (weights.dtype == torch.float32 and weights.shape == rowOfSlot.shape), "weights must be float32 of rowOfSlot's shape")
+    _check_weights(weights, rowOfSlot)
     dev = _cuda_index(dstTensor)
     _launch(L.lib().ascq_expert_combine, dev, stream, _whole(dstTensor, dev), _whole(rows, dev), dtype_code(rows), _whole(rowOfSlot, dev), _whole(weights, dev),
             tokens, k, rows.shape[0], h)
@@ -506,11 +522,15 @@ def ExpertCombineGrad(gradRows: Optional[torch.Tensor], gradWeights: Optional[to
     """Gradient of ExpertCombine (``ascq_expert_combine_grad``): ``gradRows[rowOfSlot[t, j]] = weights[t, j] * gradOut[t]`` and
     ``gradWeights[t, j] = <rows[rowOfSlot[t, j]], gradOut[t]>`` (fp32, 0 for slots without a row).  Either output may be None."""
     tokens, h = gradOut.shape
-    _need(rows.dim() == 2 and rows.shape[1] == h and rows.dtype == gradOut.dtype, "rows must be [rows, h] of gradOut's dtype")
+    dt = gradOut.dtype
+    if rows.dim() != 2 or rows.shape[1] != h or rows.dtype != dt:
+        raise ValueError("rows must be [rows, h] of gradOut's dtype")
     k = _slots(rowOfSlot, tokens)
-    _need(weights is None or (weights.dtype == torch.float32 and weights.shape == rowOfSlot.shape), "weights must be float32 of rowOfSlot's shape")
-    _need(gradRows is None or (gradRows.shape == rows.shape and gradRows.dtype == rows.dtype), "gradRows must have rows' shape and dtype")
-    _need(gradWeights is None or (gradWeights.dtype == torch.float32 and gradWeights.shape == rowOfSlot.shape), "gradWeights must be float32 of rowOfSlot's shape")
+    _check_weights(weights, rowOfSlot)
+    if gradRows is not None and (gradRows.dtype != dt or gradRows.shape != rows.shape):
+        raise ValueError("gradRows must have rows' shape and dtype")
+    if gradWeights is not None and (gradWeights.dtype != torch.float32 or gradWeights.shape != rowOfSlot.shape):
+        raise ValueError("gradWeights must be float32 of rowOfSlot's shape")
     dev = _cuda_index(gradOut)
     _launch(L.lib().ascq_expert_combine_grad, dev, stream, _whole(gradRows, dev), _whole(gradWeights, dev), _whole(gradOut, dev), _whole(rows, dev),
             dtype_code(rows), _whole(rowOfSlot, dev), _whole(weights, dev), tokens, k, rows.shape[0], h)
@@ -525,12 +545,21 @@ def LowRankAdd(dstTensor: torch.Tensor, base: Optional[torch.Tensor], X: torch.T
     X [M, K], A [L, r, K], B [L, N, r], base and dst [M, N], half or bfloat16 (X, base and dst may have a row pitch); base is the
     projection's result, None for 0, or dst itself; adapterIds int32 or int64 [M]; scale fp32 [L]."""
     M, K = X.shape
-    _need(A.dim() == 3 and A.shape[2] == K and B.dim() == 3 and B.shape[0] == A.shape[0] and B.shape[2] == A.shape[1], "A must be [L, r, K] and B [L, N, r]")
-    Lo, r, N = A.shape[0], A.shape[1], B.shape[1]
-    _need(dstTensor.shape == (M, N) and (base is None or base.shape == (M, N)), "base and dstTensor must be [M, N]")
-    _need(all(t is None or t.dtype == X.dtype for t in (dstTensor, base, A, B)), "X, A, B, base and dstTensor must have one dtype")
-    _need(adapterIds.shape == (M,), "adapterIds must be [M]")
-    _need(scale is None or (scale.dtype == torch.float32 and scale.shape == (Lo,)), "scale must be float32 [L]")
+    dt = X.dtype
+    if A.dim() != 3 or B.dim() != 3:
+        raise ValueError("A must be [L, r, K] and B [L, N, r]")
+    Lo, r, Ka = A.shape
+    Lb, N, rb = B.shape
+    if Ka != K or Lb != Lo or rb != r:
+        raise ValueError("A must be [L, r, K] and B [L, N, r]")
+    if dstTensor.shape != (M, N) or (base is not None and base is not dstTensor and base.shape != (M, N)):
+        raise ValueError("base and dstTensor must be [M, N]")
+    if dstTensor.dtype != dt or A.dtype != dt or B.dtype != dt or (base is not None and base.dtype != dt):
+        raise ValueError("X, A, B, base and dstTensor must have one dtype")
+    if adapterIds.dim() != 1 or adapterIds.numel() != M:
+        raise ValueError("adapterIds must be [M]")
+    if scale is not None and (scale.dtype != torch.float32 or scale.dim() != 1 or scale.numel() != Lo):
+        raise ValueError("scale must be float32 [L]")
     code, idc = dtype_code(X), _id_code(adapterIds)
     dev = _cuda_index(X)
     if workspace is None:

@@ -103,6 +103,22 @@ def test_in_place_pitched_rows_and_repeated_calls(m):
 
 
 @gpu
+@pytest.mark.parametrize("m", [33, 3000])
+def test_slices_of_one_buffer(m):
+    """x, base and dst as column slices of one matrix."""
+    n, k = 1024, 6144
+    x, base, a, b, scale, ids = case(m, n, k, 16, 3, torch.bfloat16)
+    want = torch.empty_like(base)
+    ops.LowRankAdd(want, base, x, a, b, ids, scale=scale)
+    wide = torch.zeros(m, k + 2 * n + 8, dtype=torch.bfloat16, device=DEV)
+    xs, bs, ds = wide[:, :k], wide[:, k:k + n], wide[:, k + n:k + 2 * n]
+    xs.copy_(x)
+    bs.copy_(base)
+    ops.LowRankAdd(ds, bs, xs, a, b, ids, scale=scale)
+    assert torch.equal(ds, want) and torch.equal(xs, x) and torch.equal(bs, base) and (wide[:, -8:] == 0).all()
+
+
+@gpu
 @pytest.mark.parametrize("m,n", [(40, 128), (1200, 20000)])
 def test_large_and_small_inner_products(m, n):
     """Inner products beyond fp16's range and among its subnormals: the second product brings them back."""

@@ -127,6 +127,23 @@ def test_row_pitches(out, pitch):
 
 
 @gpu
+@pytest.mark.parametrize("n", [256, 255])
+def test_slices_of_one_buffer(n):
+    """Source, residual, sum and norm as column slices of one matrix: they lie in each other's gaps."""
+    x, r, g = inputs(17, n, torch.bfloat16)
+    want = run(x, r, g, L.DT_I8)
+    wide = torch.zeros(17, 4 * n + 8, dtype=torch.bfloat16, device=DEV)
+    xs, rs, total, norm = (wide[:, i * n:(i + 1) * n] for i in range(4))
+    xs.copy_(x)
+    rs.copy_(r)
+    dst, scale = torch.empty_like(want[0]), torch.empty_like(want[1])
+    ops.ResidualRmsNormQuant(dst, scale, xs, g, 1e-6, residual=rs, residualOut=total, normOut=norm)
+    for a, b in zip(want, (dst, scale, total, norm)):
+        assert torch.equal(a, b)
+    assert torch.equal(xs, x) and torch.equal(rs, r) and (wide[:, 4 * n:] == 0).all()
+
+
+@gpu
 @pytest.mark.parametrize("out", [L.DT_I8, L.DT_FP8_E4M3])
 def test_rows_beyond_the_registers(out):
     x, r, g = inputs(3, 16384 + 32, torch.float16)
@@ -281,6 +298,10 @@ def test_refusals():
     refuse(L.ERR_INVALID_ARG, norm=0x30000)                      # normOut on src
     refuse(L.ERR_INVALID_ARG, total=0x50000, norm=0x50080)       # two outputs
     refuse(L.ERR_INVALID_ARG, total=0x40000)                     # residualOut on gamma
+    refuse(L.ERR_INVALID_ARG, total=0x30070, lds=128, ldo=128)   # rows of 128 bytes, 256 apart: the last 16 bytes of src's
+    refuse(L.ERR_INVALID_ARG, total=0x300F0, lds=128, ldo=128)   # the first 112 of its next row
+    refuse(L.ERR_INVALID_ARG, total=0x2FF90, lds=128, ldo=128, m=300)  # begins before src, reaches into it
+    refuse(L.ERR_INVALID_ARG, total=0x30080, lds=128, ldo=192)   # another pitch
 
 
 def test_python_refusals_name_the_reason():
