@@ -189,9 +189,11 @@ def test_other_stream_and_capture(m):
 
 
 @gpu
-def test_beside_the_w8a8_projection():
-    """One decode step of a projection with adapters: int8 matmul, then the adapters on its result in place."""
-    m, n, k, r, lo = 24, 512, 1024, 16, 5
+@pytest.mark.parametrize("m,n,k", [(24, 512, 1024), (3100, 4096, 2560)])
+def test_beside_the_w8a8_projection(m, n, k):
+    """A projection with adapters, for a decode step and for prompts: int8 matmul, then the adapters on its result in place; the
+    launches of several layers follow each other without a wait."""
+    r, lo = 16, 5
     x, _, a, b, scale, ids = case(m, n, k, r, lo, torch.bfloat16)
     g = torch.ones(k, dtype=torch.bfloat16, device=DEV)
     q, qs, y = torch.empty(m, k, dtype=torch.int8, device=DEV), torch.empty(m, device=DEV), torch.empty_like(x)
@@ -204,6 +206,35 @@ def test_beside_the_w8a8_projection():
     base = c.clone()
     ops.LowRankAdd(c, c, y, a, b, ids, scale=scale)
     check(c, y, base, a, b, scale, ids)
+    layers = [torch.empty_like(c) for _ in range(6)]
+    for t in layers:
+        ops.MatmulW8A8(t, q, w, qs, ws)
+        ops.LowRankAdd(t, t, y, a, b, ids, scale=scale)
+    ops.MatmulStatus()
+    assert all(torch.equal(t, c) for t in layers)
+
+
+@gpu
+def test_two_calls_at_once_on_two_streams():
+    """Each call has its own workspace: two long ones and two short ones in flight together."""
+    big = case(3000, 4096, 3000, 32, 4, torch.float16, span=200)
+    small = case(100, 512, 1024, 16, 8, torch.float16)
+    want = []
+    for x, base, a, b, scale, ids in (big, small):
+        want.append(torch.empty_like(base))
+        ops.LowRankAdd(want[-1], base, x, a, b, ids, scale=scale)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[torch.zeros_like(w) for w in want] for _ in streams]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for s, outs in zip(streams, got):
+            for out, (x, base, a, b, scale, ids) in zip(outs, (big, small)):
+                ops.LowRankAdd(out, base, x, a, b, ids, scale=scale, stream=s)
+    torch.cuda.synchronize()
+    for outs in got:
+        for out, w in zip(outs, want):
+            assert torch.equal(out, w)
 
 
 @gpu
