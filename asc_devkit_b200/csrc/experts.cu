@@ -270,13 +270,15 @@ struct DispatchArgs {
     const int32_t* rowOfSlot;
     int64_t tokens, rows;
     int k;
-    uint32_t segments;        // of 32 * kDispatchVecs vectors in a row
+    uint32_t segments;        // of 32 * dispatch_vecs vectors in a row
 };
-constexpr int kDispatchVecs = 4;
+// accesses of a lane that are in flight together: narrow ones (rows of odd sizes) need more of them
+template <typename V> constexpr int dispatch_vecs() { return sizeof(V) == 16 ? 4 : sizeof(V) == 4 ? 8 : 16; }
 
 // A warp takes a segment of a token's row: it reads the segment once and writes it to each of the token's rows.
 template <typename V> __global__ void __launch_bounds__(256) dispatch_kernel(const DispatchArgs a)
 {
+    constexpr int kDispatchVecs = dispatch_vecs<V>();
     pdl_begin();
     const int lane = threadIdx.x & 31;
     const int64_t item = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
@@ -354,10 +356,12 @@ template <typename T, int VEC> __device__ __forceinline__ void store_f(T* p, con
     }
 }
 
-constexpr int kCombineVecs = 2;
+// vectors of a lane: 16 bytes of two, or of what a row of an odd size allows more
+template <int VEC> constexpr int combine_vecs() { return VEC >= 4 ? 2 : VEC == 2 ? 4 : 8; }
 
 template <typename T, int VEC> __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a)
 {
+    constexpr int kCombineVecs = combine_vecs<VEC>();
     pdl_begin();
     const int lane = threadIdx.x & 31;
     const int64_t item = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
@@ -409,6 +413,7 @@ constexpr int kGradRows = 4, kGradThreads = 128;
 
 template <typename T, int VEC> __global__ void __launch_bounds__(kGradThreads, 8) combine_grad_kernel(const CombineArgs a)
 {
+    constexpr int U = VEC >= 4 ? 1 : VEC == 2 ? 2 : 4;  // vectors of a thread per step: narrow ones (rows of odd sizes) need more in flight
     __shared__ float part[kGradThreads / 32][kGradRows];
     pdl_begin();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
@@ -423,33 +428,44 @@ template <typename T, int VEC> __global__ void __launch_bounds__(kGradThreads, 8
             if (r[j] >= a.rows) r[j] = -1;
             w[j] = a.weights && j0 + j < a.k ? a.weights[t * a.k + j0 + j] : 1.0f;
         }
-        for (int64_t c = static_cast<int64_t>(threadIdx.x) * VEC; c < a.h; c += static_cast<int64_t>(blockDim.x) * VEC) {
-            const Pack<T, VEC> dv = load_v<T, VEC>(dOut + c);
-            Pack<T, VEC> v[kGradRows];
-            if (a.gradWeights) {
+        const int64_t width = static_cast<int64_t>(blockDim.x) * VEC;
+        for (int64_t c0 = static_cast<int64_t>(threadIdx.x) * VEC; c0 < a.h; c0 += U * width) {
+            Pack<T, VEC> dv[U], v[U][kGradRows];
 #pragma unroll
-                for (int j = 0; j < kGradRows; ++j)
-                    if (r[j] >= 0) v[j] = load_v<T, VEC>(static_cast<const T*>(a.in) + static_cast<int64_t>(r[j]) * a.h + c);
-            }
-            float d[VEC];
+            for (int u = 0; u < U; ++u) {
+                const int64_t c = c0 + u * width;
+                if (c >= a.h) continue;
+                dv[u] = load_v<T, VEC>(dOut + c);
+                if (a.gradWeights) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) d[i] = to_f32<T>(dv.v[i]);
-            if (a.gradRows) {
-#pragma unroll
-                for (int j = 0; j < kGradRows; ++j) {
-                    if (r[j] < 0) continue;
-                    float g[VEC];
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) g[i] = __fmul_rn(w[j], d[i]);
-                    store_f<T, VEC>(static_cast<T*>(a.gradRows) + static_cast<int64_t>(r[j]) * a.h + c, g);
+                    for (int j = 0; j < kGradRows; ++j)
+                        if (r[j] >= 0) v[u][j] = load_v<T, VEC>(static_cast<const T*>(a.in) + static_cast<int64_t>(r[j]) * a.h + c);
                 }
             }
-            if (a.gradWeights) {
 #pragma unroll
-                for (int j = 0; j < kGradRows; ++j) {
-                    if (r[j] < 0) continue;
+            for (int u = 0; u < U; ++u) {
+                const int64_t c = c0 + u * width;
+                if (c >= a.h) continue;
+                float d[VEC];
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i) dot[j] = fmaf(to_f32<T>(v[j].v[i]), d[i], dot[j]);
+                for (int i = 0; i < VEC; ++i) d[i] = to_f32<T>(dv[u].v[i]);
+                if (a.gradRows) {
+#pragma unroll
+                    for (int j = 0; j < kGradRows; ++j) {
+                        if (r[j] < 0) continue;
+                        float g[VEC];
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) g[i] = __fmul_rn(w[j], d[i]);
+                        store_f<T, VEC>(static_cast<T*>(a.gradRows) + static_cast<int64_t>(r[j]) * a.h + c, g);
+                    }
+                }
+                if (a.gradWeights) {
+#pragma unroll
+                    for (int j = 0; j < kGradRows; ++j) {
+                        if (r[j] < 0) continue;
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) dot[j] = fmaf(to_f32<T>(v[u][j].v[i]), d[i], dot[j]);
+                    }
                 }
             }
         }
@@ -543,7 +559,7 @@ extern "C" ascq_status ascq_expert_dispatch(void* dst, const void* src, size_t r
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     auto run = [&](auto tag) -> ascq_status {
         using V = decltype(tag);
-        const size_t nvec = rowBytes / sizeof(V), per = 32 * kDispatchVecs;
+        const size_t nvec = rowBytes / sizeof(V), per = 32 * dispatch_vecs<V>();
         a.segments = static_cast<uint32_t>((nvec + per - 1) / per);
         const int64_t ctas = (tokens * static_cast<int64_t>(a.segments) + 7) / 8;
         if (ctas > 0x7FFFFFFFll) return fail(ASCQ_ERR_INVALID_ARG, "the rows are too long for one launch");
@@ -576,16 +592,17 @@ extern "C" ascq_status ascq_expert_combine(void* dst, const void* in, ascq_dtype
     a.out = dst; a.in = in; a.rowOfSlot = rowOfSlot; a.weights = weights; a.tokens = tokens; a.rows = rows; a.h = h; a.k = k;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     auto run = [&](auto kernel, int vec) -> ascq_status {
-        const int64_t per = 32ll * kCombineVecs * vec;
+        const int64_t per = 32ll * (vec >= 4 ? combine_vecs<8>() : vec == 2 ? combine_vecs<2>() : combine_vecs<1>()) * vec;
         a.segments = static_cast<uint32_t>((h + per - 1) / per);
         const int64_t ctas = (tokens * static_cast<int64_t>(a.segments) + 7) / 8;
         if (ctas > 0x7FFFFFFFll) return fail(ASCQ_ERR_INVALID_ARG, "the rows are too long for one launch");
         ASCQ_CUDA_CHECK(launch_rows(kernel, dim3(static_cast<unsigned>(ctas)), 256, 0, 1, st, a));
         return ASCQ_OK;
     };
-    const bool vec = all % 16 == 0;
-    if (T == ASCQ_DT_F16) return vec ? run(combine_kernel<__half, 8>, 8) : run(combine_kernel<__half, 1>, 1);
-    if (T == ASCQ_DT_BF16) return vec ? run(combine_kernel<__nv_bfloat16, 8>, 8) : run(combine_kernel<__nv_bfloat16, 1>, 1);
+    const bool vec = all % 16 == 0, even = all % 4 == 0;
+    if (T == ASCQ_DT_F16) return vec ? run(combine_kernel<__half, 8>, 8) : even ? run(combine_kernel<__half, 2>, 2) : run(combine_kernel<__half, 1>, 1);
+    if (T == ASCQ_DT_BF16)
+        return vec ? run(combine_kernel<__nv_bfloat16, 8>, 8) : even ? run(combine_kernel<__nv_bfloat16, 2>, 2) : run(combine_kernel<__nv_bfloat16, 1>, 1);
     return vec ? run(combine_kernel<float, 4>, 4) : run(combine_kernel<float, 1>, 1);
 }
 
@@ -621,8 +638,10 @@ extern "C" ascq_status ascq_expert_combine_grad(void* gradRows, float* gradWeigh
         ASCQ_CUDA_CHECK(launch_rows(kernel, dim3(static_cast<unsigned>(tokens)), block, 0, 1, st, a));
         return ASCQ_OK;
     };
-    const bool vec = all % 16 == 0;
-    if (T == ASCQ_DT_F16) return vec ? run(combine_grad_kernel<__half, 8>, 8) : run(combine_grad_kernel<__half, 1>, 1);
-    if (T == ASCQ_DT_BF16) return vec ? run(combine_grad_kernel<__nv_bfloat16, 8>, 8) : run(combine_grad_kernel<__nv_bfloat16, 1>, 1);
+    const bool vec = all % 16 == 0, even = all % 4 == 0;
+    if (T == ASCQ_DT_F16)
+        return vec ? run(combine_grad_kernel<__half, 8>, 8) : even ? run(combine_grad_kernel<__half, 2>, 2) : run(combine_grad_kernel<__half, 1>, 1);
+    if (T == ASCQ_DT_BF16)
+        return vec ? run(combine_grad_kernel<__nv_bfloat16, 8>, 8) : even ? run(combine_grad_kernel<__nv_bfloat16, 2>, 2) : run(combine_grad_kernel<__nv_bfloat16, 1>, 1);
     return vec ? run(combine_grad_kernel<float, 4>, 4) : run(combine_grad_kernel<float, 1>, 1);
 }

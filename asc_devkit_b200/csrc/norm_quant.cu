@@ -368,7 +368,79 @@ template <typename T, typename G, int OUT, int NV> __global__ void __launch_boun
     }
 }
 
-// Odd widths, unaligned tensors, rows too long for registers: one CTA per row, one element per thread and step; the second
+// int8 from widths or tensors that 16-byte vectors do not fit: a CTA holds a row as NE groups of VEC elements per thread (2 where everything is even, else 1),
+// neighbouring threads neighbouring groups, all of them requested before the first is used.  The same arithmetic.  bf16 [2048, 7167] with residual and sum: see
+// norm_any_kernel.
+template <typename T, int VEC> __device__ __forceinline__ Pack<T, VEC> load_group(const T* p)
+{
+    if constexpr (sizeof(T) * VEC >= 4) return load_pack<T, VEC, true>(p);
+    else return Pack<T, VEC>{{*p}};
+}
+template <typename T, typename G, int VEC, int NE> __global__ void __launch_bounds__(512, 2) norm_odd_kernel(const NormArgs a)
+{
+    __shared__ float2 part[16];
+    __shared__ __align__(16) RowStats stats;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const uint32_t row = blockIdx.x, groups = a.n / VEC;
+    const T* src = static_cast<const T*>(a.src) + row * a.ldSrc;
+    const T* res = a.residual ? static_cast<const T*>(a.residual) + row * a.ldResidual : nullptr;
+    const G* gamma = static_cast<const G*>(a.gamma);
+    Pack<T, VEC> xs[NE], rs[NE];
+    Pack<G, VEC> gs[NE];
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+        const uint32_t v = i * blockDim.x + threadIdx.x;
+        if (v < groups) {
+            xs[i] = load_group<T, VEC>(src + v * VEC);
+            if (res) rs[i] = load_group<T, VEC>(res + v * VEC);
+            gs[i] = load_group<G, VEC>(gamma + v * VEC);
+        }
+    }
+    float h[NE][VEC], sum = 0.f, mx = 0.f;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+        const uint32_t v = i * blockDim.x + threadIdx.x;
+        if (v < groups) {
+            Pack<T, VEC> total;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                h[i][j] = to_f32<T>(xs[i].v[j]);
+                if (res) h[i][j] = __fadd_rn(h[i][j], to_f32<T>(rs[i].v[j]));
+                total.v[j] = narrow<T>(h[i][j]);
+                sum = fmaf(h[i][j], h[i][j], sum);
+                h[i][j] = __fmul_rn(h[i][j], to_f32<G>(gs[i].v[j]));  // from here on h * gamma
+                mx = max_abs3(mx, h[i][j], 0.f);
+            }
+            if (a.residualOut) *reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(a.residualOut) + row * a.ldResidualOut + v * VEC) = total;
+        }
+    }
+    const RowStats st = row_stats(sum, mx, part, &stats, static_cast<float>(a.n), a.epsilon);
+    const float rstd = st.rstd, top = __fmul_rn(st.mx, rstd);
+    const bool ok = finite_f32(st.mx) && finite_f32(top);
+    const I8Factor f = i8_factor(st.mx);
+    if (threadIdx.x == 0) static_cast<float*>(a.scaleOut)[row] = !ok ? __int_as_float(0x7FFFFFFF) : st.mx > 0.f ? __fdiv_rn(top, 127.0f) : 1.0f;
+    int8_t* dst = static_cast<int8_t*>(a.dst) + static_cast<size_t>(row) * a.n;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+        const uint32_t v = i * blockDim.x + threadIdx.x;
+        if (v >= groups) continue;
+        if (a.normOut) {
+            Pack<T, VEC> y;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) y.v[j] = narrow<T>(__fmul_rn(h[i][j], rstd));
+            *reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(a.normOut) + row * a.ldNormOut + v * VEC) = y;
+        }
+        float q[4] = {};
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) q[j] = __fmul_rn(f.pre != 1.0f ? h[i][j] * f.pre : h[i][j], f.mul);
+        const uint32_t codes = ok ? pack_i8x4_rni(q[0], q[1], q[2], q[3]) : 0u;
+        if constexpr (VEC == 2) *reinterpret_cast<unsigned short*>(dst + v * 2) = static_cast<unsigned short>(codes);
+        else dst[v] = static_cast<int8_t>(codes & 0xFFu);
+    }
+}
+
+// MX codes from unaligned tensors, rows too long for registers: one CTA per row, one element per thread and step; the second
 // pass computes h again from the sources (a row is in L2).  The same arithmetic.
 template <typename T, typename G> __global__ void __launch_bounds__(256) norm_any_kernel(const NormArgs a)
 {
@@ -465,8 +537,17 @@ template <typename T, typename G, int OUT> cudaError_t launch_norm_rows(const No
     return launch_norm(norm_rows_kernel<T, G, OUT, 4>, grid, block, st, a);
 }
 
-template <typename T, typename G> cudaError_t launch_norm_typed(const NormArgs& a, bool vec, cudaStream_t st)
+template <typename T, typename G, int VEC> cudaError_t launch_norm_odd(const NormArgs& a, cudaStream_t st)
 {
+    const uint32_t groups = (a.n + VEC - 1) / VEC;
+    if (groups <= 256 * 4) return launch_norm(norm_odd_kernel<T, G, VEC, 4>, a.m, std::max((groups + 3) / 4 + 31, 32u) / 32 * 32, st, a);
+    if (groups <= 256 * 8) return launch_norm(norm_odd_kernel<T, G, VEC, 8>, a.m, 256, st, a);
+    return launch_norm(norm_odd_kernel<T, G, VEC, 16>, a.m, groups <= 256 * 16 ? 256 : 512, st, a);
+}
+
+template <typename T, typename G> cudaError_t launch_norm_typed(const NormArgs& a, bool vec, bool even, cudaStream_t st)
+{
+    if (!vec && a.out == kOutI8 && a.n <= 512 * 16 * (even ? 2 : 1)) return even ? launch_norm_odd<T, G, 2>(a, st) : launch_norm_odd<T, G, 1>(a, st);
     if (!vec) return launch_norm(norm_any_kernel<T, G>, a.m, 256, st, a);
     switch (a.out) {
         case kOutI8: return launch_norm_rows<T, G, kOutI8>(a, st);
@@ -540,10 +621,14 @@ extern "C" ascq_status ascq_residual_rms_norm_quant(void* dst, ascq_dtype dstT, 
     const bool vec = p->n % 8 == 0 && p->n / 8 <= kNormThreads * kNormMaxVectors && !bad(src, 16) && !bad(residual, 16) && !bad(residualOut, 16) &&
                      !bad(normOut, 16) && !bad(gamma, 16) && !bad(dst, a.out == kOutE2M1 ? 4 : 8) && a.ldSrc * es % 16 == 0 &&
                      (!residual || a.ldResidual * es % 16 == 0) && (!residualOut || a.ldResidualOut * es % 16 == 0) && (!normOut || a.ldNormOut * es % 16 == 0);
+    const int e2 = 2 * es;  // pairs of elements, everywhere
+    const bool even = p->n % 2 == 0 && !bad(src, e2) && !bad(residual, e2) && !bad(residualOut, e2) && !bad(normOut, e2) && !bad(gamma, 2 * dtype_size(gammaT)) &&
+                      !bad(dst, 2) && a.ldSrc % 2 == 0 && (!residual || a.ldResidual % 2 == 0) && (!residualOut || a.ldResidualOut % 2 == 0) &&
+                      (!normOut || a.ldNormOut % 2 == 0);
     cudaError_t rc;
-    if (srcT == ASCQ_DT_F16) rc = gammaT == srcT ? launch_norm_typed<__half, __half>(a, vec, st) : launch_norm_typed<__half, float>(a, vec, st);
-    else if (srcT == ASCQ_DT_BF16) rc = gammaT == srcT ? launch_norm_typed<__nv_bfloat16, __nv_bfloat16>(a, vec, st) : launch_norm_typed<__nv_bfloat16, float>(a, vec, st);
-    else rc = launch_norm_typed<float, float>(a, vec, st);
+    if (srcT == ASCQ_DT_F16) rc = gammaT == srcT ? launch_norm_typed<__half, __half>(a, vec, even, st) : launch_norm_typed<__half, float>(a, vec, even, st);
+    else if (srcT == ASCQ_DT_BF16) rc = gammaT == srcT ? launch_norm_typed<__nv_bfloat16, __nv_bfloat16>(a, vec, even, st) : launch_norm_typed<__nv_bfloat16, float>(a, vec, even, st);
+    else rc = launch_norm_typed<float, float>(a, vec, even, st);
     ASCQ_CUDA_CHECK(rc);
     return ASCQ_OK;
 }

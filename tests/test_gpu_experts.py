@@ -171,7 +171,7 @@ def plain_combine(rows, ros, w):
     return out, mag
 
 
-SHAPES = [(1, 1, 1, 1), (1, 8, 256, 7168), (16, 8, 64, 2048), (33, 3, 7, 77), (6, 40, 64, 264), (500, 4, 16, 1032), (130, 9, 20, 4104), (20, 2, 4, 9000)]
+SHAPES = [(1, 1, 1, 1), (50, 4, 8, 2046), (9, 3, 5, 34), (1, 8, 256, 7168), (16, 8, 64, 2048), (33, 3, 7, 77), (6, 40, 64, 264), (500, 4, 16, 1032), (130, 9, 20, 4104), (20, 2, 4, 9000)]
 
 
 @gpu

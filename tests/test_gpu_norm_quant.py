@@ -111,7 +111,7 @@ def test_vector_kernel(m, n, dt, out):
 
 @gpu
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("m,n", [(1, 1), (4, 7), (3, 255), (2, 4097), (5, 20000)])
+@pytest.mark.parametrize("m,n", [(1, 1), (4, 7), (3, 255), (2, 4097), (5, 20000), (1, 2), (40, 1022), (3, 2049), (2, 8191), (2, 8194), (3, 16382), (1, 16385)])
 def test_odd_widths_to_int8(m, n, dt):
     x, r, g = inputs(m, n, dt)
     check(x, r, g, L.DT_I8, run(x, r, g, L.DT_I8))
