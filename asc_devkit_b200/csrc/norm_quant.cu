@@ -369,8 +369,8 @@ template <typename T, typename G, int OUT, int NV> __global__ void __launch_boun
 }
 
 // int8 from widths or tensors that 16-byte vectors do not fit: a CTA holds a row as NE groups of VEC elements per thread (2 where everything is even, else 1),
-// neighbouring threads neighbouring groups, all of them requested before the first is used.  The same arithmetic.  bf16 [2048, 7167] with residual and sum: see
-// norm_any_kernel.
+// neighbouring threads neighbouring groups, all of them requested before the first is used.  The same arithmetic.  bf16 with residual and sum: [2048, 7167] 46 us
+// (62 us an element at a time in two passes; [2048, 7168] takes 17.6 us on vectors), [4096, 1023] 14 us (20.5; 7.7), [4096, 1022] 10.4 us.
 template <typename T, int VEC> __device__ __forceinline__ Pack<T, VEC> load_group(const T* p)
 {
     if constexpr (sizeof(T) * VEC >= 4) return load_pack<T, VEC, true>(p);
@@ -540,14 +540,15 @@ template <typename T, typename G, int OUT> cudaError_t launch_norm_rows(const No
 template <typename T, typename G, int VEC> cudaError_t launch_norm_odd(const NormArgs& a, cudaStream_t st)
 {
     const uint32_t groups = (a.n + VEC - 1) / VEC;
-    if (groups <= 256 * 4) return launch_norm(norm_odd_kernel<T, G, VEC, 4>, a.m, std::max((groups + 3) / 4 + 31, 32u) / 32 * 32, st, a);
-    if (groups <= 256 * 8) return launch_norm(norm_odd_kernel<T, G, VEC, 8>, a.m, 256, st, a);
-    return launch_norm(norm_odd_kernel<T, G, VEC, 16>, a.m, groups <= 256 * 16 ? 256 : 512, st, a);
+    if (groups <= 512 * 4) return launch_norm(norm_odd_kernel<T, G, VEC, 4>, a.m, std::max((groups + 3) / 4 + 31, 32u) / 32 * 32, st, a);
+    if (groups <= 512 * 8) return launch_norm(norm_odd_kernel<T, G, VEC, 8>, a.m, (groups + 7) / 8 / 32 * 32 + 32 <= 512 ? (groups + 7) / 8 / 32 * 32 + 32 : 512, st, a);
+    if constexpr (VEC == 1) return launch_norm(norm_odd_kernel<T, G, 1, 16>, a.m, 512, st, a);
+    else return cudaErrorInvalidValue;  // (the caller's limit is 512 * 8 pairs)
 }
 
 template <typename T, typename G> cudaError_t launch_norm_typed(const NormArgs& a, bool vec, bool even, cudaStream_t st)
 {
-    if (!vec && a.out == kOutI8 && a.n <= 512 * 16 * (even ? 2 : 1)) return even ? launch_norm_odd<T, G, 2>(a, st) : launch_norm_odd<T, G, 1>(a, st);
+    if (!vec && a.out == kOutI8 && a.n <= 512 * 16) return even ? launch_norm_odd<T, G, 2>(a, st) : launch_norm_odd<T, G, 1>(a, st);
     if (!vec) return launch_norm(norm_any_kernel<T, G>, a.m, 256, st, a);
     switch (a.out) {
         case kOutI8: return launch_norm_rows<T, G, kOutI8>(a, st);
