@@ -47,6 +47,7 @@ __device__ __forceinline__ void pdl_begin()
 // run.  One launch, no scratch memory, and the order of equal keys is the slots' own.
 // What bounds it is latency (the slots themselves are a few hundred KB): a warp's numbers are all requested at the start and keys and
 // ranks stay in registers (HELD steps of 32 slots).  Longer runs (HELD = 0) count first and walk over the slots a second time.
+// 128 slots of 256 experts 2.5 us, 65536 slots of 128 experts 10 us.
 template <typename Id> __device__ __forceinline__ int sort_key(const Id* ids, int64_t s, int64_t end, int keys, int outside)
 {
     if (s >= end) return -1;
@@ -275,7 +276,8 @@ struct DispatchArgs {
 // accesses of a lane that are in flight together: narrow ones (rows of odd sizes) need more of them
 template <typename V> constexpr int dispatch_vecs() { return sizeof(V) == 16 ? 4 : sizeof(V) == 4 ? 8 : 16; }
 
-// A warp takes a segment of a token's row: it reads the segment once and writes it to each of the token's rows.
+// A warp takes a segment of a token's row: it reads the segment once and writes it to each of the token's rows.  What bounds it is HBM's
+// write side: 8192 tokens x 8 int8 rows of 7168 bytes in 84 us = 6.3 TB/s of 0.53 GB.
 template <typename V> __global__ void __launch_bounds__(256) dispatch_kernel(const DispatchArgs a)
 {
     constexpr int kDispatchVecs = dispatch_vecs<V>();
@@ -359,6 +361,8 @@ template <typename T, int VEC> __device__ __forceinline__ void store_f(T* p, con
 // vectors of a lane: 16 bytes of two, or of what a row of an odd size allows more
 template <int VEC> constexpr int combine_vecs() { return VEC >= 4 ? 2 : VEC == 2 ? 4 : 8; }
 
+// A warp takes a segment of a token's output and adds up the token's rows, four rows requested at a time.  HBM bound: 8192 tokens x 8 rows of 7168
+// bf16 in 171 us = 6.2 TB/s of 1.06 GB.
 template <typename T, int VEC> __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a)
 {
     constexpr int kCombineVecs = combine_vecs<VEC>();

@@ -5,10 +5,14 @@
 // What bounds it: x, base and dst cross HBM once (2 (K + 2 N) bytes a token), each used adapter once (2 r (K + N) bytes); with ranks up to
 // 128 the products stay below what the tensor cores do in that time.  So the tokens are grouped by adapter -- a tile is up to 16 tokens
 // of one adapter -- and both products of a tile run in one launch: a cluster of CTAs splits K for the first, adds its
-// partial sums through distributed shared memory, and splits N for the second.  The [16, r] inner product never leaves the SMs.
+// partial sums through distributed shared memory, and splits N for the second.  The [16, r] inner product never leaves the SMs.  Up to 1024
+// tokens nothing else is launched: every CTA finds its tile in the adapter numbers (4 KB).  32 tokens of 16 adapters, 4096 x 4096, rank 16: 7.1 us,
+// of which the 5 MB are 0.8 us; the rest is the chain from adapter number to token, to x and A, across the cluster, to dst.
 //
 // Both operands of the MMAs come straight from global memory: a dot product does not care in which order k is visited, so a
 // lane's 16 consecutive bytes of a row serve as the fragments of two m16n8k16 MMAs.
+//
+// Calls with enough tokens per adapter take another form, low_rank_long.cu.
 //
 // The inner product is a sum in fp32; for the second product it is split into two 16-bit terms, hi = cast(v), lo = cast(v - hi), after
 // each token's row was brought to [512, 1024) by a power of two (so that neither fp16's range nor its subnormals matter).  What the split drops is below
