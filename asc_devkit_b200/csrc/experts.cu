@@ -414,7 +414,6 @@ template <typename T, int VEC> __global__ void __launch_bounds__(256) combine_ke
 // and 40, 196 with 4 rows and 80, 249 with 8 rows and 120; CTAs of 128 threads rather than 256 (193 us) or 64 (198 us).
 constexpr int kGradRows = 4, kGradThreads = 128;
 
-
 template <typename T, int VEC> __global__ void __launch_bounds__(kGradThreads, 8) combine_grad_kernel(const CombineArgs a)
 {
     constexpr int U = VEC >= 4 ? 1 : VEC == 2 ? 2 : 4;  // vectors of a thread per step: narrow ones (rows of odd sizes) need more in flight
@@ -545,9 +544,10 @@ extern "C" ascq_status ascq_expert_dispatch(void* dst, const void* src, size_t r
     if (ldSrcBytes == 0) ldSrcBytes = rowBytes;
     if (ldSrcBytes < rowBytes) return fail(ASCQ_ERR_INVALID_ARG, "the row pitch of src is smaller than its rows");
     if ((dstScale == nullptr) != (srcScale == nullptr)) return fail(ASCQ_ERR_INVALID_ARG, "dstScale and srcScale must both be given or both be NULL");
-    if (rowBytes > (size_t{1} << 40) || ldSrcBytes > (size_t{1} << 40) || scaleRowBytes > (size_t{1} << 40)) return fail(ASCQ_ERR_INVALID_ARG, "a row is longer than 2^40 bytes");
-    if (tokens == 0 || rows == 0 || rowBytes == 0) return ASCQ_OK;
-    if (!dst || !src || !rowOfSlot) return fail(ASCQ_ERR_INVALID_ARG, "dst, src and rowOfSlot must not be NULL");
+    constexpr size_t kMost = size_t{1} << 32;  // 2^31 rows of it are below 2^64
+    if (rowBytes > kMost || ldSrcBytes > kMost || scaleRowBytes > kMost) return fail(ASCQ_ERR_INVALID_ARG, "a row or its pitch is longer than 2^32 bytes");
+    if (tokens == 0 || rows == 0 || (rowBytes == 0 && !dstScale)) return ASCQ_OK;
+    if ((rowBytes && (!dst || !src)) || !rowOfSlot) return fail(ASCQ_ERR_INVALID_ARG, "dst, src and rowOfSlot must not be NULL");
     if (dstScale && scaleRowBytes == 0) return fail(ASCQ_ERR_INVALID_ARG, "scaleRowBytes must be positive when scales are given");
     const size_t T = static_cast<size_t>(tokens), R = static_cast<size_t>(rows);
     const void* p[5] = {dst, dstScale, src, srcScale, rowOfSlot};
@@ -564,7 +564,7 @@ extern "C" ascq_status ascq_expert_dispatch(void* dst, const void* src, size_t r
     auto run = [&](auto tag) -> ascq_status {
         using V = decltype(tag);
         const size_t nvec = rowBytes / sizeof(V), per = 32 * dispatch_vecs<V>();
-        a.segments = static_cast<uint32_t>((nvec + per - 1) / per);
+        a.segments = std::max(static_cast<uint32_t>((nvec + per - 1) / per), 1u);  // the first one takes the scales, which empty rows may have too
         const int64_t ctas = (tokens * static_cast<int64_t>(a.segments) + 7) / 8;
         if (ctas > 0x7FFFFFFFll) return fail(ASCQ_ERR_INVALID_ARG, "the rows are too long for one launch");
         ASCQ_CUDA_CHECK(launch_rows(dispatch_kernel<V>, dim3(static_cast<unsigned>(ctas)), 256, 0, 1, st, a));

@@ -146,6 +146,24 @@ def test_dispatch_into_fewer_rows_than_the_slots_name():
 
 
 # ---- combine and its gradient -----------------------------------------------------------------------------------------
+@gpu
+def test_dispatch_of_scales_beside_empty_rows():
+    ids = route(37, 3, 8, outside=0.2, dtype=torch.int32).to(DEV)
+    counts, ros, _ = sort(ids, 8)
+    scale, got = torch.rand(37, device=DEV), torch.full((37 * 3,), 5.0, device=DEV)
+    ops.ExpertDispatch(torch.zeros(37 * 3, 0, dtype=torch.int8, device=DEV), torch.zeros(37, 0, dtype=torch.int8, device=DEV), ros, dstScale=got, srcScale=scale)
+    want = torch.full_like(got, 5.0)
+    named = ros >= 0
+    want[ros[named].long()] = scale[:, None].expand(37, 3)[named]
+    assert torch.equal(got, want)
+
+
+def test_dispatch_rows_whose_span_would_not_fit_64_bits():
+    st = L.lib().ascq_expert_dispatch(P(0x100000), P(0x200000), 1 << 34, 0, None, None, 0, P(0x300000), 4, 2, (1 << 31) - 1, None)
+    assert st == L.ERR_INVALID_ARG
+    assert b"2^32" in L.lib().ascq_last_error()
+
+
 def experts_case(t, k, e, h, dt, outside=0.0, seed=0):
     g = torch.Generator().manual_seed(seed + t + h)
     ids = route(t, k, e, outside=outside)
