@@ -28,6 +28,7 @@ namespace ascq {
 namespace {
 
 constexpr int kMaxRank = 128;
+constexpr int kMaxWidth = 1 << 30;  // of N and K: column indices and a step of the whole cluster beyond them stay below 2^31
 constexpr int kTile = 16;         // tokens of one adapter that share a tile
 constexpr int kWarps = 8;
 constexpr int kInlineTokens = 1024;  // up to here every CTA finds its tile in the adapter numbers itself; beyond, they are sorted first
@@ -390,6 +391,7 @@ extern "C" ascq_status ascq_low_rank_add(void* dst, int64_t ldDst, const void* b
     if (T != ASCQ_DT_F16 && T != ASCQ_DT_BF16) return fail(ASCQ_ERR_UNSUPPORTED, "x, A, B, base and dst must be half or bfloat16_t");
     if (idT != ASCQ_DT_I32 && idT != ASCQ_DT_I64) return fail(ASCQ_ERR_UNSUPPORTED, "adapterIds must be int32 or int64");
     if (M < 0 || N < 0 || K <= 0) return fail(ASCQ_ERR_INVALID_ARG, "M and N must not be negative and K must be positive");
+    if (N > kMaxWidth || K > kMaxWidth) return fail(ASCQ_ERR_INVALID_ARG, "N is %d and K is %d, which must be at most 2^30", N, K);
     if (N % 8 != 0 || K % 8 != 0) return fail(ASCQ_ERR_INVALID_ARG, "N is %d and K is %d, which must be multiples of 8", N, K);
     if (r <= 0 || r > kMaxRank || r % 8 != 0) return fail(ASCQ_ERR_INVALID_ARG, "the rank is %d, which must be a multiple of 8 up to %d", r, kMaxRank);
     if (L < 1 || L >= kMaxSortKeys) return fail(ASCQ_ERR_INVALID_ARG, "the number of adapters is %d, which must be in [1, %d]", L, kMaxSortKeys - 1);

@@ -498,7 +498,7 @@ ascq_status ascq_matmul_w4a16(void* C, ascq_dtype cT, const void* A, ascq_dtype 
  * x [M, K], A [L, r, K], B [L, N, r], base and dst [M, N] of T = half or bfloat16_t (row pitches ldX, ldBase, ldDst in elements, 0 =
  * contiguous; A and B contiguous), adapterIds [M] of idT = int32 or int64 in any order, scale fp32 [L] or NULL (1).  A token whose number is
  * outside [0, L) keeps base[t]; one whose inner product is not finite gets values that are not finite.  base may be dst itself (same pitch) or NULL (0).  Both products accumulate in fp32 and the inner one is not
- * rounded to T in between.  N % 8 == 0, K % 8 == 0, r % 8 == 0, r <= 128, L <= 1023; tensors 16-byte aligned.
+ * rounded to T in between.  N % 8 == 0, K % 8 == 0, both at most 2^30, r % 8 == 0, r <= 128, L <= 1023; tensors 16-byte aligned.
  * workspace: ascq_low_rank_add_workspace_size(M, N, K, r, L) bytes (0 for small calls), 16-byte aligned, private to this call until the
  * stream reaches the end of it.
  */

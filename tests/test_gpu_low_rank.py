@@ -267,6 +267,14 @@ def test_refusals():
     assert size(512, 11008, 4096, 128, 3) > 0 and size(512, 11008, 4096, 64, 3) == 0
 
 
+@pytest.mark.parametrize("n,k", [((1 << 30) + 8, 64), (64, (1 << 30) + 8), ((1 << 31) - 8, (1 << 31) - 8)])
+def test_widths_whose_indices_would_wrap(n, k):
+    # the second check that such a call meets is the one of dst: NULL here, so that no build launches it
+    st = L.lib().ascq_low_rank_add(None, 0, None, 0, None, 0, None, None, L.DT_BF16, None, L.DT_I32, None, 4, n, k, 16, 3, None, 0, None)
+    assert st == L.ERR_INVALID_ARG
+    assert b"2^30" in L.lib().ascq_last_error()
+
+
 def test_python_refusals():
     z = lambda *s: torch.zeros(*s, dtype=torch.float16)  # noqa: E731
     ids = torch.zeros(4, dtype=torch.int32)
