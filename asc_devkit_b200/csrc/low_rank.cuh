@@ -119,13 +119,14 @@ __device__ __forceinline__ int range_shift(float top)
     return ex == 0 || ex == 255 ? 0 : min(max(ex - 136, -126), 126);
 }
 __device__ __forceinline__ float exp2_int(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
-// v as two 16-bit terms: x = cast(v), y = cast(v - x); 0 for the second where the first is not finite
+// v as two 16-bit terms: x = cast(v), y = cast(v - x); 0 for the second where the first is not finite.  The casts saturate: beside an
+// infinity a row keeps its range, and what is finite in it must not become an infinity of the other sign.
 template <typename T> __device__ __forceinline__ uint2 split16(float v)
 {
     uint2 r;
-    r.x = pack2<T>(v, 0.f) & 0xFFFFu;
+    r.x = pack_sat<T>(v, 0.f) & 0xFFFFu;
     const float back = unpack2<T>(r.x).x;
-    r.y = fabsf(back) <= 3.4028234663852886e38f ? pack2<T>(v - back, 0.f) & 0xFFFFu : 0u;
+    r.y = fabsf(back) <= 3.4028234663852886e38f ? pack_sat<T>(v - back, 0.f) & 0xFFFFu : 0u;
     return r;
 }
 

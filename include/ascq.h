@@ -180,8 +180,9 @@ ascq_status ascq_dynamic_quant_mxfp4(uint8_t* dst_fp4, uint8_t* scale_e8m0, cons
  * All arithmetic and both sums in fp32.  src, residual, residualOut, normOut have type srcT (half, bfloat16_t or float) and
  * their own row pitches; gamma [n] has srcT or float; dst and scaleOut are contiguous.  A row whose sum of squares or
  * largest |y| is not finite in fp32 (NaN, infinity, |h| beyond 1e19) gets scale NaN and codes 0 (MX: a block with such a y gets
- * scale byte 0xFF and codes 0); residualOut is written as ever.  residualOut may be src or residual itself (same pitch); no other overlap is allowed.  Any n for int8,
- * n % 32 == 0 for the MX types; unaligned tensors and rows beyond 16384 elements take a slower kernel.
+ * scale byte 0xFF and codes 0); residualOut is written as ever.  residualOut may be src or residual itself (same pitch); no
+ * other overlap is allowed.  Any n for int8, n % 32 == 0 for the MX types; unaligned tensors and rows beyond 16384 elements
+ * take slower kernels.
  */
 typedef struct ascq_rms_norm_param {
     uint32_t m, n;        /* rows (tokens), elements of a row */
@@ -496,9 +497,11 @@ ascq_status ascq_matmul_w4a16(void* C, ascq_dtype cT, const void* A, ascq_dtype 
  * the product with its own adapter to the projection's result (ascq_matmul_w8a8, _w8a16, _f16 ...).
  *   dst[t] = cast(base[t] + scale[a] * (x[t] . A[a]^T) . B[a]^T),   a = adapterIds[t]
  * x [M, K], A [L, r, K], B [L, N, r], base and dst [M, N] of T = half or bfloat16_t (row pitches ldX, ldBase, ldDst in elements, 0 =
- * contiguous; A and B contiguous), adapterIds [M] of idT = int32 or int64 in any order, scale fp32 [L] or NULL (1).  A token whose number is
- * outside [0, L) keeps base[t]; one whose inner product is not finite gets values that are not finite.  base may be dst itself (same pitch) or NULL (0).  Both products accumulate in fp32 and the inner one is not
- * rounded to T in between.  N % 8 == 0, K % 8 == 0, both at most 2^30, r % 8 == 0, r <= 128, L <= 1023; tensors 16-byte aligned.
+ * contiguous; A and B contiguous), adapterIds [M] of idT = int32 or int64 in any order, scale fp32 [L] or NULL (1).  A token
+ * whose number is outside [0, L) keeps base[t].  Values that are not finite reach only the tokens of their own x row or
+ * adapter, and come out as values that are not finite (an infinity in B may come out as NaN).  base may be dst itself (same
+ * pitch) or NULL (0).  Both products accumulate in fp32 and the inner one is not rounded to T in between.
+ * N % 8 == 0, K % 8 == 0, both at most 2^30, r % 8 == 0, r <= 128, L <= 1023; tensors 16-byte aligned.
  * workspace: ascq_low_rank_add_workspace_size(M, N, K, r, L) bytes (0 for small calls), 16-byte aligned, private to this call until the
  * stream reaches the end of it.
  */

@@ -155,6 +155,20 @@ def test_values_that_are_not_finite_stay_in_their_token(m, n):
 
 
 @gpu
+@pytest.mark.parametrize("m,n", [(20, 64), (1300, 16384)])
+def test_infinite_inner_product_beside_large_finite_ones(m, n):
+    x = torch.zeros(m, 64, dtype=torch.float16, device=DEV)
+    x[:, :2], x[:, 5] = 30000.0, 1.0
+    a = torch.zeros(1, 16, 64, dtype=torch.float16, device=DEV)
+    a[0, 0, 5] = float("inf")
+    a[0, 1, :2] = -60000.0  # an inner product of -3.6e9
+    b = torch.ones(1, n, 16, dtype=torch.float16, device=DEV)
+    got = torch.zeros(m, n, dtype=torch.float16, device=DEV)
+    ops.LowRankAdd(got, None, x, a, b, torch.zeros(m, dtype=torch.int32, device=DEV))
+    assert (got == float("inf")).all()
+
+
+@gpu
 def test_result_that_overflows_saturates():
     x = torch.full((2, 8), 100.0, dtype=torch.float16, device=DEV)
     a, b = torch.full((1, 8, 8), 10.0, dtype=torch.float16, device=DEV), torch.full((1, 8, 8), 10.0, dtype=torch.float16, device=DEV)
