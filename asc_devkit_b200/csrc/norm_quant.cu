@@ -8,8 +8,8 @@
 //
 // What bounds it: HBM.  With bf16 tensors and residualOut an element costs 2 + 2 bytes read, 2 + 1 written.  A CTA owns whole rows and
 // keeps a row in registers between the reduction and the quantisation, so each byte moves once; the next row is requested before the
-// reduction.  bf16 [16384, 7168] to e4m3: 135 us = 6.1 TB/s, 0.95 of the measured copy rate (164 us without the early request).  For int8 the row's
-// maximum needs no second reduction: max|y| = rstd * max|h * gamma|, so sum(h^2) and max|h * gamma| go through the same
+// reduction.  bf16 [16384, 7168] to e4m3: 143 us = 5.8 TB/s, 0.90 of the measured copy rate (134 us without the look at ties;
+// before that, 164 without the early request).  For int8 the row's maximum needs no second reduction: max|y| = rstd * max|h * gamma|, so sum(h^2) and max|h * gamma| go through the same
 // shuffles and the same barrier, and RINT(y * 127 / max|y|) = RINT((h * gamma) * (127 / max|h * gamma|)) does not need rstd.
 #include "elementwise.cuh"
 
@@ -70,7 +70,7 @@ template <typename T> __device__ __forceinline__ Vec8<T> load8(const T* p)
 {
     Vec8<T> v;
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) v.w[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) v.w[i] = __ldcg(reinterpret_cast<const uint4*>(p) + i);
     return v;
 }
 template <typename T> __device__ __forceinline__ void widen8(const Vec8<T>& v, float (&f)[8])
@@ -100,22 +100,23 @@ template <typename T> __device__ __forceinline__ T narrow(float f)
     else if constexpr (std::is_same<T, __half>::value) return f32_to_f16_sat(f);
     else return f32_to_bf16_sat(f);
 }
-// the framework's narrowing rule: round to nearest even, a finite value that overflows saturates.  `top`: the largest of the magnitudes
-// (NaN if there is one); only a vector that holds something beyond the type's largest value is looked at element by element.
-template <typename T> __device__ __forceinline__ void store8(T* p, const float (&f)[8], float top)
+// Squares up to here come from values that T holds; fp32's own largest where the square would overflow.
+template <typename T> constexpr float kMostSquaredOf = std::is_same<T, __half>::value ? 65504.0f * 65504.0f : 3.4028234663852886e38f;
+// the framework's narrowing rule: round to nearest even, a finite value that overflows saturates.  `fits`: none of them is beyond the type's
+// largest value (nor NaN); only a vector that may hold one is looked at element by element.
+template <typename T> __device__ __forceinline__ void store8(T* p, const float (&f)[8], bool fits)
 {
     if constexpr (sizeof(T) == 4) {
         __stcs(reinterpret_cast<float4*>(p), make_float4(f[0], f[1], f[2], f[3]));
         __stcs(reinterpret_cast<float4*>(p) + 1, make_float4(f[4], f[5], f[6], f[7]));
     } else {
-        constexpr float kMost = std::is_same<T, __half>::value ? 65504.0f : 3.3895313892515355e38f;
         uint32_t r[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if constexpr (std::is_same<T, __half>::value) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r[i]) : "f"(f[2 * i + 1]), "f"(f[2 * i]));
             else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r[i]) : "f"(f[2 * i + 1]), "f"(f[2 * i]));
         }
-        if (__builtin_expect(!(top <= kMost), 0)) {
+        if (__builtin_expect(!fits, 0)) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if constexpr (std::is_same<T, __half>::value) r[i] = pack_f16x2_sat(f[2 * i], f[2 * i + 1]);
@@ -159,6 +160,51 @@ __device__ __forceinline__ int mx_exponent(float amax, float rstd, float rstdLo,
 // 2^-e for e in [-127, 127]; 2^-127 is a subnormal
 __device__ __forceinline__ float exp2_neg(int e) { return e == 127 ? __uint_as_float(0x00400000u) : __uint_as_float(static_cast<uint32_t>(127 - e) << 23); }
 
+// Codes on the right side of a tie.  v = fl(fl(h * gamma) * fl(rstd * 2^-e)) is within 2.5 units in the last place of y * 2^-e; only a v
+// closer than that to the middle between two codes can be cast to the wrong one, and four units are looked at: one element in 116,000.
+template <int OUT> struct Tie {
+    static constexpr bool kLooked = OUT == kOutE4M3 || OUT == kOutE5M2;  // (fp4 goes through bfloat16, whose own rounding is part of its definition)
+    static constexpr int kDrop = OUT == kOutE4M3 ? 20 : 21;              // mantissa bits that the cast drops; the middle is 100...0
+    // small for a v next to a tie: its dropped bits, counted from four units below the middle
+    static __device__ __forceinline__ uint32_t distance(float v) { return (__float_as_uint(v) << (32 - kDrop)) + (0x80000000u + (4u << (32 - kDrop))); }
+    static __device__ __forceinline__ uint32_t least(const float (&v)[8])
+    {
+        return __vimin3_u32(__vimin3_u32(__vimin3_u32(distance(v[0]), distance(v[1]), distance(v[2])), distance(v[3]), distance(v[4])), distance(v[5]),
+                            min(distance(v[6]), distance(v[7])));
+    }
+    static constexpr uint32_t kNear = 8u << (32 - kDrop);
+    // v, moved to the side of the tie where h * gamma * (rstd + rstdLo) * up lies (on it if that is exactly the middle).  Codes below
+    // the smallest normal one have their ties elsewhere, at dropped bits 0, where nothing is moved.
+    static __device__ __forceinline__ float settle(float h, float gamma, float rstd, float rstdLo, float up)
+    {
+        const float p = __fmul_rn(h, gamma), pl = fmaf(h, gamma, -p), f = __fmul_rn(rstd, up), v = __fmul_rn(p, f);
+        const float rest = __fadd_rn(fmaf(p, f, -v), fmaf(pl, f, __fmul_rn(p, __fmul_rn(rstdLo, up))));
+        const uint32_t middle = (__float_as_uint(v) & ~((1u << kDrop) - 1u)) | (1u << (kDrop - 1));
+        const float d = __fadd_rn(__fsub_rn(v, __uint_as_float(middle)), rest), out = v < 0.f ? -d : d;
+        return __uint_as_float(out > 0.f ? middle + 1u : out < 0.f ? middle - 1u : middle);
+    }
+};
+
+// h = src + residual of an element whose v = fl(fl(h * gamma) * f) is known, formed again although residualOut may have taken the place of one of
+// the two: v / (gamma * f) is within 5 units of h's last place, so the lost one is the value of T nearest to it less the other, unless the
+// lost one is so small beside h that T has several values there.  False then, and in the same cases where both are in memory, so that a call
+// in place gives the bits of one that is not.  (Keeping the old values: in
+// registers 171 us, in shared memory, which is taken from L1, 158; this way 143; 134 without a look at ties, with 16 times as many codes off.)
+template <typename T> __device__ __forceinline__ bool row_sum(T x, T r, float v, float gamma, float f, bool overSrc, bool overRes, float& h)
+{
+    float a = to_f32<T>(x), b = to_f32<T>(r);
+    if (overSrc || overRes) {
+        const float whole = __fdiv_rn(v, __fmul_rn(gamma, f));
+        if (overSrc && overRes) a = b = to_f32<T>(narrow<T>(0.5f * whole));  // src and residual are one tensor
+        else if (overSrc) a = to_f32<T>(narrow<T>(__fsub_rn(whole, b)));
+        else b = to_f32<T>(narrow<T>(__fsub_rn(whole, a)));
+    }
+    h = __fadd_rn(a, b);
+    // bf16: off by 8 * 2^-24 |h| at most, T's values at a are 2^-8 |a| apart at least (2^-9 next to a power of two); fp16: 2^-11, 2^-12
+    constexpr float kLeast = std::is_same<T, __half>::value ? 0.00390625f : 0.00048828125f;
+    return fminf(fabsf(a), fabsf(b)) >= kLeast * fabsf(h);
+}
+
 // The int8 chain's multiplier 127 / amax, in two factors so that it does not overflow where amax is close to the smallest
 // normal number: q = RINT((p * pre) * mul).  pre is 1 for every amax that a norm leaves in practice.
 struct I8Factor {
@@ -198,15 +244,15 @@ __device__ __forceinline__ Sum2 rstd_of(Sum2 sum, float n, float epsilon)
 struct RowStats {
     float rstd, rstdLo, mx, pad;
 };
-// Sum and maximum over the CTA.  The warps' sums are added exactly, since every code of the row depends on the result, and the division, the square
+// Sum and (MAX) maximum over the CTA.  The warps' sums are added exactly, since every code of the row depends on the result, and the division, the square
 // root and its correction take some two hundred instructions: one warp does that and the others read the outcome (in every warp it
 // cost as many issue slots as the elements did: 163 us instead of 136 at [16384, 7168]).
-__device__ __forceinline__ RowStats row_stats(float sum, float mx, float2* part, RowStats* stats, float n, float epsilon)
+template <bool MAX> __device__ __forceinline__ RowStats row_stats(float sum, float mx, float2* part, RowStats* stats, float n, float epsilon)
 {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-        mx = max_nan(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
+        if constexpr (MAX) mx = max_nan(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
     }
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     if (lane == 0) part[warp] = make_float2(sum, mx);
@@ -218,7 +264,7 @@ __device__ __forceinline__ RowStats row_stats(float sum, float mx, float2* part,
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) {
             all = add_exact(all, Sum2{__shfl_xor_sync(0xFFFFFFFFu, all.hi, o), __shfl_xor_sync(0xFFFFFFFFu, all.lo, o)});
-            mx = max_nan(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
+            if constexpr (MAX) mx = max_nan(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
         }
         const Sum2 r = rstd_of(all, n, epsilon);
         if (lane == 0) *stats = RowStats{finite_f32(all.hi) ? r.hi : __int_as_float(0x7FFFFFFF), r.lo, mx, 0.f};
@@ -247,6 +293,14 @@ template <typename T, typename G, int OUT, int NV> __global__ void __launch_boun
             for (int j = 0; j < static_cast<int>(sizeof(G)) / 2; ++j) g[i].w[j] = __ldg(p + j);
         }
     }
+    auto settled = [&](float v, uint32_t row, uint32_t col, const RowStats& st, int e) {
+        const T x = src[row * a.ldSrc + col], r = res ? res[row * a.ldResidual + col] : x;
+        const float g = to_f32<G>(static_cast<const G*>(a.gamma)[col]), up = exp2_neg(e);
+        float h = to_f32<T>(x);
+        if (res && sizeof(T) == 4 && a.residualOut) h = to_f32<T>(static_cast<const T*>(a.residualOut)[row * a.ldResidualOut + col]);
+        else if (res && !row_sum<T>(x, r, v, g, __fmul_rn(st.rstd, up), a.residualOut == a.src, a.residualOut == a.residual, h)) return v;
+        return Tie<OUT>::settle(h, g, st.rstd, st.rstdLo, up);
+    };
     Vec8<T> xs[NV], rs[NV];
     auto load_row = [&](uint32_t row) {
 #pragma unroll
@@ -273,7 +327,10 @@ template <typename T, typename G, int OUT, int NV> __global__ void __launch_boun
 #pragma unroll
                     for (int j = 0; j < 8; j += 2) add2_rn(h[i][j], h[i][j + 1], r[j], r[j + 1]);
                 }
-                if (a.residualOut) store8<T>(static_cast<T*>(a.residualOut) + row * a.ldResidualOut + v * 8, h[i], sizeof(T) == 4 ? 0.f : max_abs8(h[i]));
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) fma2_square(sum, sumOdd, h[i][j], h[i][j + 1]);
+                // (no element is larger than the root of the thread's sum so far)
+                if (a.residualOut) store8<T>(static_cast<T*>(a.residualOut) + row * a.ldResidualOut + v * 8, h[i], sizeof(T) == 4 || sum + sumOdd <= kMostSquaredOf<T>);
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) h[i][j] = 0.f;
@@ -287,14 +344,11 @@ template <typename T, typename G, int OUT, int NV> __global__ void __launch_boun
                 float gf[8];
                 widen8<G>(g[i], gf);
 #pragma unroll
-                for (int j = 0; j < 8; j += 2) {
-                    fma2_square(sum, sumOdd, h[i][j], h[i][j + 1]);
-                    mul2_rn(h[i][j], h[i][j + 1], gf[j], gf[j + 1]);  // from here on h * gamma
-                }
+                for (int j = 0; j < 8; j += 2) mul2_rn(h[i][j], h[i][j + 1], gf[j], gf[j + 1]);  // from here on h * gamma
                 if constexpr (OUT == kOutI8) mx = max_nan(mx, max_abs8(h[i]));
             }
         }
-        const RowStats st = row_stats(sum + sumOdd, mx, part, &stats, static_cast<float>(a.n), a.epsilon);
+        const RowStats st = row_stats<OUT == kOutI8>(sum + sumOdd, mx, part, &stats, static_cast<float>(a.n), a.epsilon);
         const float rstd = st.rstd;
         mx = st.mx;
         if (a.normOut) {
@@ -302,10 +356,11 @@ template <typename T, typename G, int OUT, int NV> __global__ void __launch_boun
             for (int i = 0; i < NV; ++i) {
                 const uint32_t v = i * blockDim.x + threadIdx.x;
                 if (v < nvec) {
+                    constexpr float kMost = std::is_same<T, __half>::value ? 65504.0f : 3.3895313892515355e38f;
                     float y[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) y[j] = __fmul_rn(h[i][j], rstd);
-                    store8<T>(static_cast<T*>(a.normOut) + row * a.ldNormOut + v * 8, y, max_abs8(y));
+                    store8<T>(static_cast<T*>(a.normOut) + row * a.ldNormOut + v * 8, y, max_abs8(y) <= kMost);
                 }
             }
         }
@@ -348,10 +403,18 @@ template <typename T, typename G, int OUT, int NV> __global__ void __launch_boun
                         // rstd * 2^-e is exact: one multiplication gives what y and its scaling would
                         const float f = __fmul_rn(rstd, exp2_neg(e));
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            mul2_rn(h[i][2 * j], h[i][2 * j + 1], f, f);
-                            c[j] = mx_pair<OUT>(h[i][2 * j], h[i][2 * j + 1]);
+                        for (int j = 0; j < 4; ++j) mul2_rn(h[i][2 * j], h[i][2 * j + 1], f, f);
+                        if constexpr (Tie<OUT>::kLooked) {
+                            uint32_t least = 0xFFFFFFFFu;
+                            least = Tie<OUT>::least(h[i]);
+                            if (__builtin_expect(least <= Tie<OUT>::kNear, 0)) {
+#pragma unroll
+                                for (int j = 0; j < 8; ++j)
+                                    if (Tie<OUT>::distance(h[i][j]) <= Tie<OUT>::kNear) h[i][j] = settled(h[i][j], row, v * 8 + j, st, e);
+                            }
                         }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) c[j] = mx_pair<OUT>(h[i][2 * j], h[i][2 * j + 1]);
                     } else {
                         const float up = exp2_neg(e);
 #pragma unroll
@@ -415,7 +478,7 @@ template <typename T, typename G, int VEC, int NE> __global__ void __launch_boun
             if (a.residualOut) *reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(a.residualOut) + row * a.ldResidualOut + v * VEC) = total;
         }
     }
-    const RowStats st = row_stats(sum, mx, part, &stats, static_cast<float>(a.n), a.epsilon);
+    const RowStats st = row_stats<true>(sum, mx, part, &stats, static_cast<float>(a.n), a.epsilon);
     const float rstd = st.rstd, top = __fmul_rn(st.mx, rstd);
     const bool ok = finite_f32(st.mx) && finite_f32(top);
     const I8Factor f = i8_factor(st.mx);
@@ -460,7 +523,7 @@ template <typename T, typename G> __global__ void __launch_bounds__(256) norm_an
         sum = fmaf(h, h, sum);
         mx = max_nan(mx, fabsf(__fmul_rn(h, to_f32<G>(gamma[c]))));
     }
-    const RowStats st = row_stats(sum, mx, part, &stats, static_cast<float>(a.n), a.epsilon);
+    const RowStats st = row_stats<true>(sum, mx, part, &stats, static_cast<float>(a.n), a.epsilon);
     const float rstd = st.rstd;
     mx = st.mx;
     const float top = __fmul_rn(mx, rstd);
@@ -472,9 +535,9 @@ template <typename T, typename G> __global__ void __launch_bounds__(256) norm_an
     // each element is read again by the thread that then overwrites it where residualOut is one of the sources
     for (uint32_t c0 = 0; c0 < a.n; c0 += blockDim.x) {
         const uint32_t c = c0 + threadIdx.x;
-        float p = 0.f;
+        float p = 0.f, h = 0.f;
         if (c < a.n) {
-            const float h = res ? __fadd_rn(to_f32<T>(src[c]), to_f32<T>(res[c])) : to_f32<T>(src[c]);
+            h = res ? __fadd_rn(to_f32<T>(src[c]), to_f32<T>(res[c])) : to_f32<T>(src[c]);
             p = __fmul_rn(h, to_f32<G>(gamma[c]));
             if (resOut) resOut[c] = narrow<T>(h);
             if (normOut) normOut[c] = narrow<T>(__fmul_rn(p, rstd));
@@ -490,7 +553,13 @@ template <typename T, typename G> __global__ void __launch_bounds__(256) norm_an
             for (int o = 16; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
             const bool ok = finite_f32(__fmul_rn(amax, rstd));
             const int e = mx_exponent(amax, rstd, st.rstdLo, out_emax(a.out));
-            const float v = __fmul_rn(y, exp2_neg(e));
+            float v = __fmul_rn(y, exp2_neg(e));
+            if (ok && e > -80 && e < 80 && c < a.n) {
+                if (a.out == kOutE4M3 && Tie<kOutE4M3>::distance(v) <= Tie<kOutE4M3>::kNear)
+                    v = Tie<kOutE4M3>::settle(h, to_f32<G>(gamma[c]), rstd, st.rstdLo, exp2_neg(e));
+                if (a.out == kOutE5M2 && Tie<kOutE5M2>::distance(v) <= Tie<kOutE5M2>::kNear)
+                    v = Tie<kOutE5M2>::settle(h, to_f32<G>(gamma[c]), rstd, st.rstdLo, exp2_neg(e));
+            }
             const float next = __shfl_down_sync(0xFFFFFFFFu, v, 1);
             if (c < a.n) {
                 if (a.out == kOutE2M1) {
@@ -528,7 +597,7 @@ template <typename T, typename G, int OUT> cudaError_t launch_norm_rows(const No
     while (nv < kNormMaxVectors && (nvec + nv - 1) / nv > kNormThreads) nv *= 2;
     const unsigned block = ((nvec + nv - 1) / nv + 31) / 32 * 32;
     // About 1280 threads per SM, each CTA walking over its rows with the next one on its way.  Measured: bf16 [16384, 7168] to e4m3 (448
-    // threads) 182 / 135 / 147 us with 1 / 2 / 3 CTAs per SM; half [1031, 5120] to int8 (320 threads) 8.2 / 8.1 / 5.6 / 5.5 / 5.6 us with
+    // threads) 199 / 141 / 170 us with 1 / 2 / 3 CTAs per SM; half [1031, 5120] to int8 (320 threads) 8.2 / 8.1 / 5.6 / 5.5 / 5.6 us with
     // 1 to 5.  Rows above 8192 elements need 128 registers a thread: one CTA.
     const unsigned perSm = nv >= 4 ? 1u : std::max(1u, 1280u / block);
     const unsigned grid = std::min<uint64_t>(a.m, static_cast<uint64_t>(sm_count()) * perSm);

@@ -176,6 +176,34 @@ def test_in_place_residual(n):
 
 
 @gpu
+@pytest.mark.parametrize("place", ["own", "src", "residual", "unaligned"])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("out", [L.DT_FP8_E4M3, L.DT_FP8_E5M2])
+def test_mx_codes_next_to_a_tie(out, dt, place):
+    """Whole numbers: h and its sum of squares are exact and n is a power of two, so rstd is known to 2^-44 and the code has to be the exact one for
+    every element further than 2^-40 from the middle between two codes (three roundings to fp32 would reach 2^-23)."""
+    m, n, eps = 4096, 1024, 2.0 ** -20
+    g = torch.Generator().manual_seed(5)
+    x, r = ((torch.randint(1, 9, (m, n), generator=g) * (1 - 2 * torch.randint(0, 2, (m, n), generator=g))).to(dt).to(DEV) for _ in range(2))
+    gamma = (1 + 0.2 * torch.randn(n, generator=g)).to(DEV)
+    h = x.double() + r.double()
+    y = h * gamma.double() / torch.sqrt((h * h).mean(-1, keepdim=True) + eps)
+    dst, scale = torch.empty(m, n, dtype=torch.uint8, device=DEV), torch.empty(m, n // 32, dtype=torch.uint8, device=DEV)
+    if place == "unaligned":
+        wide = torch.empty(m, n + 1, dtype=dt, device=DEV)
+        wide[:, 1:] = x
+        x = wide[:, 1:]
+    total = {"own": torch.empty_like(r), "src": x, "residual": r, "unaligned": None}[place]
+    ops.ResidualRmsNormQuant(dst, scale, x, gamma, eps, residual=r, residualOut=total, dst_dtype=out)
+    v = (y.reshape(m, -1, 32) / torch.exp2(scale.double() - 127)[..., None]).reshape(m, n)
+    got = dst.view(torch.float8_e4m3fn if out == L.DT_FP8_E4M3 else torch.float8_e5m2).double()
+    low, high = to_grid(v * (1 - 2.0 ** -40), out), to_grid(v * (1 + 2.0 ** -40), out)
+    wrong = (got != low) & (got != high)
+    assert not wrong.any(), f"{int(wrong.sum())} codes on the wrong side"
+    assert total is None or torch.equal(total.double(), h)
+
+
+@gpu
 @pytest.mark.parametrize("n", [512, 511])
 def test_special_rows_int8(n):
     x, r, g = inputs(8, n, torch.bfloat16, residual=False)
