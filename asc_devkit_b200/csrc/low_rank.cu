@@ -240,6 +240,10 @@ template <typename T, int NB> __global__ void __launch_bounds__(32 * kWarps, NB 
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+            if (__builtin_expect(!(top <= 3.4028234663852886e38f), 0)) {
+#pragma unroll
+                for (int i = 0; i < (R + 31) / 32; ++i) v[i] = inside_range<T>(v[i]);
+            }
             const int shift = range_shift(top);
             const float down = exp2_int(-shift);
             if (lane == 0) unit[row] = exp2_int(shift);

@@ -119,14 +119,20 @@ __device__ __forceinline__ int range_shift(float top)
     return ex == 0 || ex == 255 ? 0 : min(max(ex - 136, -126), 126);
 }
 __device__ __forceinline__ float exp2_int(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
-// v as two 16-bit terms: x = cast(v), y = cast(v - x); 0 for the second where the first is not finite.  The casts saturate: beside an
-// infinity a row keeps its range, and what is finite in it must not become an infinity of the other sign.
+// Beside an infinity a row keeps its range; what is finite in it must not become an infinity of the other sign.  (Only rows with a `top` that
+// is not finite come here: casts that saturate, for every row, cost 9 us of 62 at 8192 tokens.)
+template <typename T> __device__ __forceinline__ float inside_range(float v)
+{
+    constexpr float kMost = std::is_same<T, __half>::value ? 65504.0f : 3.3895313892515355e38f;
+    return fabsf(v) <= 3.4028234663852886e38f ? fminf(fmaxf(v, -kMost), kMost) : v;
+}
+// v as two 16-bit terms: x = cast(v), y = cast(v - x); 0 for the second where the first is not finite
 template <typename T> __device__ __forceinline__ uint2 split16(float v)
 {
     uint2 r;
-    r.x = pack_sat<T>(v, 0.f) & 0xFFFFu;
+    r.x = pack2<T>(v, 0.f) & 0xFFFFu;
     const float back = unpack2<T>(r.x).x;
-    r.y = fabsf(back) <= 3.4028234663852886e38f ? pack_sat<T>(v - back, 0.f) & 0xFFFFu : 0u;
+    r.y = fabsf(back) <= 3.4028234663852886e38f ? pack2<T>(v - back, 0.f) & 0xFFFFu : 0u;
     return r;
 }
 

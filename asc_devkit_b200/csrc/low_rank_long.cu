@@ -93,6 +93,10 @@ __device__ __forceinline__ void finish_rows(const float* part, int there, int st
 #pragma unroll
     for (int s = 1; s < CTAS; s <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, s));
     if (row >= there) return;
+    if (__builtin_expect(!(top <= 3.4028234663852886e38f), 0)) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[i] = inside_range<T>(v[i]);
+    }
     const int shift = range_shift(top);
     const float down = exp2_int(-shift);
     if (col0 == 0) o.unit[start + row] = exp2_int(shift);
