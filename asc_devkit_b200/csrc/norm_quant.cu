@@ -172,6 +172,7 @@ template <int OUT> struct Tie {
         return __vimin3_u32(__vimin3_u32(__vimin3_u32(distance(v[0]), distance(v[1]), distance(v[2])), distance(v[3]), distance(v[4])), distance(v[5]),
                             min(distance(v[6]), distance(v[7])));
     }
+    static constexpr float kLowest = OUT == kOutE4M3 ? 0.015625f : 6.103515625e-05f;  // the smallest normal code
     static constexpr uint32_t kNear = 8u << (32 - kDrop);
     // v, moved to the side of the tie where h * gamma * (rstd + rstdLo) * up lies (on it if that is exactly the middle).  Codes below
     // the smallest normal one have their ties elsewhere, at dropped bits 0, where nothing is moved.
@@ -294,6 +295,7 @@ template <typename T, typename G, int OUT, int NV> __global__ void __launch_boun
         }
     }
     auto settled = [&](float v, uint32_t row, uint32_t col, const RowStats& st, int e) {
+        if (fabsf(v) < Tie<OUT>::kLowest) return v;  // no tie there; and above it gamma * f = v / h is far from underflow
         const T x = src[row * a.ldSrc + col], r = res ? res[row * a.ldResidual + col] : x;
         const float g = to_f32<G>(static_cast<const G*>(a.gamma)[col]), up = exp2_neg(e);
         float h = to_f32<T>(x);
