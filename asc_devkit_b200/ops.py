@@ -51,12 +51,14 @@ def _ptr_pitched(t: torch.Tensor):
 
 
 def _workspace(need: int, device, stream: Optional[torch.cuda.Stream]) -> torch.Tensor:
-    """A temporary workspace for a call that returns while its kernels still run.  The caching allocator hands a freed
-    block back to torch's current stream; when the kernels run on another stream the block is tied to that one too."""
-    ws = torch.empty(max(int(need), 256), dtype=torch.uint8, device=device)
-    if stream is not None and stream != torch.cuda.current_stream(ws.device):
-        ws.record_stream(stream)
-    return ws
+    """A temporary workspace for a call that returns while its kernels still run.  It comes from the pool of the stream that the
+    kernels run on: the caching allocator hands a freed block only to later work on the stream it was taken for, so the
+    next owner is ordered behind these kernels.  (A block of another stream's pool may still be read by that stream's work.)"""
+    size = max(int(need), 256)
+    if stream is None:
+        return torch.empty(size, dtype=torch.uint8, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(size, dtype=torch.uint8, device=device)
 
 
 def _stream(stream: Optional[torch.cuda.Stream]):

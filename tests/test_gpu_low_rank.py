@@ -252,6 +252,45 @@ def test_two_calls_at_once_on_two_streams():
 
 
 @gpu
+@pytest.mark.parametrize("size", [4096, 3 << 20, 40 << 20])
+def test_workspaces_of_two_streams_are_never_the_same_block(size):
+    """What one stream's call gave back may still be read by its kernels: a call on another stream must not get it, in either
+    direction.  (Nothing runs here: only the addresses count.)"""
+    dev, other = torch.device(DEV), torch.cuda.Stream()
+    mine = ops._workspace(size, dev, None)
+    at = mine.data_ptr()
+    del mine
+    theirs = ops._workspace(size, dev, other)
+    assert theirs.data_ptr() != at
+    back = theirs.data_ptr()
+    del theirs
+    mine = ops._workspace(size, dev, None)
+    assert mine.data_ptr() != back
+    del mine
+    assert ops._workspace(size, dev, other).data_ptr() == back  # the same stream's next call may have it
+
+
+@gpu
+@pytest.mark.parametrize("m,n,k", [(1500, 256, 512), (3000, 4096, 3000)])
+def test_a_call_on_another_stream_takes_its_own_workspace(m, n, k, monkeypatch):
+    """The public call's workspace: taken while `stream` is torch's current stream."""
+    x, base, a, b, scale, ids = case(m, n, k, 16, 4, torch.bfloat16)
+    want, got, s, seen = torch.empty_like(base), torch.empty_like(base), torch.cuda.Stream(), []
+    ops.LowRankAdd(want, base, x, a, b, ids, scale=scale)
+    s.wait_stream(torch.cuda.current_stream())
+    empty = torch.empty
+
+    def note(*args, **kw):
+        seen.append(torch.cuda.current_stream())
+        return empty(*args, **kw)
+    monkeypatch.setattr(torch, "empty", note)
+    ops.LowRankAdd(got, base, x, a, b, ids, scale=scale, stream=s)
+    monkeypatch.undo()
+    s.synchronize()
+    assert seen == [s] and torch.equal(got, want)
+
+
+@gpu
 def test_empty():
     e = lambda *s: torch.empty(*s, dtype=torch.float16, device=DEV)  # noqa: E731
     ops.LowRankAdd(e(0, 16), e(0, 16), e(0, 8), e(2, 8, 8), e(2, 16, 8), torch.empty(0, dtype=torch.int32, device=DEV))
