@@ -156,6 +156,8 @@ template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_ra
         tmem_alloc(&tmemSlot, C::kTmemCols);
         tmem_relinquish();
     }
+    // A dependent launch may take tensor memory too: it is let in only when this CTA has its columns.
+    __syncthreads();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (warp == 0) find_tile<kRows>(tileIdx, p.L + 1, [&](int e) { return static_cast<int>(p.counts[e]); }, found);
@@ -314,6 +316,9 @@ __global__ void __launch_bounds__(kOuterThreads, NB <= 8 ? 2 : 1) low_rank_outer
         tmem_alloc(&tmemSlot, 2 * kBlockCols);
         tmem_relinquish();
     }
+    tc_fence_before();
+    __syncthreads();  // before a dependent launch, which may take tensor memory too, is let in
+    tc_fence_after();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int4* tiles = static_cast<const int4*>(o.tiles);
@@ -321,9 +326,6 @@ __global__ void __launch_bounds__(kOuterThreads, NB <= 8 ? 2 : 1) low_rank_outer
     const int64_t total = static_cast<int64_t>(tiles[tileBound].x) * perTile;
     int64_t pos = total * blockIdx.x / gridDim.x;
     const int64_t end = total * (blockIdx.x + 1) / gridDim.x;
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
     bool ok = true;
     uint32_t it = 0, segment = 0;  // blocks multiplied so far, and tiles: the barriers' slots and phases go by them
     while (pos < end && ok) {
