@@ -97,6 +97,7 @@ SIGNATURES = {
     "ascq_group_matmul_mxfp4_sharded": (_i, [_vp, C.POINTER(_vp), _vp, _vp, _vp, _vp, _P64, _i, _i, _i, _vp, C.c_size_t, _vp]),
     "ascq_set_wait_limit_cycles": (_i, [C.c_longlong]),
     "ascq_test_withhold_after": (_i, [_i]),
+    "ascq_test_withhold_low_rank": (_i, [_i, _i]),
     "ascq_measure_tensor_rate": (_i, [_i, _i, C.POINTER(C.c_double), _vp]),
     "ascq_low_rank_add": (_i, [_vp, C.c_int64, _vp, C.c_int64, _vp, C.c_int64, _vp, _vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _vp, C.c_size_t, _vp]),
     "ascq_low_rank_add_workspace_size": (C.c_size_t, [_i, _i, _i, _i, _i]),

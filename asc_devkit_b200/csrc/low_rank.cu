@@ -439,7 +439,7 @@ extern "C" ascq_status ascq_low_rank_add(void* dst, int64_t ldDst, const void* b
         p.counts = counts;
         p.order = order;
         if (ws.tiles) {
-            const LowRankScratch o{w + ws.tiles, w + ws.v, reinterpret_cast<float*>(w + ws.unit)};
+            const LowRankScratch o{w + ws.tiles, w + ws.v, reinterpret_cast<float*>(w + ws.unit), 0, 0};
             const int64_t tiles = tile_bound(M, L, kLongTile);
             if (tiles > 0x7FFFFFF) return fail(ASCQ_ERR_INVALID_ARG, "M is too large for one launch");
             return low_rank_long(p, T == ASCQ_DT_F16, o, static_cast<unsigned>(tiles), st);

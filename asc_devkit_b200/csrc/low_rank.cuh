@@ -23,6 +23,7 @@ struct LowRankScratch {
     void* tiles;   // int4 per tile
     void* v;       // split inner products
     float* unit;   // [M]
+    int stopA, stopB;  // a CTA loads no chunk of A (first launch), no block of B (second) from this number on; set by low_rank_long
 };
 constexpr int kLongTile = 128;
 size_t low_rank_long_tiles_bytes(int64_t tiles);

@@ -38,11 +38,12 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool i
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-// Waits, bounded, for a copy that is on its way although the CTA gives up.
+// Waits for copies or MMAs that were issued, also when the CTA gives up: none may be under way when its memory is given back.  They end by
+// themselves, so the bound is there for a broken machine only; it is not the adjustable limit, which may be short and has just run out.
 __device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity)
 {
     const long long t0 = clock64();
-    while (!mbar_try_wait(bar, parity) && clock64() - t0 < c_waitCycles) {}
+    while (!mbar_try_wait(bar, parity) && clock64() - t0 < kWaitCycles) {}
 }
 // this thread's finished copies become visible to the tensor cores, and the barrier learns of it
 __device__ __forceinline__ void publish(uint64_t* bar)
@@ -210,16 +211,17 @@ template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_ra
             }
         } else if (warp == 9) {
             if (elect_one()) {
+                const int loads = min(n, o.stopA);
                 int i = 0;
-                for (; i < n; ++i) {
+                for (; i < loads; ++i) {
                     const int s = i % C::kStages;
                     if (i >= C::kStages && !(ok = mbar_wait_bounded(&emptyBar[s], (i / C::kStages - 1) & 1, &abortFlag))) break;
                     // rows behind the adapter's rank are the next adapter's (or zeros): columns of D that finish_rows leaves out
                     mbar_arrive_expect_tx(&aBar[s], C::kABytes);
                     tma_load_2d(ring + s * C::kStageBytes + kAtomBytes, &mapA, &aBar[s], (first + i) * 64, adapter * p.r);
                 }
-                if (!ok)  // no copy may be on its way when the CTA ends
-                    for (int j = max(i - C::kStages, 0); j < i; ++j) drain(&aBar[j % C::kStages], (j / C::kStages) & 1);
+                // (whoever gives up: the MMAs need not have waited for the last loads)
+                for (int j = max(i - C::kStages, 0); j < i; ++j) drain(&aBar[j % C::kStages], (j / C::kStages) & 1);
             }
         } else if (elect_one()) {
             constexpr uint32_t idesc = idesc_f16(kRows, R, std::is_same<T, __half>::value ? 0 : 1);
@@ -233,7 +235,10 @@ template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_ra
                 for (int k = 0; k < 4; ++k) mma_f16(tmemSlot, descX + 2 * k, descA + 2 * k, idesc, (i | k) != 0);
                 tc_commit(&emptyBar[s]);
             }
-            if (ok && n > 0) tc_commit(&doneBar);
+            if (n > 0) {  // the MMAs issued so far, all of them or not
+                tc_commit(&doneBar);
+                drain(&doneBar, 0);
+            }
         }
         __syncwarp();
         // Each CTA of the cluster finishes its share of the rows: the others' sums are stored into its shared memory (nobody waits for a
@@ -328,6 +333,7 @@ __global__ void __launch_bounds__(kOuterThreads, NB <= 8 ? 2 : 1) low_rank_outer
     const int64_t end = total * (blockIdx.x + 1) / gridDim.x;
     bool ok = true;
     uint32_t it = 0, segment = 0;  // blocks multiplied so far, and tiles: the barriers' slots and phases go by them
+    uint32_t issued = 0;           // blocks whose MMAs were issued
     while (pos < end && ok) {
         const int tileIdx = static_cast<int>(pos / perTile), first = static_cast<int>(pos % perTile);
         const int blocks = static_cast<int>(min(end - pos, static_cast<int64_t>(perTile - first)));
@@ -435,8 +441,9 @@ __global__ void __launch_bounds__(kOuterThreads, NB <= 8 ? 2 : 1) low_rank_outer
             const int steps = (p.r + 15) / 16;
             auto done = [&](uint32_t n) { return mbar_wait_bounded(&outBar[n & 1], (n >> 1) & 1, &abortFlag); };  // block n's MMAs
             int asked = 0;  // blocks of B asked for
+            bool begun = false;
             auto load_b = [&](int b) {
-                if (b >= blocks) return;
+                if (b >= blocks || it + b >= static_cast<uint32_t>(o.stopB)) return;
                 asked = b + 1;
                 const uint32_t s = (it + b) % 3;
                 mbar_arrive_expect_tx(&bBar[s], C::kBBytes);
@@ -446,6 +453,7 @@ __global__ void __launch_bounds__(kOuterThreads, NB <= 8 ? 2 : 1) low_rank_outer
             };
             if (it > 0) ok = done(it - 1);  // V and the slots of B are read no more
             if (ok) {
+                begun = true;
                 mbar_arrive_expect_tx(&vBar, C::kVBytes);
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
@@ -468,8 +476,9 @@ __global__ void __launch_bounds__(kOuterThreads, NB <= 8 ? 2 : 1) low_rank_outer
                         mma_f16(tmemSlot + (n & 1) * kBlockCols, smem_desc_sw128(v + (h * C::kAtoms + (k >> 2)) * kAtomBytes) + 2 * (k & 3),
                                 smem_desc_sw128(w + (k >> 2) * kBlockCols * 128) + 2 * (k & 3), idesc, (h | k) != 0);
                 tc_commit(&outBar[n & 1]);
+                issued = n + 1;
             }
-            if (!ok && asked > 0) {  // no copy may be on its way when the CTA ends
+            if (!ok && begun) {  // no copy may be on its way when the CTA ends
                 drain(&vBar, segment & 1);
                 for (int b = max(asked - 3, 0); b < asked; ++b) drain(&bBar[(it + b) % 3], ((it + b) / 3) & 1);
             }
@@ -479,6 +488,11 @@ __global__ void __launch_bounds__(kOuterThreads, NB <= 8 ? 2 : 1) low_rank_outer
         it += blocks;
     }
     __syncwarp();
+    if (warp == 8) {  // nor an MMA, should the warps that wait for it have given up
+        issued = __reduce_max_sync(0xFFFFFFFFu, issued);
+        if (issued > 0) drain(&outBar[(issued - 1) & 1], ((issued - 1) >> 1) & 1);
+        __syncwarp();
+    }
     tc_fence_before();
     __syncthreads();
     if (warp == 8) {
@@ -571,6 +585,14 @@ template <typename T, int NB> ascq_status launch_long(const LowRankArgs& p, cons
     ASCQ_CUDA_CHECK(launch_pdl(low_rank_outer_kernel<T, NB>, dim3(grid), kOuterThreads, Outer<NB>::kBytes, 1, st, p, o, static_cast<int>(tiles), mapB, mapV));
     return ASCQ_OK;
 }
+// Test hook (ascq_test_withhold_low_rank): the loads that the next call makes of A and B, per CTA; -1: all.
+std::atomic<int> g_stopANext{-1}, g_stopBNext{-1};
+int stop_of(std::atomic<int>& next)
+{
+    const int stop = next.exchange(-1);
+    return stop < 0 ? INT32_MAX : stop;
+}
+
 template <typename T> ascq_status launch_long_typed(const LowRankArgs& p, const LowRankScratch& o, unsigned tiles, cudaStream_t st)
 {
     switch (rank_blocks(p.r)) {
@@ -586,8 +608,11 @@ template <typename T> ascq_status launch_long_typed(const LowRankArgs& p, const 
 size_t low_rank_long_tiles_bytes(int64_t tiles) { return static_cast<size_t>(tiles + 1) * 16; }
 size_t low_rank_long_inner_bytes(int M, int r) { return static_cast<size_t>(M) * 2 * rank_pitch(rank_blocks(r)) * 2; }
 
-ascq_status low_rank_long(const LowRankArgs& p, bool half, const LowRankScratch& o, unsigned tiles, ::CUstream_st* st)
+ascq_status low_rank_long(const LowRankArgs& p, bool half, const LowRankScratch& scratch, unsigned tiles, ::CUstream_st* st)
 {
+    LowRankScratch o = scratch;
+    o.stopA = stop_of(g_stopANext);
+    o.stopB = stop_of(g_stopBNext);
     return half ? launch_long_typed<__half>(p, o, tiles, st) : launch_long_typed<__nv_bfloat16>(p, o, tiles, st);
 }
 
@@ -609,3 +634,10 @@ ascq_status low_rank_set_wait_cycles(long long cycles)
     return ASCQ_OK;
 }
 }  // namespace ascq
+
+extern "C" ascq_status ascq_test_withhold_low_rank(int chunksOfA, int blocksOfB)
+{
+    ascq::g_stopANext.store(chunksOfA < 0 ? -1 : chunksOfA);
+    ascq::g_stopBNext.store(blocksOfB < 0 ? -1 : blocksOfB);
+    return ASCQ_OK;
+}

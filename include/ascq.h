@@ -628,6 +628,11 @@ ascq_status ascq_measure_tensor_rate(ascq_dtype operandT, int kBlocks, double* o
  * lower the wait limit first.
  */
 ascq_status ascq_test_withhold_after(int kBlocks);
+/*
+ * The same for the next ascq_low_rank_add in its form for many tokens: its CTAs load no chunk of A (first launch) from the given
+ * one on and no block of B (second launch); < 0: all of them.
+ */
+ascq_status ascq_test_withhold_low_rank(int chunksOfA, int blocksOfB);
 
 /*
  * Synchronises `stream`, then reads and clears the status word the matmul kernels keep on the

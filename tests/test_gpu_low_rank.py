@@ -291,6 +291,35 @@ def test_a_call_on_another_stream_takes_its_own_workspace(m, n, k, monkeypatch):
 
 
 @gpu
+@pytest.mark.parametrize("m,n,k,r,lo,span", [(1700, 4104, 8200, 16, 3, 1), (4700, 4096, 264, 64, 16, 300), (1400, 4096, 5000, 128, 2, 1030)])
+@pytest.mark.parametrize("chunks,blocks", [(0, -1), (3, -1), (-1, 0), (-1, 2)])
+def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_exact(m, n, k, r, lo, span, chunks, blocks):
+    """Loads of A (first launch) or B (second) that are never made, a wait limit of about ten milliseconds: every role leaves
+    its loop, what was issued has ended before shared and tensor memory are given back, and the status names the timeout once."""
+    x, base, a, b, scale, ids = case(m, n, k, r, lo, torch.float16, span)
+    want, got = torch.empty_like(base), torch.empty_like(base)
+    ops.LowRankAdd(want, base, x, a, b, ids, scale=scale)
+    ops.MatmulStatus()
+    if chunks > 0 and k < 4096:
+        return  # (too few chunks in a CTA for the third to be missed)
+    ops.SetWaitLimitCycles(20_000_000)
+    try:
+        L.check(L.lib().ascq_test_withhold_low_rank(chunks, blocks))
+        ops.LowRankAdd(got, base, x, a, b, ids, scale=scale)
+        with pytest.raises(ops.AscqError) as e:
+            ops.MatmulStatus()
+        assert e.value.status == L.ERR_TIMEOUT and "low-rank" in e.value.message
+    finally:
+        ops.SetWaitLimitCycles(0)
+    ops.MatmulStatus()  # the status word was cleared
+    for _ in range(2):
+        got.fill_(3.0)
+        ops.LowRankAdd(got, base, x, a, b, ids, scale=scale)
+        ops.MatmulStatus()
+        assert torch.equal(got, want)
+
+
+@gpu
 def test_empty():
     e = lambda *s: torch.empty(*s, dtype=torch.float16, device=DEV)  # noqa: E731
     ops.LowRankAdd(e(0, 16), e(0, 16), e(0, 8), e(2, 8, 8), e(2, 16, 8), torch.empty(0, dtype=torch.int32, device=DEV))
