@@ -15,7 +15,7 @@
 // Calls with enough tokens per adapter take another form, low_rank_long.cu.
 //
 // The inner product is a sum in fp32; for the second product it is split into two 16-bit terms, hi = cast(v), lo = cast(v - hi), after
-// each token's row was brought to [512, 1024) by a power of two (so that neither fp16's range nor its subnormals matter).  What the split drops is below
+// each token's row was multiplied by a power of two that keeps both inside the type's range (range_shift).  What the split drops is below
 // 2^-16 (bf16) or 2^-22 (fp16) of the row's largest value: the result carries one visible rounding, the one to dst's type.
 #include "experts.cuh"
 #include "low_rank.cuh"
@@ -244,7 +244,7 @@ template <typename T, int NB> __global__ void __launch_bounds__(32 * kWarps, NB 
 #pragma unroll
                 for (int i = 0; i < (R + 31) / 32; ++i) v[i] = inside_range<T>(v[i]);
             }
-            const int shift = range_shift(top);
+            const int shift = range_shift<T>(top);
             const float down = exp2_int(-shift);
             if (lane == 0) unit[row] = exp2_int(shift);
             unsigned short* h = reinterpret_cast<unsigned short*>(hi + row * VP);

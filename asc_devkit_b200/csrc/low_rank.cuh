@@ -112,12 +112,16 @@ __device__ __forceinline__ void st_cluster_v4(uint32_t addr, uint4 v)
 {
     asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
-// Exponent of the power of two that brings a row whose largest magnitude is `top` to [512, 1024); rows that are zero, subnormal or
-// not finite stay as they are.
-__device__ __forceinline__ int range_shift(float top)
+// A row whose largest magnitude is `top` is multiplied by 2^-shift before the split and its products by 2^shift.
+// half: to [512, 1024), clear of its range's end and of its subnormals (|B| <= 65504 keeps the sums far below fp32's end); rows that are zero,
+// subnormal or not finite stay as they are.
+// bfloat16 has fp32's exponents: the products are formed where the formula has them, so that they overflow only where it does.  Only a row
+// next to fp32's end, whose cast would be an infinity, is halved, and one so small that the later terms would be subnormal goes up by 2^32.
+template <typename T> __device__ __forceinline__ int range_shift(float top)
 {
     const int ex = static_cast<int>(__float_as_uint(top) >> 23);
-    return ex == 0 || ex == 255 ? 0 : min(max(ex - 136, -126), 126);
+    if constexpr (std::is_same<T, __half>::value) return ex == 0 || ex == 255 ? 0 : min(max(ex - 136, -126), 126);
+    else return ex == 254 ? 1 : ex < 32 ? -32 : 0;
 }
 __device__ __forceinline__ float exp2_int(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
 // Beside an infinity a row keeps its range; what is finite in it must not become an infinity of the other sign.  (Only rows with a `top` that

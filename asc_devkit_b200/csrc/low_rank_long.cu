@@ -98,7 +98,7 @@ __device__ __forceinline__ void finish_rows(const float* part, int there, int st
 #pragma unroll
         for (int i = 0; i < W; ++i) v[i] = inside_range<T>(v[i]);
     }
-    const int shift = range_shift(top);
+    const int shift = range_shift<T>(top);
     const float down = exp2_int(-shift);
     if (col0 == 0) o.unit[start + row] = exp2_int(shift);
     uint32_t hi[W / 2], lo[W / 2];

@@ -131,6 +131,36 @@ def test_large_and_small_inner_products(m, n):
 
 
 @gpu
+@pytest.mark.parametrize("m,n", [(40, 128), (1200, 20000)])
+@pytest.mark.parametrize("ex,eb", [(-7, 119), (-100, 122), (-100, 100), (-60, 20), (100, -100), (119, -122), (110, 10)])
+def test_bfloat16_over_its_whole_range(m, n, ex, eb):
+    """Inner products near 2^ex, B near 2^eb: their products are in range, so is every step towards them."""
+    x, base, a, b, scale, ids = case(m, n, 256, 16, 2, torch.bfloat16, ids=torch.zeros(m))
+    xs, bs = (x.double() * 2.0 ** ex).to(torch.bfloat16), (b.double() * 2.0 ** eb).to(torch.bfloat16)
+    for own in (base, None):
+        got = torch.empty_like(base)
+        ops.LowRankAdd(got, own, xs, a, bs, ids, scale=scale)
+        assert torch.isfinite(got).all()
+        check(got, xs, own, a, bs, scale, ids)
+
+
+@gpu
+@pytest.mark.parametrize("m,n", [(20, 64), (1300, 16384)])
+def test_bfloat16_inner_product_next_to_the_end_of_fp32(m, n):
+    """1.9921875 * 2^127 * 1.003 lies between bfloat16's largest value and fp32's."""
+    x = torch.zeros(m, 64, dtype=torch.bfloat16, device=DEV)
+    x[:, 3] = 2.0 ** 64
+    a = torch.zeros(1, 16, 64, dtype=torch.bfloat16, device=DEV)
+    a[0, 5, 3] = 1.9921875 * 2.0 ** 63
+    b = torch.full((1, n, 16), 2.0 ** -20, dtype=torch.bfloat16, device=DEV)
+    scale = torch.tensor([1.003], device=DEV)
+    got = torch.zeros(m, n, dtype=torch.bfloat16, device=DEV)
+    ids = torch.zeros(m, dtype=torch.int32, device=DEV)
+    ops.LowRankAdd(got, None, x, a, b, ids, scale=scale)
+    check(got, x, None, a, b, scale, ids)
+
+
+@gpu
 @pytest.mark.parametrize("m,n", [(60, 64), (1300, 16384)])
 def test_values_that_are_not_finite_stay_in_their_token(m, n):
     x, base, a, b, scale, ids = case(m, n, 128, 16, 3, torch.bfloat16)
