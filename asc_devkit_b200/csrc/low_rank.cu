@@ -16,7 +16,9 @@
 //
 // The inner product is a sum in fp32; for the second product it is split into two 16-bit terms, hi = cast(v), lo = cast(v - hi), after
 // each token's row was multiplied by a power of two that keeps both inside the type's range (range_shift).  What the split drops is below
-// 2^-16 (bf16) or 2^-22 (fp16) of the row's largest value: the result carries one visible rounding, the one to dst's type.
+// 2^-16 (bf16) or 2^-22 (fp16) of the value, a 2^8-th or less of what x, A and base lost when they were rounded to their type; beside the result's own
+// rounding it shows only where terms of the sum cancel by more than that.  A third term keeps all 24 bits in bf16 and was measured: us, two / three
+// terms, 32 tokens of rank 16 7.1 / 7.5, 256 of rank 128 24.4 / 27.2, 8192 tokens of 4096 x 4096 at rank 64 63 / 67, at rank 128 79 / 88.
 #include "experts.cuh"
 #include "low_rank.cuh"
 #include "sm100_ptx.cuh"

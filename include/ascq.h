@@ -500,7 +500,8 @@ ascq_status ascq_matmul_w4a16(void* C, ascq_dtype cT, const void* A, ascq_dtype 
  * contiguous; A and B contiguous), adapterIds [M] of idT = int32 or int64 in any order, scale fp32 [L] or NULL (1).  A token
  * whose number is outside [0, L) keeps base[t].  Values that are not finite reach only the tokens of their own x row or
  * adapter, and come out as values that are not finite (an infinity in B may come out as NaN).  base may be dst itself (same
- * pitch) or NULL (0).  Both products accumulate in fp32 and the inner one is not rounded to T in between.
+ * pitch) or NULL (0).  Both products accumulate in fp32.  The inner one enters the second as two values
+ * of T, hi + lo: 2^-16 (bfloat16_t) or 2^-22 (half) of each inner product is lost there, where rounding it to T would lose 2^-8 or 2^-11.
  * N % 8 == 0, K % 8 == 0, both at most 2^30, r % 8 == 0, r <= 128, L <= 1023; tensors 16-byte aligned.
  * workspace: ascq_low_rank_add_workspace_size(M, N, K, r, L) bytes (0 for small calls), 16-byte aligned, private to this call until the
  * stream reaches the end of it.
