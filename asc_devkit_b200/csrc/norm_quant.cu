@@ -159,6 +159,10 @@ __device__ __forceinline__ int mx_exponent(float amax, float rstd, float rstdLo,
 }
 // 2^-e for e in [-127, 127]; 2^-127 is a subnormal
 __device__ __forceinline__ float exp2_neg(int e) { return e == 127 ? __uint_as_float(0x00400000u) : __uint_as_float(static_cast<uint32_t>(127 - e) << 23); }
+// Whether a block with shared exponent e takes one multiplication, by f = rstd * 2^-e: no |y| that has a code other than 0 is near fp32's
+// subnormals, nor, with f below 2^100, an |h * gamma| that has a normal one.  (Beyond is f only where epsilon and the row are tiny: rstd is at most 2^10 for epsilon
+// = 1e-6.)
+__device__ __forceinline__ bool single_factor(int e, float f) { return e > -80 && e < 80 && f < 1.2676506002282294e30f; }
 
 // Codes on the right side of a tie.  v = fl(fl(h * gamma) * fl(rstd * 2^-e)) is within 2.5 units in the last place of y * 2^-e; only a v
 // closer than that to the middle between two codes can be cast to the wrong one, and four units are looked at: one element in 116,000.
@@ -236,8 +240,8 @@ __device__ __forceinline__ Sum2 rstd_of(Sum2 sum, float n, float epsilon)
     const float q = __fdiv_rn(sum.hi, n);
     const float ql = __fdiv_rn(__fadd_rn(fmaf(-q, n, sum.hi), sum.lo), n);
     const Sum2 v = add_exact(Sum2{q, ql}, Sum2{epsilon, 0.f});
-    const float r = __frsqrt_rn(v.hi), t = __fmul_rn(r, r), tl = fmaf(r, r, -t);
-    const float e = fmaf(-v.lo, t, fmaf(-v.hi, tl, fmaf(-v.hi, t, 1.0f)));
+    const float r = __frsqrt_rn(v.hi), s = __fmul_rn(v.hi, r), sl = fmaf(v.hi, r, -s);  // (r * r would overflow for an epsilon below 2^-128)
+    const float e = fmaf(__fmul_rn(-v.lo, r), r, fmaf(-sl, r, fmaf(-s, r, 1.0f)));
     return Sum2{r, 0.5f * r * e};
 }
 
@@ -401,9 +405,9 @@ template <typename T, typename G, int OUT, int NV> __global__ void __launch_boun
                     const bool ok = finite_f32(__fmul_rn(amax, rstd));
                     const int e = mx_exponent(amax, rstd, st.rstdLo, out_emax(OUT));
                     uint32_t c[4];
-                    if (__builtin_expect(ok && e > -80 && e < 80, 1)) {
-                        // rstd * 2^-e is exact: one multiplication gives what y and its scaling would
-                        const float f = __fmul_rn(rstd, exp2_neg(e));
+                    const float f = __fmul_rn(rstd, exp2_neg(e));
+                    if (__builtin_expect(ok && single_factor(e, f), 1)) {
+                        // f is exact: one multiplication gives what y and its scaling would
 #pragma unroll
                         for (int j = 0; j < 4; ++j) mul2_rn(h[i][2 * j], h[i][2 * j + 1], f, f);
                         if constexpr (Tie<OUT>::kLooked) {
@@ -556,7 +560,7 @@ template <typename T, typename G> __global__ void __launch_bounds__(256) norm_an
             const bool ok = finite_f32(__fmul_rn(amax, rstd));
             const int e = mx_exponent(amax, rstd, st.rstdLo, out_emax(a.out));
             float v = __fmul_rn(y, exp2_neg(e));
-            if (ok && e > -80 && e < 80 && c < a.n) {
+            if (ok && single_factor(e, __fmul_rn(rstd, exp2_neg(e))) && c < a.n) {
                 if (a.out == kOutE4M3 && Tie<kOutE4M3>::distance(v) <= Tie<kOutE4M3>::kNear)
                     v = Tie<kOutE4M3>::settle(h, to_f32<G>(gamma[c]), rstd, st.rstdLo, exp2_neg(e));
                 if (a.out == kOutE5M2 && Tie<kOutE5M2>::distance(v) <= Tie<kOutE5M2>::kNear)

@@ -204,6 +204,42 @@ def test_mx_codes_next_to_a_tie(out, dt, place):
 
 
 @gpu
+@pytest.mark.parametrize("pitch", [0, 5])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("out", [L.DT_FP8_E4M3, L.DT_FP8_E5M2, L.DT_FP4X2_E2M1])
+def test_small_epsilon_and_blocks_far_below_the_row(out, dt, pitch):
+    """Rows of 1e-20 with blocks down to fp32's last normal numbers (and zeros) under an epsilon of 1e-36: rstd is 2^59.8, and for the smaller
+    blocks rstd * 2^-e alone would be beyond fp32."""
+    x, _, g = inputs(6, 512, dt, residual=False, pitch=pitch)
+    factor = torch.exp2(-111.0 - torch.arange(16, device=DEV)).repeat(6, 1)
+    factor[:, 0] = 1e-20
+    x.copy_((x.float().reshape(6, 16, 32) * factor[..., None]).reshape(6, 512))
+    x[:, 5::32] = 0
+    check(x, None, g, out, run(x, None, g, out, eps=1e-36), eps=1e-36)
+
+
+@gpu
+@pytest.mark.parametrize("pitch", [0, 5])
+@pytest.mark.parametrize("out", [L.DT_FP8_E4M3, L.DT_FP8_E5M2])
+def test_codes_next_to_a_tie_under_a_subnormal_epsilon(out, pitch):
+    """epsilon 2^-148, squares below 2^-196: rstd is 2^74 to 2^-49, and its remainder has to be a number."""
+    m, n = 4096, 1024
+    rng = torch.Generator().manual_seed(6)
+    wide = torch.zeros(m, n + pitch, device=DEV)
+    x = wide[:, :n]
+    x.copy_(torch.randint(1, 4097, (m, n), generator=rng).double() * 2.0 ** -110)
+    gamma = (2.0 ** 30 * (1 + 0.2 * torch.randn(n, generator=rng))).to(DEV)
+    dst, scale = torch.empty(m, n, dtype=torch.uint8, device=DEV), torch.empty(m, n // 32, dtype=torch.uint8, device=DEV)
+    ops.ResidualRmsNormQuant(dst, scale, x, gamma, 2.0 ** -148, dst_dtype=out)
+    y = x.double() * gamma.double() * 2.0 ** 74
+    v = (y.reshape(m, -1, 32) / torch.exp2(scale.double() - 127)[..., None]).reshape(m, n)
+    got = dst.view(torch.float8_e4m3fn if out == L.DT_FP8_E4M3 else torch.float8_e5m2).double()
+    low, high = to_grid(v * (1 - 2.0 ** -40), out), to_grid(v * (1 + 2.0 ** -40), out)
+    wrong = (got != low) & (got != high)
+    assert not wrong.any(), f"{int(wrong.sum())} codes on the wrong side"
+
+
+@gpu
 @pytest.mark.parametrize("n", [512, 511])
 def test_special_rows_int8(n):
     x, r, g = inputs(8, n, torch.bfloat16, residual=False)
