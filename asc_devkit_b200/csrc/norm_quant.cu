@@ -192,9 +192,15 @@ template <int OUT> struct Tie {
 
 // h = src + residual of an element whose v = fl(fl(h * gamma) * f) is known, formed again although residualOut may have taken the place of one of
 // the two: v / (gamma * f) is within 5 units of h's last place, so the lost one is the value of T nearest to it less the other, unless the
-// lost one is so small beside h that T has several values there.  False then, and in the same cases where both are in memory, so that a call
-// in place gives the bits of one that is not.  (Keeping the old values: in
+// lost one is so small beside h that T has several values there (see `separable`).  False then, and in the same cases where both are in memory, so that
+// a call in place gives the bits of one that is not.  (Keeping the old values: in
 // registers 171 us, in shared memory, which is taken from L1, 158; this way 143; 134 without a look at ties, with 16 times as many codes off.)
+template <typename T> __device__ __forceinline__ bool separable(float a, float b, float h)
+{
+    // bf16: off by 8 * 2^-24 |h| at most, T's values at a are 2^-8 |a| apart at least (2^-9 next to a power of two); fp16: 2^-11, 2^-12
+    constexpr float kLeast = std::is_same<T, __half>::value ? 0.00390625f : 0.00048828125f;
+    return sizeof(T) == 4 || fminf(fabsf(a), fabsf(b)) >= kLeast * fabsf(h);  // (fp32: h itself is in memory, in residualOut or as the two)
+}
 template <typename T> __device__ __forceinline__ bool row_sum(T x, T r, float v, float gamma, float f, bool overSrc, bool overRes, float& h)
 {
     float a = to_f32<T>(x), b = to_f32<T>(r);
@@ -205,9 +211,7 @@ template <typename T> __device__ __forceinline__ bool row_sum(T x, T r, float v,
         else b = to_f32<T>(narrow<T>(__fsub_rn(whole, a)));
     }
     h = __fadd_rn(a, b);
-    // bf16: off by 8 * 2^-24 |h| at most, T's values at a are 2^-8 |a| apart at least (2^-9 next to a power of two); fp16: 2^-11, 2^-12
-    constexpr float kLeast = std::is_same<T, __half>::value ? 0.00390625f : 0.00048828125f;
-    return fminf(fabsf(a), fabsf(b)) >= kLeast * fabsf(h);
+    return separable<T>(a, b, h);
 }
 
 // The int8 chain's multiplier 127 / amax, in two factors so that it does not overflow where amax is close to the smallest
@@ -542,8 +546,11 @@ template <typename T, typename G> __global__ void __launch_bounds__(256) norm_an
     for (uint32_t c0 = 0; c0 < a.n; c0 += blockDim.x) {
         const uint32_t c = c0 + threadIdx.x;
         float p = 0.f, h = 0.f;
+        bool settles = true;  // the vector kernel's rule
         if (c < a.n) {
-            h = res ? __fadd_rn(to_f32<T>(src[c]), to_f32<T>(res[c])) : to_f32<T>(src[c]);
+            const float x = to_f32<T>(src[c]), r = res ? to_f32<T>(res[c]) : 0.f;
+            h = res ? __fadd_rn(x, r) : x;
+            settles = !res || separable<T>(x, r, h);
             p = __fmul_rn(h, to_f32<G>(gamma[c]));
             if (resOut) resOut[c] = narrow<T>(h);
             if (normOut) normOut[c] = narrow<T>(__fmul_rn(p, rstd));
@@ -560,7 +567,7 @@ template <typename T, typename G> __global__ void __launch_bounds__(256) norm_an
             const bool ok = finite_f32(__fmul_rn(amax, rstd));
             const int e = mx_exponent(amax, rstd, st.rstdLo, out_emax(a.out));
             float v = __fmul_rn(y, exp2_neg(e));
-            if (ok && single_factor(e, __fmul_rn(rstd, exp2_neg(e))) && c < a.n) {
+            if (ok && single_factor(e, __fmul_rn(rstd, exp2_neg(e))) && settles && c < a.n) {
                 if (a.out == kOutE4M3 && Tie<kOutE4M3>::distance(v) <= Tie<kOutE4M3>::kNear)
                     v = Tie<kOutE4M3>::settle(h, to_f32<G>(gamma[c]), rstd, st.rstdLo, exp2_neg(e));
                 if (a.out == kOutE5M2 && Tie<kOutE5M2>::distance(v) <= Tie<kOutE5M2>::kNear)

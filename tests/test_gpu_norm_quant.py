@@ -204,6 +204,39 @@ def test_mx_codes_next_to_a_tie(out, dt, place):
 
 
 @gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("out", [L.DT_FP8_E4M3, L.DT_FP8_E5M2])
+@pytest.mark.parametrize("small", [False, True])
+def test_mx_codes_do_not_depend_on_the_outputs_or_the_alignment(small, out, dt):
+    """The same values with residualOut, without it, in the place of either operand and from unaligned rows: the same codes, also where one
+    operand is 0 or far below the other.  Whole numbers, whose squares add up exactly in any order; with small operands (2^-13 of whole
+    numbers) only the calls of one kernel are compared."""
+    m, n = 16384, 2048
+    g = torch.Generator(device=DEV).manual_seed(9)
+    def whole():
+        return torch.randint(1, 17, (m, n), generator=g, device=DEV) * (1 - 2 * torch.randint(0, 2, (m, n), generator=g, device=DEV))
+    x, r = whole().to(dt), whole().to(dt)
+    r *= 2.0 ** -13 if small else 1.0
+    r[torch.rand(m, n, generator=g, device=DEV) < 0.5] = 0
+    x[:, ::7] = 0
+    gamma = 1 + 0.2 * torch.randn(n, generator=g, device=DEV)
+    seen = {}
+    for place in ("own", "none", "src", "residual") + (() if small else ("unaligned",)):
+        dst, scale = torch.empty(m, n, dtype=torch.uint8, device=DEV), torch.empty(m, n // 32, dtype=torch.uint8, device=DEV)
+        xs, rs = x.clone(), r.clone()
+        if place == "unaligned":
+            wide = torch.empty(m, n + 1, dtype=dt, device=DEV)
+            wide[:, 1:] = x
+            xs = wide[:, 1:]
+        total = {"own": torch.empty_like(r), "src": xs, "residual": rs}.get(place)
+        ops.ResidualRmsNormQuant(dst, scale, xs, gamma, 2.0 ** -20, residual=rs, residualOut=total, dst_dtype=out)
+        seen[place] = dst, scale
+    for place, (dst, scale) in seen.items():
+        assert torch.equal(scale, seen["own"][1]), place
+        assert torch.equal(dst, seen["own"][0]), f"{place}: {int((dst != seen['own'][0]).sum())} other codes"
+
+
+@gpu
 @pytest.mark.parametrize("pitch", [0, 5])
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("out", [L.DT_FP8_E4M3, L.DT_FP8_E5M2, L.DT_FP4X2_E2M1])
