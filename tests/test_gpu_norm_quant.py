@@ -204,6 +204,49 @@ def test_mx_codes_next_to_a_tie(out, dt, place):
 
 
 @gpu
+@pytest.mark.parametrize("place", ["own", "none", "src", "residual", "unaligned", "alone"])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("out", [L.DT_FP8_E4M3, L.DT_FP8_E5M2, L.DT_FP4X2_E2M1])
+def test_block_exponents_next_to_a_power_of_two(out, dt, place):
+    """One element of a block decides its exponent, and gamma puts it within a few of its own steps of a power of two.  Whole numbers, n a power of
+    two: h and the sum are exact and rstd is known to 2^-44, so what is left is the rounding of h * gamma, half a step of fp32: the exponent has
+    to be the exact one wherever |y| is further than 2^-24 + 2^-40 from the power."""
+    n, eps, calls = 1024, 2.0 ** -20, 60
+    rng = torch.Generator().manual_seed(31)
+    wrong = sided = 0
+    for call in range(calls):
+        def whole(low, high, *shape):
+            return torch.randint(low, high + 1, shape, generator=rng) * (1 - 2 * torch.randint(0, 2, shape, generator=rng))
+        x, r = whole(1, 8, 1, n), whole(1, 8, 1, n)
+        at = torch.arange(32) * 32 + torch.randint(0, 32, (32,), generator=rng)
+        x[0, at], r[0, at] = 20 + whole(1, 9, 32), 9 + whole(1, 6, 32)   # h from 14 to 44
+        if place == "alone":
+            x, r = x + r, torch.zeros_like(r)
+        h = (x + r).double()
+        rstd = 1 / torch.sqrt((h * h).mean() + eps)
+        power = 2.0 ** torch.randint(-3, 4, (32,), generator=rng)
+        gamma = torch.full((n,), 2.0 ** -9)
+        near = (power / (h[0, at] * rstd)).float()
+        gamma[at] = near + torch.randint(-2, 3, (32,), generator=rng) * (torch.nextafter(near, 2 * near) - near)
+        xs, rs, gs = x.to(dt).to(DEV), r.to(dt).to(DEV), gamma.to(DEV)
+        if place == "unaligned":
+            wide = torch.empty(1, n + 1, dtype=dt, device=DEV)
+            wide[:, 1:] = xs
+            xs = wide[:, 1:]
+        total = {"own": torch.empty_like(rs), "src": xs, "residual": rs}.get(place)
+        dst = torch.empty(1, n // (2 if out == L.DT_FP4X2_E2M1 else 1), dtype=torch.uint8, device=DEV)
+        scale = torch.empty(1, 32, dtype=torch.uint8, device=DEV)
+        ops.ResidualRmsNormQuant(dst, scale, xs, gs, eps, residual=None if place == "alone" else rs, residualOut=total, dst_dtype=out)
+        y = (h * gamma.double() * rstd).reshape(32, 32).abs().amax(-1)
+        clear = (y / power - 1).abs() > 2.0 ** -24 + 2.0 ** -40
+        want = torch.floor(torch.log2(power)) - (y < power).double() - EMAX[out]
+        wrong += int(((scale[0].cpu().double() - 127 != want) & clear).sum())
+        sided += int((y < power).sum())
+    assert 32 * calls / 4 < sided < 32 * calls * 3 / 4   # both sides are met
+    assert wrong == 0, f"{wrong} exponents on the wrong side"
+
+
+@gpu
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("out", [L.DT_FP8_E4M3, L.DT_FP8_E5M2])
 @pytest.mark.parametrize("small", [False, True])
