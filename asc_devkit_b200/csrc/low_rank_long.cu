@@ -542,6 +542,9 @@ template <typename T, int NB> int resident_clusters(int size)
     return n;
 }
 
+// Devices that these kernels were ever launched (or captured) on: only there is a status word to read.
+std::atomic<bool> g_launched[kMaxDevices];
+
 template <typename T, int NB> ascq_status launch_long(const LowRankArgs& p, const LowRankScratch& o, unsigned tiles, cudaStream_t st)
 {
     static PerDeviceOnce once;
@@ -553,6 +556,7 @@ template <typename T, int NB> ascq_status launch_long(const LowRankArgs& p, cons
         for (int i = 0; i < 4; ++i) resident[dev][i].store(resident_clusters<T, NB>(1 << i), std::memory_order_relaxed);
         once.mark(dev);
     }
+    g_launched[dev].store(true, std::memory_order_relaxed);
     // K is split over a cluster so that the waves of clusters take the least time: a wave's chunks, and about ten more for its start and its end.  How many
     // tiles there are only the device knows; half of the adapters are taken to leave a tile partly filled.
     const int64_t chunks = (p.K + 63) / 64, expected = p.M / kRows + std::min(p.L + 1, p.M) / 2 + 1;
@@ -620,6 +624,7 @@ ascq_status low_rank_long(const LowRankArgs& p, bool half, const LowRankScratch&
 ascq_status low_rank_read_status(::CUstream_st* st)
 {
     int v = 0, zero = 0;
+    if (!g_launched[current_device()].load(std::memory_order_relaxed)) return ASCQ_OK;  // no copy and no wait for programs without adapters
     ASCQ_CUDA_CHECK(cudaMemcpyFromSymbolAsync(&v, g_low_rank_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st));
     ASCQ_CUDA_CHECK(cudaStreamSynchronize(st));
     if (v != 0) {

@@ -349,6 +349,43 @@ def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_exact(m, n, k, r,
         assert torch.equal(got, want)
 
 
+STATUS_COPIES = """
+import torch
+from torch.profiler import ProfilerActivity, profile
+from asc_devkit_b200 import ops
+
+def copies():
+    ops.MatmulStatus()
+    with profile(activities=[ProfilerActivity.CUDA]) as p:
+        for _ in range(5):
+            ops.MatmulStatus()
+    return sum(e.count for e in p.key_averages() if "Memcpy" in e.key and "DtoH" in e.key.replace(" ", "")) / 5
+
+torch.zeros(1, device="cuda:0")
+z = lambda *s: torch.zeros(*s, dtype=torch.float16, device="cuda:0")
+before = copies()
+ops.LowRankAdd(z(4, 16), None, z(4, 8), z(2, 8, 8), z(2, 16, 8), torch.zeros(4, dtype=torch.int32, device="cuda:0"))
+few = copies()
+ops.LowRankAdd(z(2000, 8192), None, z(2000, 4096), z(2, 16, 4096), z(2, 8192, 16), torch.zeros(2000, dtype=torch.int32, device="cuda:0"))
+print("copies", before, few, copies())
+"""
+
+
+@gpu
+def test_status_of_a_program_without_adapters_costs_what_it_did():
+    """ascq_matmul_status reads the status word of the adapters' kernels (a copy and a wait of its own) only after a call that launched them."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, "-c", STATUS_COPIES], cwd=root, capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0, out.stderr[-2000:]
+    before, few, after = (float(v) for v in out.stdout.split("copies")[1].split())
+    if after == 0:
+        pytest.skip("the profiler records no copies here")
+    assert before == 3 and few == 3 and after == 4, out.stdout   # int8 / half matmuls, MX matmuls, exchange; then the adapters
+
+
 @gpu
 def test_empty():
     e = lambda *s: torch.empty(*s, dtype=torch.float16, device=DEV)  # noqa: E731
