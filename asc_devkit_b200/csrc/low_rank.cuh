@@ -102,12 +102,6 @@ template <typename T> __device__ __forceinline__ uint4 pack8_sat(const float (&f
     }
     return make_uint4(r[0], r[1], r[2], r[3]);
 }
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr)
-{
-    float f;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(addr) : "memory");
-    return f;
-}
 __device__ __forceinline__ void st_cluster_v4(uint32_t addr, uint4 v)
 {
     asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");

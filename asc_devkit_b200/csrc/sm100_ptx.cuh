@@ -155,13 +155,6 @@ __device__ __forceinline__ void tma_load_2d(void* smemDst, const CUtensorMap* m,
         ::"r"(smem_u32(smemDst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
         : "memory");
 }
-__device__ __forceinline__ void tma_load_3d(void* smemDst, const CUtensorMap* m, uint64_t* bar, int c0, int c1, int c2)
-{
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-        ::"r"(smem_u32(smemDst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
-        : "memory");
-}
 
 // Untiled bulk copy global -> shared; both addresses 16-byte aligned, bytes a multiple of 16.
 // TMA store of one 2D box from shared memory (bulk async-group completion).  c0 (innermost) times the element size must

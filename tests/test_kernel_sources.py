@@ -39,3 +39,10 @@ def test_tensor_memory_is_taken_before_a_dependent_launch_is_let_in(path):
 def test_the_sources_hold_such_kernels():
     both = [name for path in SOURCES for name, body in kernels(path) if "tmem_alloc" in body and "launch_dependents" in body]
     assert {"low_rank_inner_kernel", "low_rank_outer_kernel"} <= set(both) and len(both) >= 3, both
+
+
+def test_every_device_helper_is_called():
+    text = "".join(re.sub(r"//[^\n]*", "", open(p).read()) for p in glob.glob(os.path.join(CSRC, "*")) if p.endswith((".cu", ".cuh", ".h", ".cpp")))
+    names = set(re.findall(r"__device__ __forceinline__ (?:const )?[\w:<>, ]+?[ *&]+(\w+)\(", text))
+    assert len(names) > 100
+    assert not [n for n in sorted(names) if len(re.findall(rf"\b{n}\b", text)) < 2]
