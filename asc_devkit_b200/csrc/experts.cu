@@ -617,7 +617,7 @@ extern "C" ascq_status ascq_expert_combine_grad(void* gradRows, float* gradWeigh
     if (rc != ASCQ_OK) return rc;
     if (!float_type(T)) return fail(ASCQ_ERR_UNSUPPORTED, "rows must be half, bfloat16_t or float");
     if (h < 0 || h > 0x7FFFFFFFll) return fail(ASCQ_ERR_INVALID_ARG, "h must be in [0, 2^31)");
-    if (tokens == 0 || (rows == 0 && !gradWeights)) return ASCQ_OK;
+    if (tokens == 0 || ((rows == 0 || h == 0) && !gradWeights)) return ASCQ_OK;  // (empty tensors have no address)
     if (!gradRows && !gradWeights) return fail(ASCQ_ERR_INVALID_ARG, "gradRows and gradWeights are both NULL");
     if ((h && !gradOut) || !rowOfSlot || (gradWeights && rows && h && !in)) return fail(ASCQ_ERR_INVALID_ARG, "gradOut, rows and rowOfSlot must not be NULL");
     const size_t es = dtype_size(T), N = static_cast<size_t>(tokens);

@@ -443,6 +443,13 @@ def test_combine_grad_refusals():
     assert call(dw=0x200001) == L.ERR_ALIGNMENT
 
 
+def test_combine_grad_of_empty_rows_is_no_error():
+    """Rows of no elements: nothing to write, and torch gives such tensors no address.  (No CUDA work: this runs without a GPU.)"""
+    grad = L.lib().ascq_expert_combine_grad
+    assert grad(None, None, None, None, L.DT_F16, P(0x500000), P(0x600000), 4, 2, 8, 0, None) == L.OK
+    assert grad(None, None, None, None, L.DT_F16, P(0x500000), P(0x600000), 4, 2, 0, 64, None) == L.OK
+
+
 def test_python_refusals():
     i32 = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
     with pytest.raises(TypeError, match="int32 or int64"):
