@@ -199,6 +199,24 @@ def test_infinite_inner_product_beside_large_finite_ones(m, n):
 
 
 @gpu
+@pytest.mark.parametrize("m,n,k", [(40, 136, 264), (2000, 8200, 3000)])
+def test_ranks_beyond_one_call(m, n, k):
+    """As the header says: a rank of 4 padded with zeros, one of 256 in two calls (each of which rounds its result)."""
+    x, base, a, b, scale, ids = case(m, n, k, 256, 3, torch.float16)
+    four, padded = (a[:, :4].contiguous(), b[:, :, :4].contiguous()), (torch.zeros_like(a[:, :8]), torch.zeros_like(b[:, :, :8]))
+    padded[0][:, :4], padded[1][:, :, :4] = four
+    got = torch.empty_like(base)
+    ops.LowRankAdd(got, base, x, padded[0].contiguous(), padded[1].contiguous(), ids, scale=scale)
+    check(got, x, base, *four, scale, ids)
+    first = torch.empty_like(base)
+    ops.LowRankAdd(first, base, x, a[:, :128].contiguous(), b[:, :, :128].contiguous(), ids, scale=scale)
+    check(first, x, base, a[:, :128], b[:, :, :128], scale, ids)
+    got.copy_(first)
+    ops.LowRankAdd(got, got, x, a[:, 128:].contiguous(), b[:, :, 128:].contiguous(), ids, scale=scale)
+    check(got, x, first, a[:, 128:], b[:, :, 128:], scale, ids)
+
+
+@gpu
 def test_result_that_overflows_saturates():
     x = torch.full((2, 8), 100.0, dtype=torch.float16, device=DEV)
     a, b = torch.full((1, 8, 8), 10.0, dtype=torch.float16, device=DEV), torch.full((1, 8, 8), 10.0, dtype=torch.float16, device=DEV)
