@@ -277,7 +277,8 @@ struct DispatchArgs {
 template <typename V> constexpr int dispatch_vecs() { return sizeof(V) == 16 ? 4 : sizeof(V) == 4 ? 8 : 16; }
 
 // A warp takes a segment of a token's row: it reads the segment once and writes it to each of the token's rows.  What bounds it is HBM's
-// write side: 8192 tokens x 8 int8 rows of 7168 bytes in 84 us = 6.3 TB/s of 0.53 GB.
+// write side: 8192 tokens x 8 int8 rows of 7168 bytes in 84 us = 6.3 TB/s of 0.53 GB; E4M3 rows with their 224 scale bytes 88 us,
+// packed fp4 rows with theirs 49 us (of 0.28 GB).  Rows of an odd number of bytes move in single bytes: 7167 of them 154 us.
 template <typename V> __global__ void __launch_bounds__(256) dispatch_kernel(const DispatchArgs a)
 {
     constexpr int kDispatchVecs = dispatch_vecs<V>();
@@ -411,7 +412,8 @@ template <typename T, int VEC> __global__ void __launch_bounds__(256) combine_ke
 // One CTA per token.  A thread requests its vectors of kGradRows of the token's rows together; gradOut's row is read again (from
 // L1 or L2) for the next kGradRows.  What bounds it is how many requests an SM has in flight, so the rows per step trade against
 // occupancy: at 8192 tokens, k = 8, h = 4096 in bf16 (177 us at the copy rate) 187 us with 4 rows and 64 registers, 213 with 2 rows
-// and 40, 196 with 4 rows and 80, 249 with 8 rows and 120; CTAs of 128 threads rather than 256 (193 us) or 64 (198 us).
+// and 40, 196 with 4 rows and 80, 249 with 8 rows and 120; CTAs of 128 threads rather than 256 (193 us) or 64 (198 us).  (All on one box;
+// on another the form taken has 193 us.  Rows of odd sizes: 4096 x 4 x 2048 25 us, x 2047 55, x 2046 61.)
 constexpr int kGradRows = 4, kGradThreads = 128;
 
 template <typename T, int VEC> __global__ void __launch_bounds__(kGradThreads, 8) combine_grad_kernel(const CombineArgs a)

@@ -8,8 +8,8 @@
 //
 // What bounds it: HBM.  With bf16 tensors and residualOut an element costs 2 + 2 bytes read, 2 + 1 written.  A CTA owns whole rows and
 // keeps a row in registers between the reduction and the quantisation, so each byte moves once; the next row is requested before the
-// reduction.  bf16 [16384, 7168] to e4m3: 143 us = 5.8 TB/s, 0.90 of the measured copy rate (134 us without the look at ties;
-// before that, 164 without the early request).  For int8 the row's maximum needs no second reduction: max|y| = rstd * max|h * gamma|, so sum(h^2) and max|h * gamma| go through the same
+// reduction.  bf16 [16384, 7168] to e4m3: 141 us = 5.9 TB/s, 0.91 of the measured copy rate (134 us without the look at ties;
+// before that, 164 without the early request); to e2m1 130 us; [2048, 16384] to int8 38 us, to e4m3 45.  For int8 the row's maximum needs no second reduction: max|y| = rstd * max|h * gamma|, so sum(h^2) and max|h * gamma| go through the same
 // shuffles and the same barrier, and RINT(y * 127 / max|y|) = RINT((h * gamma) * (127 / max|h * gamma|)) does not need rstd.
 #include "elementwise.cuh"
 
@@ -167,7 +167,7 @@ __device__ __forceinline__ float exp2_neg(int e) { return e == 127 ? __uint_as_f
 __device__ __forceinline__ bool single_factor(int e, float f) { return e > -80 && e < 80 && f < 1.2676506002282294e30f; }
 
 // Codes on the right side of a tie.  v = fl(fl(h * gamma) * fl(rstd * 2^-e)) is within 2.5 units in the last place of y * 2^-e; only a v
-// closer than that to the middle between two codes can be cast to the wrong one, and four units are looked at: one element in 116,000.
+// closer than that to the middle between two codes can be cast to the wrong one, and four units are looked at: one element in 116,000 (E5M2: in 233,000).
 template <int OUT> struct Tie {
     static constexpr bool kLooked = OUT == kOutE4M3 || OUT == kOutE5M2;  // (fp4 goes through bfloat16, whose own rounding is part of its definition)
     static constexpr int kDrop = OUT == kOutE4M3 ? 20 : 21;              // mantissa bits that the cast drops; the middle is 100...0
@@ -196,7 +196,7 @@ template <int OUT> struct Tie {
 // the two: v / (gamma * f) is within 5 units of h's last place, so the lost one is the value of T nearest to it less the other, unless the
 // lost one is so small beside h that T has several values there (see `separable`).  False then, and in the same cases where both are in memory, so that
 // a call in place gives the bits of one that is not.  (Keeping the old values: in
-// registers 171 us, in shared memory, which is taken from L1, 158; this way 143; 134 without a look at ties, with 16 times as many codes off.)
+// registers 171 us, in shared memory, which is taken from L1, 158; this way 141 to 143; 134 without a look at ties, with ten times as many codes off.)
 template <typename T> __device__ __forceinline__ bool separable(float a, float b, float h)
 {
     // bf16: off by 8 * 2^-24 |h| at most, T's values at a are 2^-8 |a| apart at least (2^-9 next to a power of two); fp16: 2^-11, 2^-12
@@ -445,7 +445,7 @@ template <typename T, typename G, int OUT, int NV> __global__ void __launch_boun
 
 // int8 from widths or tensors that 16-byte vectors do not fit: a CTA holds a row as NE groups of VEC elements per thread (2 where everything is even, else 1),
 // neighbouring threads neighbouring groups, all of them requested before the first is used.  The same arithmetic.  bf16 with residual and sum: [2048, 7167] 46 us
-// (62 us an element at a time in two passes; [2048, 7168] takes 17.6 us on vectors), [4096, 1023] 14 us (20.5; 7.7), [4096, 1022] 10.4 us.
+// (62 us an element at a time in two passes; [2048, 7168] takes 16 us on vectors), [4096, 1023] 14 us (20.5; 7.3), [4096, 1022] 10 us.
 template <typename T, int VEC> __device__ __forceinline__ Pack<T, VEC> load_group(const T* p)
 {
     if constexpr (sizeof(T) * VEC >= 4) return load_pack<T, VEC, true>(p);
@@ -613,7 +613,8 @@ template <typename T, typename G, int OUT> cudaError_t launch_norm_rows(const No
     const unsigned block = ((nvec + nv - 1) / nv + 31) / 32 * 32;
     // About 1280 threads per SM, each CTA walking over its rows with the next one on its way.  Measured: bf16 [16384, 7168] to e4m3 (448
     // threads) 199 / 141 / 170 us with 1 / 2 / 3 CTAs per SM; half [1031, 5120] to int8 (320 threads) 8.2 / 8.1 / 5.6 / 5.5 / 5.6 us with
-    // 1 to 5.  Rows above 8192 elements need 128 registers a thread: one CTA.
+    // 1 to 5.  Rows above 8192 elements need 128 registers a thread, so that one CTA is all an SM holds: [2048, 16384] to int8 38 us = 0.94 of the
+    // copy rate, to e4m3 45 us = 0.81.
     const unsigned perSm = nv >= 4 ? 1u : std::max(1u, 1280u / block);
     const unsigned grid = std::min<uint64_t>(a.m, static_cast<uint64_t>(sm_count()) * perSm);
     if (nv == 1) return launch_norm(norm_rows_kernel<T, G, OUT, 1>, grid, block, st, a);
