@@ -191,7 +191,7 @@ template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_ra
             }
             for (int i = group; i < n; i += 2) {
                 const int s = i % C::kStages;
-                if (i >= C::kStages && !(ok = mbar_wait_bounded(&emptyBar[s], (i / C::kStages - 1) & 1, &abortFlag))) break;
+                if (i >= C::kStages && !(ok = mbar_wait_bounded<false>(&emptyBar[s], (i / C::kStages - 1) & 1, &abortFlag))) break;
                 const bool kIn = (first + i) * 64 + piece * 8 < p.K;
                 const uint32_t slot = at + s * C::kStageBytes;
                 // a row without a token keeps whatever the slot holds: a row of A times it is a row of D that nobody reads
@@ -215,7 +215,7 @@ template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_ra
                 int i = 0;
                 for (; i < loads; ++i) {
                     const int s = i % C::kStages;
-                    if (i >= C::kStages && !(ok = mbar_wait_bounded(&emptyBar[s], (i / C::kStages - 1) & 1, &abortFlag))) break;
+                    if (i >= C::kStages && !(ok = mbar_wait_bounded<false>(&emptyBar[s], (i / C::kStages - 1) & 1, &abortFlag))) break;
                     // rows behind the adapter's rank are the next adapter's (or zeros): columns of D that finish_rows leaves out
                     mbar_arrive_expect_tx(&aBar[s], C::kABytes);
                     tma_load_2d(ring + s * C::kStageBytes + kAtomBytes, &mapA, &aBar[s], (first + i) * 64, adapter * p.r);
@@ -227,7 +227,7 @@ template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_ra
             constexpr uint32_t idesc = idesc_f16(kRows, R, std::is_same<T, __half>::value ? 0 : 1);
             for (int i = 0; i < n && ok; ++i) {
                 const int s = i % C::kStages;
-                if (!(ok = mbar_wait_bounded(&aBar[s], (i / C::kStages) & 1, &abortFlag) && mbar_wait_bounded(&fullBar[s], (i / C::kStages) & 1, &abortFlag))) break;
+                if (!(ok = mbar_wait_bounded<false>(&aBar[s], (i / C::kStages) & 1, &abortFlag) && mbar_wait_bounded<false>(&fullBar[s], (i / C::kStages) & 1, &abortFlag))) break;
                 tc_fence_after();
                 const uint32_t at = smem_u32(ring) + s * C::kStageBytes;
                 const uint64_t descX = smem_desc_sw128(at), descA = smem_desc_sw128(at + kAtomBytes);
@@ -247,7 +247,7 @@ template <typename T, int NB> __global__ void __launch_bounds__(kThreads) low_ra
         const int share = kRows / clusterCtas;
         cluster_wait();  // every CTA of the cluster has started (they arrived at the top)
         if (warp < 4) {
-            if (n > 0) ok = ok && mbar_wait_bounded(&doneBar, 0, &abortFlag);
+            if (n > 0) ok = ok && mbar_wait_bounded<false>(&doneBar, 0, &abortFlag);
             __syncwarp();
             tc_fence_after();
             const uint32_t to = mapa_u32(smem_u32(part + (rank * share + threadIdx.x % share) * kPitch), threadIdx.x / share);
@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(kOuterThreads, NB <= 8 ? 2 : 1) low_rank_outer
                 __syncwarp();  // the warp has read the values of block n - 1 out of the slot that is filled now
                 request(b + 2);
                 cp_wait<2>();
-                ok = mbar_wait_bounded(&outBar[n & 1], (n >> 1) & 1, &abortFlag);
+                ok = mbar_wait_bounded<false>(&outBar[n & 1], (n >> 1) & 1, &abortFlag);
                 // base's values of block n, copied by the warp's lanes, are there for all of them; and the lanes give up together
                 if (!(ok = __all_sync(0xFFFFFFFFu, ok))) break;
                 __syncwarp();
@@ -439,7 +439,7 @@ __global__ void __launch_bounds__(kOuterThreads, NB <= 8 ? 2 : 1) low_rank_outer
         } else if (elect_one()) {
             constexpr uint32_t idesc = idesc_f16(kRows, kBlockCols, std::is_same<T, __half>::value ? 0 : 1);
             const int steps = (p.r + 15) / 16;
-            auto done = [&](uint32_t n) { return mbar_wait_bounded(&outBar[n & 1], (n >> 1) & 1, &abortFlag); };  // block n's MMAs
+            auto done = [&](uint32_t n) { return mbar_wait_bounded<false>(&outBar[n & 1], (n >> 1) & 1, &abortFlag); };  // block n's MMAs
             int asked = 0;  // blocks of B asked for
             bool begun = false;
             auto load_b = [&](int b) {
@@ -461,14 +461,14 @@ __global__ void __launch_bounds__(kOuterThreads, NB <= 8 ? 2 : 1) low_rank_outer
                     for (int ka = 0; ka < C::kAtoms; ++ka) tma_load_2d(sV + (h * C::kAtoms + ka) * kAtomBytes, &mapV, &vBar, h * VP + ka * 64, start);
                 load_b(0);
                 load_b(1);
-                ok = mbar_wait_bounded(&vBar, segment & 1, &abortFlag);
+                ok = mbar_wait_bounded<false>(&vBar, segment & 1, &abortFlag);
             }
             for (int b = 0; b < blocks && ok; ++b) {
                 const uint32_t n = it + b;
                 if (b > 0 && !(ok = done(n - 1))) break;
                 load_b(b + 2);
-                if (!(ok = mbar_wait_bounded(&bBar[n % 3], (n / 3) & 1, &abortFlag))) break;
-                if (n >= 2 && !(ok = mbar_wait_bounded(&freeBar[n & 1], ((n >> 1) & 1) ^ 1, &abortFlag))) break;
+                if (!(ok = mbar_wait_bounded<false>(&bBar[n % 3], (n / 3) & 1, &abortFlag))) break;
+                if (n >= 2 && !(ok = mbar_wait_bounded<false>(&freeBar[n & 1], ((n >> 1) & 1) ^ 1, &abortFlag))) break;
                 tc_fence_after();
                 const uint32_t v = smem_u32(sV), w = smem_u32(sB) + (n % 3) * C::kBBytes;
                 for (int h = 0; h < 2; ++h)

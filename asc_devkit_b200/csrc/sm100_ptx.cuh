@@ -74,7 +74,9 @@ __device__ __forceinline__ void raise_abort(volatile int* abortFlag)
     }
 }
 
-__device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity, volatile int* abortFlag)
+// PAIR false: for kernels whose CTAs wait for nothing of one another in these loops, in clusters of any size.  The partner's flag is left
+// alone: unless a cluster barrier has been passed, nothing says that the partner runs yet and its shared memory may be written.
+template <bool PAIR = true> __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity, volatile int* abortFlag)
 {
     if (mbar_try_wait(bar, parity)) return true;
     const long long t0 = clock64();
@@ -83,7 +85,8 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
         if ((++spins & 0x3Fu) == 0) {
             if (*abortFlag) return false;
             if (clock64() - t0 > c_waitCycles) {
-                raise_abort(abortFlag);
+                if constexpr (PAIR) raise_abort(abortFlag);
+                else *abortFlag = 1;
                 return false;
             }
         }

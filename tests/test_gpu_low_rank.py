@@ -339,7 +339,7 @@ def test_a_call_on_another_stream_takes_its_own_workspace(m, n, k, monkeypatch):
 
 
 @gpu
-@pytest.mark.parametrize("m,n,k,r,lo,span", [(1700, 4104, 8200, 16, 3, 1), (4700, 4096, 264, 64, 16, 300), (1400, 4096, 5000, 128, 2, 1030)])
+@pytest.mark.parametrize("m,n,k,r,lo,span", [(1700, 4104, 8200, 16, 3, 1), (4700, 4096, 264, 64, 16, 300), (1400, 4096, 5000, 128, 2, 1030), (8192, 4096, 4096, 64, 16, 700)])
 @pytest.mark.parametrize("chunks,blocks", [(0, -1), (3, -1), (-1, 0), (-1, 2)])
 def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_exact(m, n, k, r, lo, span, chunks, blocks):
     """Loads of A (first launch) or B (second) that are never made, a wait limit of about ten milliseconds: every role leaves

@@ -41,6 +41,16 @@ def test_the_sources_hold_such_kernels():
     assert {"low_rank_inner_kernel", "low_rank_outer_kernel"} <= set(both) and len(both) >= 3, both
 
 
+def test_only_kernels_behind_a_cluster_barrier_write_a_partners_abort_flag():
+    """A wait that gives up may raise the flag in the partner's shared memory only where a cluster barrier was passed first; until then nothing says that
+    the partner runs."""
+    for path in SOURCES:
+        for name, body in kernels(path):
+            waits = [m.start() for m in re.finditer(r"mbar_wait_bounded(_\w+)?\(", body)]  # (the form without a partner is mbar_wait_bounded<false>)
+            if waits:
+                assert 0 <= body.find("cluster_wait();") < waits[0], name
+
+
 def test_every_device_helper_is_called():
     text = "".join(re.sub(r"//[^\n]*", "", open(p).read()) for p in glob.glob(os.path.join(CSRC, "*")) if p.endswith((".cu", ".cuh", ".h", ".cpp")))
     names = set(re.findall(r"__device__ __forceinline__ (?:const )?[\w:<>, ]+?[ *&]+(\w+)\(", text))
