@@ -55,7 +55,7 @@ def _workspace(need: int, device, stream: Optional[torch.cuda.Stream]) -> torch.
     kernels run on: the caching allocator hands a freed block only to later work on the stream it was taken for, so the
     next owner is ordered behind these kernels.  (A block of another stream's pool may still be read by that stream's work.)"""
     size = max(int(need), 256)
-    if stream is None:
+    if stream is None or stream.cuda_stream == torch._C._cuda_getCurrentRawStream(stream.device_index):
         return torch.empty(size, dtype=torch.uint8, device=device)
     with torch.cuda.stream(stream):
         return torch.empty(size, dtype=torch.uint8, device=device)
@@ -181,10 +181,11 @@ def _launch(fn, dev: int, stream: Optional[torch.cuda.Stream], *args):
         L.check(rc)
 
 
-def _check_sizes(*sizes: int):
-    """The C ABI takes these as 32-bit numbers, and ctypes would drop the bits above."""
-    if max(sizes) > 0x7FFFFFFF:
-        raise ValueError(f"a size of {max(sizes)} is beyond 2^31 - 1, the most that one call takes")
+_INT_MAX = 0x7FFFFFFF  # the C ABI takes sizes as 32-bit numbers, and ctypes would drop the bits above
+
+
+def _too_large(*sizes: int):
+    raise ValueError(f"a size of {max(sizes)} is beyond 2^31 - 1, the most that one call takes")
 
 
 _MX_TARGETS = {L.DT_FP8_E4M3: 1, L.DT_FP8_E5M2: 1, L.DT_FP4X2_E2M1: 2}
@@ -217,7 +218,8 @@ def ResidualRmsNormQuant(dstTensor: torch.Tensor, scaleOut: torch.Tensor, srcTen
             raise ValueError("dstTensor must hold one byte per code (fp4: per two codes)")
         if scaleOut.element_size() != 1 or scaleOut.numel() != m * (n // 32):
             raise ValueError("scaleOut must hold one byte per 32 elements")
-    _check_sizes(m, n)
+    if m > _INT_MAX or n > _INT_MAX:
+        _too_large(m, n)
     dev = _cuda_index(srcTensor)
     (sp, ls), (rp, lr), (ro, lro), (no, lno) = _rows(srcTensor, dev), _rows(residual, dev), _rows(residualOut, dev), _rows(normOut, dev)
     _launch(L.lib().ascq_residual_rms_norm_quant, dev, stream, _whole(dstTensor, dev), dst_dtype, _whole(scaleOut, dev), ro, no, sp, rp, _whole(gamma, dev),
@@ -465,7 +467,8 @@ def ExpertSort(counts: torch.Tensor, rowOfSlot: torch.Tensor, expertIds: torch.T
         raise ValueError("rowOfSlot must be int32 with one element per slot")
     if slotOfRow is not None and (slotOfRow.dtype != torch.int32 or slotOfRow.numel() != n):
         raise ValueError("slotOfRow must be int32 with one element per slot")
-    _check_sizes(counts.numel())
+    if counts.numel() > _INT_MAX:
+        _too_large(counts.numel())
     dev = _cuda_index(expertIds)
     _launch(L.lib().ascq_expert_sort, dev, stream, _whole(counts, dev), _whole(rowOfSlot, dev), _whole(slotOfRow, dev), _whole(expertIds, dev), code, n,
             counts.numel())
@@ -476,7 +479,8 @@ def _slots(rowOfSlot: torch.Tensor, tokens: int) -> int:
     if rowOfSlot.dtype == torch.int32 and rowOfSlot.dim() == 2:
         t, k = rowOfSlot.shape
         if t == tokens and k > 0:
-            _check_sizes(k)
+            if k > _INT_MAX:
+                _too_large(k)
             return k
     raise ValueError("rowOfSlot must be int32 [tokens, k]")
 
@@ -572,7 +576,8 @@ def LowRankAdd(dstTensor: torch.Tensor, base: Optional[torch.Tensor], X: torch.T
     if scale is not None and (scale.dtype != torch.float32 or scale.dim() != 1 or scale.numel() != Lo):
         raise ValueError("scale must be float32 [L]")
     code, idc = dtype_code(X), _id_code(adapterIds)
-    _check_sizes(M, N, K, r, Lo)
+    if max(M, N, K, r, Lo) > _INT_MAX:
+        _too_large(M, N, K, r, Lo)
     dev = _cuda_index(X)
     if workspace is None:
         need = L.lib().ascq_low_rank_add_workspace_size(M, N, K, r, Lo)
