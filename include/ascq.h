@@ -503,7 +503,7 @@ ascq_status ascq_matmul_w4a16(void* C, ascq_dtype cT, const void* A, ascq_dtype 
  * pitch) or NULL (0).  Both products accumulate in fp32.  The inner one enters the second as two values
  * of T, hi + lo: 2^-16 (bfloat16_t) or 2^-22 (half) of each inner product is lost there, where rounding it to T would lose 2^-8 or 2^-11.
  * N % 8 == 0, K % 8 == 0, both at most 2^30, r % 8 == 0, r <= 128, L <= 1023; tensors 16-byte aligned.  Other ranks: pad A's
- * rows and B's columns with zeros once (finite x: the same bits); above 128, one call for each 128 of them, dst as the next one's base.
+ * rows and B's columns with zeros once (they add nothing while x is finite); above 128, one call for each 128 of them, dst as the next one's base.
  * workspace: ascq_low_rank_add_workspace_size(M, N, K, r, L) bytes (0 for small calls), 16-byte aligned, private to this call until the
  * stream reaches the end of it.
  */
