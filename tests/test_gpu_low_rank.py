@@ -367,6 +367,32 @@ def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_exact(m, n, k, r,
         assert torch.equal(got, want)
 
 
+@gpu
+@pytest.mark.parametrize("m,n,k,r,lo,span", [(1700, 4104, 8200, 16, 3, 1), (1400, 4096, 5000, 128, 2, 1030), (8192, 4096, 4096, 64, 16, 700)])
+@pytest.mark.parametrize("limit", [1, 3000, 30000])
+def test_a_limit_shorter_than_ordinary_waits(m, n, k, r, lo, span, limit):
+    """CTAs give up with their own copies and MMAs under way, at any point of their loops; the call after it, with the ordinary limit, is exact."""
+    x, base, a, b, scale, ids = case(m, n, k, r, lo, torch.bfloat16, span)
+    want, got = torch.empty_like(base), torch.empty_like(base)
+    ops.LowRankAdd(want, base, x, a, b, ids, scale=scale)
+    ops.MatmulStatus()
+    ops.SetWaitLimitCycles(limit)
+    try:
+        for _ in range(3):
+            ops.LowRankAdd(got, base, x, a, b, ids, scale=scale)
+            try:
+                ops.MatmulStatus()
+                assert torch.equal(got, want)  # nobody gave up
+            except ops.AscqError as e:
+                assert e.status == L.ERR_TIMEOUT
+    finally:
+        ops.SetWaitLimitCycles(0)
+    got.fill_(3.0)
+    ops.LowRankAdd(got, base, x, a, b, ids, scale=scale)
+    ops.MatmulStatus()
+    assert torch.equal(got, want)
+
+
 STATUS_COPIES = """
 import torch
 from torch.profiler import ProfilerActivity, profile
